@@ -8,6 +8,8 @@ Modules:
   ops       the wgsl-ops.js closures (op(ctx, ...) -> dispatch(...)), fp32, reference layouts
   blocks    the fused blocks (resnet, conv, groupnorm, attn, cross-attn, block-full, tembed) and
             their runXBench drivers with the reference's result schema
+  layers    attention-layer operators for batches whose requests differ (adapters per row, head norms with
+            axial rotation, attention over encoder states with lengths and masks)
   unet      the SD-Turbo U-Net plan (CUDA-graph replay of the whole forward)
 
 There is no CPU fallback: importing this package on a machine without a CUDA device works (so the
@@ -82,6 +84,12 @@ SIGNATURES = {
     "di_gn_table_nhwc": (_I, [_P, _I, _P, _I, _P, _I, _I, _I, _I, _F, _P, _P, _P]),
     "di_conv3x3_nhwc_gn": (_I, [_P, _I, _P, _I, _P, _I, _I, _I, _I, _P, _I, _P, _P, _P, _P, _I, _P]),
     "di_attention": (_I, [_P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I]),
+    "di_linear_lora_workspace": (_SZ, [_P, _I, _I, _I, _I, _I]),
+    "di_linear_lora": (_I, [_P, _I, _P, _LL, _I, _I, _P, _I, _P, _P, _I, _I, _P, _P, _P, _P, _LL, _I, _P, _LL, _P, _SZ]),
+    "di_qk_norm_rope": (_I, [_P, _I, _P, _LL, _I, _P, _LL, _I, _I, _I, _P, _P, _F, _P, _I, _I, _P, ctypes.c_double, _I, _P,
+                             _LL, _P, _LL]),
+    "di_cross_attention_workspace": (_SZ, [_P, _I, _I, _I, _I, _I, _I]),
+    "di_cross_attention": (_I, [_P, _I] + [_P, _P] * 4 + [_I] * 6 + [_P, _P, _P, _F, _P, _SZ]),
     "di_tembed": (_I, [_P, _P, _I, _P, _P, _P, _P, _I, _I, _P]),
     "di_synth_uniform": (None, [ctypes.c_uint64, ctypes.c_char_p, _SZ, _F, _P]),
     "di_synth_normal": (None, [ctypes.c_uint64, ctypes.c_char_p, _SZ, _F, _F, _P]),

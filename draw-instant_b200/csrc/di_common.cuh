@@ -63,6 +63,21 @@ struct Ctx {
 };
 
 Ctx* ctx_of(di_ctx_t h);
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// Makes a context's device current for the scope of one call (its stream may be the default stream, which
+// belongs to whichever device is current) and puts the caller's device back.
+struct DeviceGuard {
+  int before = -1;
+  explicit DeviceGuard(int device) {
+    int cur = -1;
+    if (cudaGetDevice(&cur) == cudaSuccess && cur != device && cudaSetDevice(device) == cudaSuccess) before = cur;
+  }
+  ~DeviceGuard() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+  DeviceGuard(const DeviceGuard&) = delete;
+  DeviceGuard& operator=(const DeviceGuard&) = delete;
+};
 void* workspace(Ctx* c, size_t bytes, int slot);
 
 int set_error(Ctx* c, int code, const std::string& msg);

@@ -1,0 +1,239 @@
+"""Attention-layer operators for batches whose requests differ from one another, beside di_linear and di_attention:
+
+linear_lora      a linear layer with a low-rank adapter per row beside the shared weight (di_linear_lora)
+qk_norm_rope     RMS norm of query and key heads with the rotation by position axes (di_qk_norm_rope)
+cross_attention  attention over an encoder's states with lengths and a key mask per request (di_cross_attention)
+
+They take and return torch tensors on the context's device (fp16 or bf16 activations and weights, fp32 norm
+weights, biases and scales, int32 indices) and launch on the context's stream without synchronising.  Scratch
+memory is allocated by torch on that stream for each call, so calls on several streams, and graphs captured from
+them, share none.  A result is the `out` that was passed, or a new tensor.  Bad arguments raise DIError.
+
+    q = linear_lora(ctx, x, w_q, a_q, b_q, scale, rows).view(B * S, H, 64)
+    qk_norm_rope(ctx, q, q_weight=g, positions=pos, axis_dims=(32, 32), q_out=q)
+    o = cross_attention(ctx, q.view(B, S, H, 64), k, v, kv_len=prompt_lengths)
+"""
+from __future__ import annotations
+
+import ctypes
+import functools
+
+import torch
+
+from . import DI_BF16, DI_F16, Context, DIError, lib
+
+__all__ = ["linear_lora", "qk_norm_rope", "cross_attention"]
+
+_CODE = {torch.float16: DI_F16, torch.bfloat16: DI_BF16}
+_ACT = {"none": 0, "silu": 1, "gelu": 2}
+_PAIRING = {"interleaved": 0, "halves": 1}
+
+
+def _code(t, what: str) -> int:
+    code = _CODE.get(t.dtype)
+    if code is None:
+        raise DIError(f"{what}: tensors must be float16 or bfloat16, got {t.dtype}")
+    return code
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise DIError(what)
+
+
+def _on(ctx: Context, what: str, *tensors) -> None:
+    """Every tensor must live on the context's device (there is no CPU path)."""
+    for t in tensors:
+        if t is not None and t.get_device() != ctx.device:
+            raise DIError(f"{what}: tensors must be CUDA tensors on device {ctx.device}, got one on {t.device}")
+
+
+def _like(t, dtype, shape, what: str) -> None:
+    """A contiguous tensor of this type and shape, or None."""
+    if t is not None and (t.dtype != dtype or t.shape != shape or not t.is_contiguous()):
+        raise DIError(f"{what} must be a contiguous {dtype} tensor of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+
+
+def _new(ctx: Context, shape, dtype):
+    """A tensor whose memory belongs to the context's stream."""
+    if torch.cuda.current_stream(ctx.device).cuda_stream == ctx.stream.cuda_stream:
+        return torch.empty(shape, dtype=dtype, device=ctx.stream.device)
+    with torch.cuda.stream(ctx.stream):
+        return torch.empty(shape, dtype=dtype, device=ctx.stream.device)
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+@functools.lru_cache(maxsize=256)
+def _i64x3(a: int, b: int, c: int):
+    return (ctypes.c_longlong * 3)(a, b, c)
+
+
+@functools.lru_cache(maxsize=64)
+def _ints(vals):
+    return (ctypes.c_int * max(1, len(vals)))(*vals)
+
+
+def _rows(t, shape, dtype, what: str):
+    """A [.., n] tensor of contiguous rows; returns its row stride."""
+    if t.dtype != dtype or t.shape != shape or (t.stride(1) != 1 and shape[1] > 1):
+        raise DIError(f"{what} must be a {dtype} tensor of shape {tuple(shape)} with contiguous rows, "
+                      f"got {t.dtype} {tuple(t.shape)} with strides {t.stride()}")
+    return t.stride(0) if shape[0] > 1 else shape[1]
+
+
+def linear_lora(ctx: Context, x, w, a, b, scale, row_adapter, bias=None, residual=None, act: str = "none", out=None):
+    """act(x w^T + bias + scale[i] (x a[i]^T) b[i]^T) + residual with i = row_adapter[row], per row of x.
+
+    x [M, K], w [N, K], a [L, r, K], b [L, N, r] (fp16 or bf16), scale [L] fp32, row_adapter [M] int32 on the
+    device (negative: no adapter), bias [N] fp32, residual and out [M, N].  K a multiple of 64, N of 16, r of 8 up
+    to 128: adapters of other ranks are padded with zeros.  x, residual and out may have a row stride.  Rows may
+    take the adapters in any order; equal neighbours are fastest.  act: none, silu or gelu, before the residual.
+    An index past the last adapter sets DEVERR_BOUNDS in the context's fault word and counts as none."""
+    what = "linear_lora"
+    code, dt = _code(x, what), x.dtype
+    _need(x.dim() == 2 and w.dim() == 2 and a.dim() == 3 and b.dim() == 3, f"{what}: x and w are matrices, a and b have three axes")
+    M, K = x.shape
+    N, (L, r) = w.shape[0], a.shape[:2]
+    _need(M > 0 and N > 0 and K > 0 and L > 0, f"{what}: empty tensors")
+    _need(act in _ACT, f"{what}: act must be one of {', '.join(_ACT)}")
+    ldx = _rows(x, (M, K), dt, f"{what}: x")
+    _like(w, dt, (N, K), f"{what}: w")
+    _like(a, dt, (L, r, K), f"{what}: a")
+    _like(b, dt, (L, N, r), f"{what}: b")
+    _like(scale, torch.float32, (L,), f"{what}: scale")
+    _like(row_adapter, torch.int32, (M,), f"{what}: row_adapter")
+    _like(bias, torch.float32, (N,), f"{what}: bias")
+    ldr = 0 if residual is None else _rows(residual, (M, N), dt, f"{what}: residual")
+    ldy = N if out is None else _rows(out, (M, N), dt, f"{what}: out")
+    _on(ctx, what, x, w, a, b, scale, row_adapter, bias, residual, out)
+    if out is None:
+        out = _new(ctx, (M, N), dt)
+    n = lib().di_linear_lora_workspace(ctx.h, M, N, K, r, L)
+    ws = _new(ctx, (n,), torch.uint8) if n else None
+    ctx.check(lib().di_linear_lora(ctx.h, code, x.data_ptr(), ldx, M, K, w.data_ptr(), N, a.data_ptr(), b.data_ptr(), r, L,
+                                   scale.data_ptr(), row_adapter.data_ptr(), _p(bias), _p(residual), ldr, _ACT[act],
+                                   out.data_ptr(), ldy, _p(ws), n), what)
+    return out
+
+
+def _heads(t, dt, D, what: str):
+    """A [T, H, D] tensor whose heads are contiguous; returns (H, token stride)."""
+    _need(t.dim() == 3, f"{what} must have the axes [tokens, heads, head dim]")
+    T, H, d = t.shape
+    if t.dtype != dt or d != D or t.stride(2) != 1 or (H > 1 and t.stride(1) != D):
+        raise DIError(f"{what} must be a {dt} tensor [tokens, heads, {D}] whose heads are contiguous, "
+                      f"got {t.dtype} {tuple(t.shape)} with strides {t.stride()}")
+    return H, (t.stride(0) if T > 1 else H * D)
+
+
+def qk_norm_rope(ctx: Context, q, k=None, q_weight=None, k_weight=None, eps: float = 1e-6, positions=None, axis_dims=(),
+                 theta: float = 10000.0, pairing: str = "interleaved", q_out=None, k_out=None):
+    """Per head: x * rsqrt(mean(x^2) + eps) * weight, then the rotation by the token's positions; returns
+    (q_out, k_out), or q_out alone when there is no k.
+
+    q [T, Hq, D] and k [T, Hk, D] with D 64 or 128 (fp16 or bf16; tokens may be strided, as in a fused
+    projection; the outputs may be the inputs).  q_weight, k_weight [D] fp32, None: no norm.  positions [P, n] int32
+    on the device, token t takes row t % P, None: no rotation.  axis_dims: n = 1 to 3 even dims that sum to D, in
+    the positions' order; pair j of axis a turns by positions[., a] * theta^(-2 j / axis_dims[a]).  pairing:
+    "interleaved" (values 2i, 2i + 1) or "halves" (values i, i + D / 2)."""
+    what = "qk_norm_rope"
+    code, dt = _code(q, what), q.dtype
+    _need(q.dim() == 3, f"{what}: q must have the axes [tokens, heads, head dim]")
+    T, _, D = q.shape
+    _need(T > 0 and q.shape[1] > 0, f"{what}: empty tensors")
+    _need(D in (64, 128), f"{what}: head dim must be 64 or 128, got {D}")
+    _need(pairing in _PAIRING, f"{what}: pairing must be one of {', '.join(_PAIRING)}")
+    Hq, ldq = _heads(q, dt, D, f"{what}: q")
+    Hk = ldk = ldko = 0
+    if k is not None:
+        Hk, ldk = _heads(k, dt, D, f"{what}: k")
+        _need(Hk > 0 and k.shape[0] == T, f"{what}: k must have the tokens of q and at least one head")
+    else:
+        _need(k_out is None, f"{what}: k_out without k")
+    _like(q_weight, torch.float32, (D,), f"{what}: q_weight")
+    _like(k_weight, torch.float32, (D,), f"{what}: k_weight")
+    axis_dims = tuple(axis_dims)
+    P = 0
+    if positions is not None:
+        _need(1 <= len(axis_dims) <= 3 and all(d > 0 and d % 2 == 0 for d in axis_dims) and sum(axis_dims) == D,
+              f"{what}: axis_dims must be 1 to 3 even dims that sum to the head dim")
+        _need(positions.dim() == 2 and positions.shape[0] > 0, f"{what}: positions must have the axes [rows, position axes]")
+        P = positions.shape[0]
+        _like(positions, torch.int32, (P, len(axis_dims)), f"{what}: positions")
+        _need(theta > 0, f"{what}: theta must be positive")
+    else:
+        _need(not axis_dims, f"{what}: axis_dims without positions")
+    if q_out is not None:
+        _need(q_out.shape == q.shape, f"{what}: q_out must have the shape of q")
+        ldqo = _heads(q_out, dt, D, f"{what}: q_out")[1]
+    else:
+        ldqo = Hq * D
+    if k_out is not None:
+        _need(k_out.shape == k.shape, f"{what}: k_out must have the shape of k")
+        ldko = _heads(k_out, dt, D, f"{what}: k_out")[1]
+    elif Hk:
+        ldko = Hk * D
+    _on(ctx, what, q, k, q_weight, k_weight, positions, q_out, k_out)
+    if q_out is None:
+        q_out = _new(ctx, (T, Hq, D), dt)
+    if k is not None and k_out is None:
+        k_out = _new(ctx, (T, Hk, D), dt)
+    ctx.check(lib().di_qk_norm_rope(ctx.h, code, q.data_ptr(), ldq, Hq, _p(k), ldk, Hk, T, D, _p(q_weight),
+                                    _p(k_weight), eps, _p(positions), P, len(axis_dims), _ints(axis_dims), theta,
+                                    _PAIRING[pairing], q_out.data_ptr(), ldqo, _p(k_out), ldko), what)
+    return q_out if k is None else (q_out, k_out)
+
+
+def _bshd(t, dt, what: str):
+    """Batch, token and head strides of a [B, S, H, D] tensor whose last axis is contiguous."""
+    sb, ss, sh, sd = t.stride()
+    if t.dtype != dt or sd != 1:
+        raise DIError(f"{what} must be a {dt} tensor [batch, tokens, heads, head dim] with a contiguous last axis, "
+                      f"got {t.dtype} {tuple(t.shape)} with strides {t.stride()}")
+    return _i64x3(sb, ss, sh)
+
+
+def cross_attention(ctx: Context, q, k, v, kv_len=None, q_len=None, key_mask=None, scale: float | None = None, out=None):
+    """softmax(scale q k^T) v over each request's valid keys.
+
+    q [B, Sq, H, D], k and v [B, Skv, Hkv, D] (fp16 or bf16), H a multiple of Hkv (query head h reads key head
+    h / (H / Hkv)), D 64 or 128; any strides that are multiples of 8 elements with a contiguous last axis, so token-major
+    and head-major layouts, slices of fused projections and keys and values expanded over the batch all go in place.
+    Key j of request b is valid when j < kv_len[b] and key_mask[b, j] != 0 (kv_len [B] int32, key_mask [B, Skv] uint8 or
+    bool, both on the device, None: all); what masked keys and values hold, infinities and NaN included, has no effect.
+    A request without a valid key gives zeros.  Query rows from q_len[b] on (int32) are not computed and
+    their rows of out stay as they were.  scale: positive, 1 / sqrt(D) by default."""
+    what = "cross_attention"
+    code, dt = _code(q, what), q.dtype
+    _need(q.dim() == 4 and k.dim() == 4 and v.dim() == 4, f"{what}: q, k and v must have the axes [batch, tokens, heads, head dim]")
+    B, Sq, H, D = q.shape
+    Skv, Hkv = k.shape[1:3]
+    _need(B > 0 and Sq > 0 and H > 0 and Skv > 0 and Hkv > 0, f"{what}: empty tensors")
+    _need(D in (64, 128), f"{what}: head dim must be 64 or 128, got {D}")
+    _need(k.shape == (B, Skv, Hkv, D) and v.shape == k.shape, f"{what}: k and v must be [{B}, tokens, heads, {D}], alike")
+    _need(H % Hkv == 0, f"{what}: the query heads must be a multiple of the key heads")
+    if scale is None:
+        scale = D ** -0.5
+    _need(0 < scale < float("inf"), f"{what}: scale must be positive and finite")
+    qs, ks, vs = _bshd(q, dt, f"{what}: q"), _bshd(k, dt, f"{what}: k"), _bshd(v, dt, f"{what}: v")
+    _like(kv_len, torch.int32, (B,), f"{what}: kv_len")
+    _like(q_len, torch.int32, (B,), f"{what}: q_len")
+    if key_mask is not None and key_mask.dtype == torch.bool:
+        key_mask = key_mask.view(torch.uint8)
+    _like(key_mask, torch.uint8, (B, Skv), f"{what}: key_mask")
+    if out is not None:
+        _need(out.shape == q.shape, f"{what}: out must have the shape of q")
+        os_ = _bshd(out, dt, f"{what}: out")
+    else:
+        os_ = _i64x3(Sq * H * D, H * D, D)
+    _on(ctx, what, q, k, v, kv_len, q_len, key_mask, out)
+    if out is None:
+        out = _new(ctx, (B, Sq, H, D), dt)
+    n = lib().di_cross_attention_workspace(ctx.h, B, H, Hkv, Sq, Skv, D)
+    ws = _new(ctx, (n,), torch.uint8) if n else None
+    ctx.check(lib().di_cross_attention(ctx.h, code, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(), os_,
+                                       B, H, Hkv, Sq, Skv, D, _p(q_len), _p(kv_len), _p(key_mask), scale, _p(ws), n), what)
+    return out
