@@ -5,24 +5,24 @@
 // A negative index takes no adapter; an index past the last adapter takes none either and sets
 // DEVERR_BOUNDS in the device error word.
 //
-// Tiles (M > kSkinnyRows): one persistent tensor-core kernel computes all of it in one pass over X.  A unit is a
-// tile of 128 rows and BN columns.  The adapters that its rows name, each once, are its slots.  The B
-// operand of the main loop is [W rows of the tile; A rows of the slots] in one shared-memory block, so one MMA
-// of N = BN + slots * rank accumulates X W^T and X A^T together.  The second part, T, is then scaled,
-// split into two 16-bit parts (hi + lo: 2^-17 relative for bf16) and written back to TMEM over itself, where it is
-// the A operand of the products T B^T that add to the first part, each slot's in the lanes of its own rows only (so
-// an adapter's infinities stay with its rows).  Those follow a few K blocks into the next unit's main loop,
-// when T has been written, so the tensor pipe does not wait.
-// More adapters in a tile than a pass has slots for take further passes over X with A rows alone.
-//   warp 0       TMA loads through one ring of stages
-//   warp 1       MMA issue
-//   warp 2       slots of a unit: its distinct adapters and their rows, each row's scale
-//   warps 4-7    T: TMEM -> scaled, 16-bit -> TMEM
-//   warps 8-15   epilogue: bias, activation, residual, stores through shared memory by TMA
+// Two launches.  The first computes T = scale[a] X A[a]^T, a row's own `rank` values; the second is the product with
+// W and adds T B[a]^T.  The first kernel lets the second start as soon as its own wait for earlier kernels is over, so the
+// second reads X and W at once and waits only before it reads T.
 //
-// Few rows (M <= kSkinnyRows): two launches.  The first computes T in 32 bits, the second streams W once from
-// memory into mma.sync fragments (a tile of 16 weight rows by 8 rows of X), starting before the first is done, and adds
-// the rows' own B products with plain FMAs: every byte of W, A and B is read about once, whoever owns it.
+// Tiles (M > kSkinnyRows): T is kept as two 16-bit parts, hi + lo (2^-17 relative for bf16), and is simply more of K:
+// after the K blocks of X and W come, for every adapter that the tile's rows name, a block of [T_hi | T_lo] against that
+// adapter's B.  Its MMAs write the accumulator rows that name the adapter and no others (the output-lane mask of
+// tcgen05.mma), so a tile may mix adapters at the price of a block each, and an adapter's infinities stay with its rows.
+// One persistent CTA per SM, or CTA pair (cta_group::2: 256 rows, each CTA loads half of B):
+//   warp 0       TMA loads through one ring of stages
+//   warp 1       MMA issue (the pair's first CTA)
+//   warp 2       the tile's distinct adapters and the rows of each
+//   warps 4-11   epilogue: bias, activation, residual (fetched by TMA during the main loop), stores by TMA
+// The accumulator is double-buffered, so a tile's epilogue runs under the next one's main loop.
+//
+// Few rows (M <= kSkinnyRows): T in 32 bits; the second launch streams W once from memory into mma.sync fragments (16
+// weight rows by 8 rows of X) and adds the rows' own B products with plain FMAs: every byte of W, A and B is
+// read about once, whoever owns it.
 #include <algorithm>
 #include <cstring>
 
@@ -31,7 +31,7 @@
 namespace di {
 
 struct LoraParams {
-  CUtensorMap tmX, tmW, tmA, tmB, tmY;
+  CUtensorMap tmX, tmW, tmT, tmB, tmR, tmY;
   const void *X, *W, *A, *B, *R;
   void* Y;
   long long ldx, ldr, ldy;
@@ -41,44 +41,74 @@ struct LoraParams {
   int act;
   int* err;
   // tiles
-  int BN, rp, slots, stages, mt, nt;  // rp: rank rounded up to 16; slots adapters per pass
+  int BN, stages, mt, nt;
   uint32_t stage_bytes;
+  uint16_t* T16;  // [M][t_ld]: 64-column groups, hi and lo parts of 32 ranks (r <= 32) or of 64 in two groups
+  int t_ld;
   // few rows
-  float* T;  // [M][r] scale[a] * X A^T
+  float* T;       // [M][r]
 };
 
 namespace {
 
 constexpr int kSkinnyRows = 128;
-constexpr int kLThreads = 512;
-constexpr int kLists = 3;       // units whose slots are held
-constexpr int kDefer = 4;       // K blocks of the next unit before this unit's T B^T products
-constexpr int kMaxStages = 10;
-constexpr uint32_t kSlab = 2048;  // 32 x 32 16-bit outputs of one epilogue warp
+constexpr int kLThreads = 384;
+constexpr int kMaxStages = 12;
+constexpr int kSlots = 32;        // adapters per list entry
+constexpr int kLists = 3;
+constexpr int kSlabs = 3;         // residual / output slabs per epilogue warp
+constexpr uint32_t kSlab = 2048;  // 32 x 32 16-bit values
 
 struct SlotList {
-  int n;            // adapters in the unit
-  int ids[128];
-  uint4 others[128];  // per slot: the rows (TMEM lanes) that do not name its adapter
-  float scale[128];   // per row
+  int n, more;               // adapters here; more of the tile's adapters follow in the next entry
+  int ids[kSlots];
+  uint32_t others[kSlots][8];  // rows of the tile (accumulator lanes) that do not name the adapter
 };
-constexpr uint32_t kFixedSmem = 1024 + 8 * kSlab + ((kLists * sizeof(SlotList) + 15) / 16 * 16) + 512;
+constexpr uint32_t kListBytes = (kLists * sizeof(SlotList) + 15) / 16 * 16;
+constexpr uint32_t kBarBytes = 8 * (2 * kMaxStages + 2 * kLists + 4 + 8 * kSlabs) + 16;
+constexpr uint32_t kFixedSmem = 1024 + 8 * kSlabs * kSlab + 8 * 128 + kListBytes + (kBarBytes + 15) / 16 * 16;
 
-// D[tmem] += A[tmem] * B[smem desc] in all lanes but those of `off` (bit l of its words: lane l): A's 16-bit values lie
-// two to a column, row m in lane m
-__device__ __forceinline__ void umma_f16_ta_rows(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
-                                                 const uint4& off) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.eq.b32 p, 0, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, "
-      "{%4, %5, %6, %7}, p;\n\t}\n"
-      ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(off.x), "r"(off.y), "r"(off.z), "r"(off.w)
-      : "memory");
+// As umma_f16 / umma_f16_pair, adding to D in all lanes but those of `off` (bit l of word w: row 32 w + l).
+template <bool PAIR>
+__device__ __forceinline__ void umma_f16_rows(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                              const uint32_t* off) {
+  if (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.eq.b32 p, 0, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, "
+        "{%4, %5, %6, %7, %8, %9, %10, %11}, p;\n\t}\n"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3]), "r"(off[4]),
+          "r"(off[5]), "r"(off[6]), "r"(off[7])
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.eq.b32 p, 0, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, "
+        "{%4, %5, %6, %7}, p;\n\t}\n"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3])
+        : "memory");
 }
-__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* m, uint64_t* bar, int c0, int c1, int c2) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-      ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
-      : "memory");
+template <bool PAIR>
+__device__ __forceinline__ void load_2d(void* dst, const CUtensorMap* m, uint32_t bar, int c0, int c1) {
+  if (PAIR) {
+    tma_load_2d_pair(dst, m, bar, c0, c1);
+  } else {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+        ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0), "r"(c1)
+        : "memory");
+  }
+}
+template <bool PAIR>
+__device__ __forceinline__ void load_3d(void* dst, const CUtensorMap* m, uint32_t bar, int c0, int c1, int c2) {
+  if (PAIR)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, "
+        "%5}], [%2];" ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
+        "[%2];" ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
 }
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -94,6 +124,15 @@ __device__ __forceinline__ float2 unpack2(uint32_t w) {
   return BF16 ? __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&w)) : __half22float2(*reinterpret_cast<__half2*>(&w));
 }
 __device__ __forceinline__ float act_of(float v, int act) { return act == 1 ? silu_f(v) : act == 2 ? gelu_erf(v) : v; }
+template <bool BF16>
+__device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (BF16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 
 // Buffer index and phase of a ring.
 struct Ring {
@@ -101,382 +140,433 @@ struct Ring {
   __device__ __forceinline__ void advance(int n) {
     if (++s == n) { s = 0; ph ^= 1; }
   }
+  __device__ __forceinline__ void back(int n) {
+    if (--s < 0) { s = n - 1; ph ^= 1; }
+  }
 };
 
-// Walks a CTA's stages in the order that the loader fills and the MMA warp drains them: K blocks of each pass, and
-// the T B^T blocks of a pass at once, or, for a unit's last pass, kDefer K blocks into the next unit.
-// kblock(pass, kb), pass_done(pass, count), expand(list slot, pass, count) return false to stop.
-template <typename Begin, typename KBlock, typename PassDone, typename Expand, typename End>
-__device__ __forceinline__ bool walk_units(const LoraParams& p, Begin begin, KBlock kblock, PassDone pass_done,
-                                           Expand expand, End end) {
-  const int units = p.mt * p.nt, nk = p.K / 64;
-  int pend_pass = -1, pend_u = 0;
-  for (int u = blockIdx.x; u < units; u += gridDim.x) {
-    int nd = 0;
-    if (!begin(u, nd)) return false;
-    const int passes = max(1, (nd + p.slots - 1) / p.slots);
-    for (int ps = 0; ps < passes; ++ps) {
-      const int cnt = min(p.slots, nd - ps * p.slots);
-      for (int kb = 0; kb < nk; ++kb) {
-        if (pend_pass >= 0 && kb == min(kDefer, nk - 1)) {
-          if (!expand(pend_u, pend_pass)) return false;
-          end(pend_u);
-          pend_pass = -1;
-        }
-        if (!kblock(u, ps, kb, cnt)) return false;
+// ---- tiles: T = scale X A^T in two 16-bit parts ----
+
+// ROWS rows of X by 32 ranks per block; the warps are KW shares of K by ROWS / RW groups of RW rows, summed in shared memory.
+// A lane's 16-byte loads of 8 consecutive k stand for two 16-wide MMA steps: both operands use the same order of k.
+// Bound: the bytes of X; the rows' adapters come from L2, once per block for each adapter its rows name.
+template <bool BF16, int ROWS, int RW>
+__global__ void __launch_bounds__(256) lora_t_kernel(const __grid_constant__ LoraParams p) {
+  constexpr int KW = 8 * RW / ROWS, MT = RW / 8;
+  __shared__ float red[KW][ROWS][33];
+  pdl_begin();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const int m0 = blockIdx.y * ROWS, j0 = blockIdx.x * 32;
+  const int kw = warp % KW, rw = warp / KW * RW;
+  constexpr int IDS = (ROWS + 31) / 32;
+  int ids[IDS];
+#pragma unroll
+  for (int i = 0; i < IDS; ++i) {
+    const int l = i * 32 + lane;
+    ids[i] = l < ROWS && m0 + l < p.M ? __ldg(p.rows + m0 + l) : -1;
+    if (ids[i] >= p.L) ids[i] = -1;
+  }
+  const uint16_t* xr[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t)  // rows past the last are computed and not stored
+    xr[t] = static_cast<const uint16_t*>(p.X) + min(m0 + rw + t * 8 + lane / 4, p.M - 1) * p.ldx + (lane & 3) * 8;
+#pragma unroll
+  for (int i = 0; i < IDS; ++i) {
+    unsigned open;
+    while ((open = __ballot_sync(0xffffffffu, ids[i] >= 0)) != 0) {  // the same in every warp of the block
+      const int id = __shfl_sync(0xffffffffu, ids[i], __ffs(open) - 1);
+      unsigned mine[IDS];
+#pragma unroll
+      for (int k = 0; k < IDS; ++k) {
+        mine[k] = __ballot_sync(0xffffffffu, ids[k] == id);
+        if (ids[k] == id) ids[k] = -1;
       }
-      pass_done(u, ps, cnt);
-      if (cnt > 0) {
-        if (ps == passes - 1) {
-          pend_pass = ps;
-          pend_u = u;
-        } else if (!expand(u, ps)) {
-          return false;
+      float acc[2][MT][4] = {};
+      const uint16_t* ar[4];  // ranks j0 + 8 i + lane / 4; those past the last read the last and are dropped
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        ar[k] = static_cast<const uint16_t*>(p.A) + ((long long)id * p.r + min(j0 + k * 8 + lane / 4, p.r - 1)) * p.K +
+                (lane & 3) * 8;
+#pragma unroll 2
+      for (int k = kw * 32; k < p.K; k += KW * 32) {
+        uint4 a[4], b[MT];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) a[q] = __ldg(reinterpret_cast<const uint4*>(ar[q] + k));
+#pragma unroll
+        for (int t = 0; t < MT; ++t) b[t] = __ldg(reinterpret_cast<const uint4*>(xr[t] + k));
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const uint32_t f0[4] = {a[2 * q].x, a[2 * q + 1].x, a[2 * q].y, a[2 * q + 1].y};
+          const uint32_t f1[4] = {a[2 * q].z, a[2 * q + 1].z, a[2 * q].w, a[2 * q + 1].w};
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            mma_16x8x16<BF16>(acc[q][t], f0, b[t].x, b[t].y);
+            mma_16x8x16<BF16>(acc[q][t], f1, b[t].z, b[t].w);
+          }
         }
-      } else {
-        end(u);
       }
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {  // d[0..1]: rank lane / 4, rows 2 (lane & 3) + {0, 1}; d[2..3]: rank + 8
+          const int m = rw + t * 8 + (lane & 3) * 2, j = q * 16 + lane / 4;
+          red[kw][m][j] = acc[q][t][0];
+          red[kw][m + 1][j] = acc[q][t][1];
+          red[kw][m][j + 8] = acc[q][t][2];
+          red[kw][m + 1][j + 8] = acc[q][t][3];
+        }
+      __syncthreads();
+      const float sc = __ldg(p.scale + id);
+      for (int o = threadIdx.x; o < ROWS * 16; o += 256) {  // two ranks each
+        const int m = o / 16, j = o % 16 * 2;
+        if (!((mine[m / 32] >> (m % 32)) & 1)) continue;
+        const int rank = j0 + j;
+        if (rank >= (p.r + 15) / 16 * 16) continue;
+        float x = 0.f, y = 0.f;
+#pragma unroll
+        for (int k = 0; k < KW; ++k) { x += red[k][m][j]; y += red[k][m][j + 1]; }
+        x *= sc;
+        y *= sc;
+        if (rank >= p.r) x = y = 0.f;  // the last 16-wide step's empty half (r is a multiple of 8)
+        const uint32_t hi = pack2<BF16>(x, y);
+        const float2 h = unpack2<BF16>(hi);
+        // a part that is not finite stands alone (inf - inf would be NaN)
+        const uint32_t lo = pack2<BF16>(isinf(h.x) ? 0.f : x - h.x, isinf(h.y) ? 0.f : y - h.y);
+        const int half = p.r <= 32 ? 32 : 64;
+        uint16_t* t = p.T16 + (long long)(m0 + m) * p.t_ld + rank / half * (2 * half) + rank % half;
+        *reinterpret_cast<uint32_t*>(t) = hi;
+        *reinterpret_cast<uint32_t*>(t + half) = lo;
+      }
+      __syncthreads();
     }
   }
-  if (pend_pass >= 0) {
-    if (!expand(pend_u, pend_pass)) return false;
-    end(pend_u);
-  }
-  return true;
 }
 
-template <bool BF16>
+// ---- tiles: Y ----
+
+template <bool BF16, bool PAIR>
 __global__ void __launch_bounds__(kLThreads, 1) lora_tile_kernel(const __grid_constant__ LoraParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sStage = smem;                                    // [stages]: 128 X rows, then W and A rows, 128 B each
-  uint8_t* sSlab = smem + p.stages * p.stage_bytes;          // [8]
-  SlotList* lists = reinterpret_cast<SlotList*>(sSlab + 8 * kSlab);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sSlab + 8 * kSlab + (kLists * sizeof(SlotList) + 15) / 16 * 16);
-  uint64_t* full = bars;                       // [kMaxStages]
+  uint8_t* sStage = smem;                            // [stages]: 128 rows of X or T, then rows of W or B, 128 bytes each
+  uint8_t* sSlab = smem + p.stages * p.stage_bytes;  // [8][kSlabs]
+  float* sBias = reinterpret_cast<float*>(sSlab + 8 * kSlabs * kSlab);  // [8][32]
+  SlotList* lists = reinterpret_cast<SlotList*>(sBias + 8 * 32);
+  uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(lists) + kListBytes);  // [kMaxStages]
   uint64_t* empty = full + kMaxStages;         // [kMaxStages]
   uint64_t* list_full = empty + kMaxStages;    // [kLists]
   uint64_t* list_empty = list_full + kLists;   // [kLists]
-  uint64_t* t_ready = list_empty + kLists;     // [2] X A^T of accumulator ab complete
-  uint64_t* t_full = t_ready + 2;              // [2] T written
-  uint64_t* d_full = t_full + 2;               // [2] accumulator complete
-  uint64_t* d_empty = d_full + 2;              // [2] accumulator read
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(d_empty + 2);
+  uint64_t* d_full = list_empty + kLists;      // [2] accumulator complete
+  uint64_t* d_empty = d_full + 2;              // [2] accumulator read (a pair: by both, on the first CTA's)
+  uint64_t* r_full = d_empty + 2;              // [8][kSlabs] residual landed
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(r_full + 8 * kSlabs);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int rank = PAIR ? (int)cluster_ctarank() : 0;
+  const int first = PAIR ? (int)blockIdx.x / 2 : (int)blockIdx.x, step = PAIR ? (int)gridDim.x / 2 : (int)gridDim.x;
+  const bool issues = rank == 0;  // this CTA's warp 1 issues the MMAs
   if (threadIdx.x == 0) {
     for (int i = 0; i < p.stages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
-    for (int i = 0; i < kLists; ++i) { mbar_init(&list_full[i], 1); mbar_init(&list_empty[i], 6); }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&t_ready[i], 1);
-      mbar_init(&t_full[i], 4);
-      mbar_init(&d_full[i], 1);
-      mbar_init(&d_empty[i], 8);
-    }
+    for (int i = 0; i < kLists; ++i) { mbar_init(&list_full[i], 1); mbar_init(&list_empty[i], issues ? 2 : 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&d_full[i], 1); mbar_init(&d_empty[i], PAIR ? 16 : 8); }
+    for (int i = 0; i < 8 * kSlabs; ++i) mbar_init(&r_full[i], 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 1) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  if (warp == 1) {
+    if (PAIR) { tmem_alloc_pair(tmem_slot, 512); tmem_relinquish_pair(); }
+    else { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  }
   tc_fence_before();
-  __syncthreads();
+  if (PAIR) cluster_sync();  // both CTAs' barriers are initialised before either signals the other
+  else __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  pdl_begin();
-  const int units = p.mt * p.nt;
-  // TMEM: accumulator ab of the unit's BN columns at 256 ab, its X A^T (then T) behind them
+  const uint32_t full0 = PAIR ? mapa_shared(smem_u32(full), 0) : smem_u32(full);
+  const uint32_t d_empty0 = PAIR ? mapa_shared(smem_u32(d_empty), 0) : smem_u32(d_empty);
+  pdl_trigger();
+  // lora_t_kernel let this one start after its own wait for earlier kernels: X, W, the indices, R and Y are safe to use
+  // at once, T only after pdl_wait.
+  constexpr int TM = PAIR ? 256 : 128;
+  const int units = p.mt * p.nt, nk = p.K / 64;
+  const int groups = p.r <= 32 ? 1 : (p.r + 63) / 64;  // rank groups, each one block of B
+  const uint32_t b_rows = PAIR ? p.BN / 2 : p.BN;      // rows of W or B that this CTA loads
 
   if (warp == 0) {
     if (elect_one()) {
       tma_prefetch_desc(&p.tmX);
       tma_prefetch_desc(&p.tmW);
-      tma_prefetch_desc(&p.tmA);
+      tma_prefetch_desc(&p.tmT);
       tma_prefetch_desc(&p.tmB);
-      Ring st, li, le;  // stages, lists begun, lists ended
-      int cur = 0;      // list of the unit that is being loaded
+      Ring st, li;
+      bool ok = true, waited = false;
       unsigned issued = 0;
-      auto stage = [&]() {
-        return !*abort_flag && mbar_wait(&empty[st.s], st.ph ^ 1, p.err, DEVERR_WAIT_TMA);
+      auto stage = [&](uint32_t bytes) {  // the next free stage, armed for `bytes` of each CTA
+        if (*abort_flag || !mbar_wait<PAIR>(&empty[st.s], st.ph ^ 1, p.err, DEVERR_WAIT_TMA)) return false;
+        if (issues) mbar_arrive_expect_tx(&full[st.s], PAIR ? 2 * bytes : bytes);
+        ++issued;
+        return true;
       };
-      const bool ok = walk_units(
-          p,
-          [&](int u, int& nd) {
-            if (*abort_flag || !mbar_wait(&list_full[li.s], li.ph, p.err, DEVERR_WAIT_TMA)) return false;
-            cur = li.s;
-            nd = lists[cur].n;
-            li.advance(kLists);
-            return true;
-          },
-          [&](int u, int ps, int kb, int cnt) {
-            if (!stage()) return false;
-            uint8_t* d = sStage + st.s * p.stage_bytes;
-            mbar_arrive_expect_tx(&full[st.s], 16384u + (uint32_t)((ps == 0 ? p.BN : 0) + max(cnt, 0) * p.rp) * 128u);
-            tma_load_2d(d, &p.tmX, &full[st.s], kb * 64, u / p.nt * 128);
-            if (ps == 0) tma_load_2d(d + 16384, &p.tmW, &full[st.s], kb * 64, u % p.nt * p.BN);
-            for (int g = 0; g < cnt; ++g)
-              tma_load_3d(d + 16384 + (p.BN + g * p.rp) * 128, &p.tmA, &full[st.s], kb * 64, 0,
-                          lists[cur].ids[ps * p.slots + g]);
-            st.advance(p.stages);
-            ++issued;
-            return true;
-          },
-          [&](int, int, int) {},
-          [&](int u, int ps) {
-            const int cnt = min(p.slots, lists[le.s].n - ps * p.slots);
-            for (int g = 0; g < cnt; ++g)
-              for (int c = 0; c < p.rp; c += 64) {
-                if (!stage()) return false;
-                mbar_arrive_expect_tx(&full[st.s], (uint32_t)p.BN * 128u);
-                tma_load_3d(sStage + st.s * p.stage_bytes + 16384, &p.tmB, &full[st.s], c, u % p.nt * p.BN,
-                            lists[le.s].ids[ps * p.slots + g]);
+      for (int u = first; ok && u < units; u += step) {
+        const int m0 = u / p.nt * TM + rank * 128, n0 = u % p.nt * p.BN + rank * (int)b_rows;
+        for (int kb = 0; ok && kb < nk; ++kb) {
+          if (!(ok = stage(16384u + b_rows * 128u))) break;
+          uint8_t* d = sStage + st.s * p.stage_bytes;
+          load_2d<PAIR>(d, &p.tmX, full0 + st.s * 8, kb * 64, m0);
+          load_2d<PAIR>(d + 16384, &p.tmW, full0 + st.s * 8, kb * 64, n0);
+          st.advance(p.stages);
+        }
+        for (bool more = true; ok && more;) {
+          if (!(ok = !*abort_flag && mbar_wait(&list_full[li.s], li.ph, p.err, DEVERR_WAIT_TMA))) break;
+          const SlotList& l = lists[li.s];
+          more = l.more;
+          if (l.n && !waited) {
+            pdl_wait();
+            waited = true;
+          }
+          for (int g = 0; ok && g < l.n; ++g)
+            for (int c = 0; ok && c < groups; ++c) {
+              if (!(ok = stage(16384u + b_rows * 128u))) break;
+              uint8_t* d = sStage + st.s * p.stage_bytes;
+              load_2d<PAIR>(d, &p.tmT, full0 + st.s * 8, c * 128, m0);
+              load_3d<PAIR>(d + 16384, &p.tmB, full0 + st.s * 8, c * 64, n0, l.ids[g]);
+              st.advance(p.stages);
+              if (p.r > 32) {  // the lo parts, against the same B
+                if (!(ok = stage(16384u))) break;
+                load_2d<PAIR>(sStage + st.s * p.stage_bytes, &p.tmT, full0 + st.s * 8, c * 128 + 64, m0);
                 st.advance(p.stages);
-                ++issued;
               }
-            return true;
-          },
-          [&](int) {
-            mbar_arrive(&list_empty[le.s]);
-            le.advance(kLists);
-          });
+            }
+          mbar_arrive(&list_empty[li.s]);
+          li.advance(kLists);
+        }
+      }
       if (!ok) {  // leave no copy in flight behind
         *abort_flag = 1;
-        for (unsigned i = 0; i < min(issued, (unsigned)p.stages); ++i) {
-          st.s = st.s ? st.s - 1 : (st.ph ^= 1, p.stages - 1);
-          mbar_wait(&full[st.s], st.ph, p.err, DEVERR_WAIT_TMA);
+        for (unsigned i = 0; issues && i < min(issued, (unsigned)p.stages); ++i) {
+          st.back(p.stages);
+          mbar_wait<PAIR>(&full[st.s], st.ph, p.err, DEVERR_WAIT_TMA);
         }
       }
     }
   } else if (warp == 1) {
-    if (elect_one()) {
-      Ring st, li, le;
-      int ab_u = -1;          // accumulator of the unit in its main loop
-      int nu = 0;             // units begun
-      int eu = 0;             // units ended
-      int ph_t[2] = {0, 0};
-      auto stage = [&]() {
-        return !*abort_flag && mbar_wait(&full[st.s], st.ph, p.err, DEVERR_WAIT_MMA);
+    if (issues && elect_one()) {
+      Ring st, li;
+      bool ok = true;
+      int nu = 0;
+      const uint32_t id = idesc_f16(TM, 0, BF16) | ((uint32_t)(p.BN >> 3) << 17);
+      auto commit = [&](uint64_t* bar) {
+        if (PAIR) umma_commit_pair(bar, 0x3);
+        else umma_commit(bar);
       };
-      const bool ok = walk_units(
-          p,
-          [&](int u, int& nd) {
-            if (*abort_flag || !mbar_wait(&list_full[li.s], li.ph, p.err, DEVERR_WAIT_MMA)) return false;
-            nd = lists[li.s].n;
-            li.advance(kLists);
-            ab_u = nu & 1;
-            if (!mbar_wait(&d_empty[ab_u], ((nu >> 1) & 1) ^ 1, p.err, DEVERR_WAIT_MMA)) return false;
-            ++nu;
-            return true;
-          },
-          [&](int u, int ps, int kb, int cnt) {
-            if (!stage()) return false;
-            tc_fence_after();
-            const uint32_t a = smem_u32(sStage + st.s * p.stage_bytes);
-            const int first = ps == 0 ? 0 : p.BN, n = (ps == 0 ? p.BN : 0) + max(cnt, 0) * p.rp;
-            const uint32_t id = idesc_f16(128, 0, BF16) | ((uint32_t)(n >> 3) << 17);
+      auto stage = [&]() {
+        const bool r = !*abort_flag && mbar_wait<PAIR>(&full[st.s], st.ph, p.err, DEVERR_WAIT_MMA);
+        tc_fence_after();
+        return r;
+      };
+      for (int u = first; ok && u < units; u += step, ++nu) {
+        const int ab = nu & 1;
+        const uint32_t d = tmem + ab * 256;
+        ok = !*abort_flag && mbar_wait<PAIR>(&d_empty[ab], ((nu >> 1) & 1) ^ 1, p.err, DEVERR_WAIT_MMA);
+        for (int kb = 0; ok && kb < nk; ++kb) {
+          if (!(ok = stage())) break;
+          const uint32_t a = smem_u32(sStage + st.s * p.stage_bytes);
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              umma_f16(tmem + ab_u * 256 + first, sdesc_sw128(a + k * 32, 16, 1024),
-                       sdesc_sw128(a + 16384 + first * 128 + k * 32, 16, 1024), id, (kb | k) != 0);
-            umma_commit(&empty[st.s]);
-            st.advance(p.stages);
-            return true;
-          },
-          [&](int u, int ps, int cnt) { umma_commit(cnt > 0 ? &t_ready[ab_u] : &d_full[ab_u]); },
-          [&](int u, int ps) {
-            const int ab = eu & 1, nd = lists[le.s].n, cnt = min(p.slots, nd - ps * p.slots);
-            if (*abort_flag || !mbar_wait(&t_full[ab], ph_t[ab], p.err, DEVERR_WAIT_MMA)) return false;
-            ph_t[ab] ^= 1;
-            const uint32_t d = tmem + ab * 256, t = d + p.BN;
-            const uint32_t id = idesc_f16(128, 0, BF16) | ((uint32_t)(p.BN >> 3) << 17);
-            for (int g = 0; g < cnt; ++g) {
-              const uint4 off = lists[le.s].others[ps * p.slots + g];
-              for (int c = 0; c < p.rp; c += 64) {
-                if (!stage()) return false;
-                tc_fence_after();
-                const uint32_t b = smem_u32(sStage + st.s * p.stage_bytes + 16384);
-                for (int k = 0; k < min(64, p.rp - c); k += 16) {
-                  const int col = g * p.rp + c + k;  // 32 T columns: 16 of hi pairs, then 16 of lo pairs
-                  const uint32_t at = t + col / 32 * 32 + col % 32 / 2;
-                  const uint64_t bd = sdesc_sw128(b + k * 2, 16, 1024);
-                  umma_f16_ta_rows(d, at, bd, id, off);
-                  umma_f16_ta_rows(d, at + 16, bd, id, off);
-                }
-                umma_commit(&empty[st.s]);
+          for (int k = 0; k < 4; ++k) {
+            const uint64_t ad = sdesc_sw128(a + k * 32, 16, 1024), bd = sdesc_sw128(a + 16384 + k * 32, 16, 1024);
+            if (PAIR) umma_f16_pair(d, ad, bd, id, (kb | k) != 0);
+            else umma_f16(d, ad, bd, id, (kb | k) != 0);
+          }
+          commit(&empty[st.s]);
+          st.advance(p.stages);
+        }
+        for (bool more = true; ok && more;) {
+          if (!(ok = !*abort_flag && mbar_wait(&list_full[li.s], li.ph, p.err, DEVERR_WAIT_MMA))) break;
+          const SlotList& l = lists[li.s];
+          more = l.more;
+          for (int g = 0; ok && g < l.n; ++g)
+            for (int c = 0; ok && c < groups; ++c) {
+              if (!(ok = stage())) break;
+              const uint32_t t = smem_u32(sStage + st.s * p.stage_bytes), b = t + 16384;
+              const int s0 = st.s, steps = (min(p.r - c * 64, 64) + 15) / 16;
+              for (int k = 0; k < steps; ++k)
+                umma_f16_rows<PAIR>(d, sdesc_sw128(t + k * 32, 16, 1024), sdesc_sw128(b + k * 32, 16, 1024), id, l.others[g]);
+              st.advance(p.stages);
+              uint32_t lo = t + 64;
+              if (p.r > 32) {
+                if (!(ok = stage())) break;
+                lo = smem_u32(sStage + st.s * p.stage_bytes);
+              }
+              for (int k = 0; k < steps; ++k)
+                umma_f16_rows<PAIR>(d, sdesc_sw128(lo + k * 32, 16, 1024), sdesc_sw128(b + k * 32, 16, 1024), id, l.others[g]);
+              commit(&empty[s0]);
+              if (p.r > 32) {
+                commit(&empty[st.s]);
                 st.advance(p.stages);
               }
             }
-            if ((ps + 1) * p.slots >= nd) umma_commit(&d_full[ab]);
-            return true;
-          },
-          [&](int) {
-            mbar_arrive(&list_empty[le.s]);
-            le.advance(kLists);
-            ++eu;
-          });
+          mbar_arrive(&list_empty[li.s]);
+          li.advance(kLists);
+        }
+        if (ok) commit(&d_full[ab]);
+      }
       if (!ok) *abort_flag = 1;
     }
   } else if (warp == 2) {
     Ring li;
-    for (int u = blockIdx.x; u < units; u += gridDim.x) {
-      const bool ok = !*abort_flag && mbar_wait(&list_empty[li.s], li.ph ^ 1, p.err, DEVERR_WAIT_EPI);
-      if (!__all_sync(0xffffffffu, ok)) { *abort_flag = 1; break; }
-      SlotList& l = lists[li.s];
-      int a[4];
-      bool open_rows[4];  // rows whose adapter has no slot yet
+    bool ok = true;
+    for (int u = first; ok && u < units; u += step) {
+      constexpr int RL = TM / 32;  // rows per lane
+      int a[RL];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int m = u / p.nt * 128 + i * 32 + lane;
+      for (int i = 0; i < RL; ++i) {
+        const int m = u / p.nt * TM + i * 32 + lane;
         a[i] = m < p.M ? __ldg(p.rows + m) : -1;
         if (a[i] >= p.L) {
           atomicOr(p.err, DEVERR_BOUNDS);
           a[i] = -1;
         }
-        l.scale[i * 32 + lane] = a[i] >= 0 ? __ldg(p.scale + a[i]) : 0.f;
-        open_rows[i] = a[i] >= 0;
       }
-      int n = 0;
+      int n = -1;  // adapters in the open list entry, -1: none open
+      auto open_entry = [&] {
+        const bool w = !*abort_flag && mbar_wait(&list_empty[li.s], li.ph ^ 1, p.err, DEVERR_WAIT_EPI);
+        n = 0;
+        return __all_sync(0xffffffffu, w) != 0;
+      };
+      auto close_entry = [&](int more) {
+        if (lane == 0) {
+          lists[li.s].n = n;
+          lists[li.s].more = more;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&list_full[li.s]);
+        li.advance(kLists);
+      };
+      ok = open_entry();
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < RL; ++i) {
         unsigned open;
-        while ((open = __ballot_sync(0xffffffffu, open_rows[i])) != 0) {
+        while (ok && (open = __ballot_sync(0xffffffffu, a[i] >= 0)) != 0) {
+          if (n == kSlots) {
+            close_entry(1);
+            if (!(ok = open_entry())) break;
+          }
           const int id = __shfl_sync(0xffffffffu, a[i], __ffs(open) - 1);
-          unsigned b[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            b[k] = __ballot_sync(0xffffffffu, a[k] != id);
-            open_rows[k] = open_rows[k] && a[k] != id;
+          for (int k = 0; k < RL; ++k) {
+            const unsigned o = __ballot_sync(0xffffffffu, a[k] != id);
+            if (a[k] == id) a[k] = -1;
+            if (lane == 0) lists[li.s].others[n][k] = o;
           }
-          if (lane == 0) {
-            l.ids[n] = id;
-            l.others[n] = make_uint4(b[0], b[1], b[2], b[3]);
-          }
+          if (lane == 0) lists[li.s].ids[n] = id;
           ++n;
         }
       }
-      if (lane == 0) l.n = n;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&list_full[li.s]);
-      li.advance(kLists);
-    }
-  } else if (warp >= 4 && warp < 8) {
-    const int q = warp & 3, row = q * 32 + lane;
-    Ring li;
-    int nu = 0, ph[2] = {0, 0};
-    bool ok = true;
-    for (int u = blockIdx.x; ok && u < units; u += gridDim.x, ++nu) {
-      ok = !*abort_flag && mbar_wait(&list_full[li.s], li.ph, p.err, DEVERR_WAIT_EPI);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      const int nd = lists[li.s].n, ab = nu & 1;
-      const float sc = lists[li.s].scale[row];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&list_empty[li.s]);
-      li.advance(kLists);
-      const uint32_t t = tmem + ab * 256 + p.BN + (static_cast<uint32_t>(q * 32) << 16);
-      for (int first = 0; first < nd; first += p.slots) {
-        ok = !*abort_flag && mbar_wait(&t_ready[ab], ph[ab], p.err, DEVERR_WAIT_EPI);
-        ok = __all_sync(0xffffffffu, ok);
-        ph[ab] ^= 1;
-        if (!ok) break;
-        tc_fence_after();
-        const int cols = min(p.slots, nd - first) * p.rp;
-        for (int c = 0; c < cols; c += 32) {
-          uint32_t r[32];
-          tmem_ld32(t + c, r);
-          tmem_wait_ld();
-          uint32_t w[32];  // 16 hi pairs, 16 lo pairs
-#pragma unroll
-          for (int k = 0; k < 32; k += 2) {
-            const float x = sc * __uint_as_float(r[k]), y = sc * __uint_as_float(r[k + 1]);
-            w[k / 2] = pack2<BF16>(x, y);
-            const float2 h = unpack2<BF16>(w[k / 2]);
-            // a part that is not finite stands alone (inf - inf would be NaN)
-            w[16 + k / 2] = pack2<BF16>(isinf(h.x) ? 0.f : x - h.x, isinf(h.y) ? 0.f : y - h.y);
-          }
-          tmem_st32(t + c, w);
-        }
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&t_full[ab]);
-      }
+      if (ok) close_entry(0);
     }
     if (!ok) *abort_flag = 1;
-  } else if (warp >= 8) {
-    const int q = warp & 3, half = (warp - 8) / 4;
-    uint8_t* slab = sSlab + (warp - 8) * kSlab;
+  } else if (warp >= 4) {
+    const int ew = warp - 4, q = warp & 3, half = ew / 4;
+    uint8_t* slabs = sSlab + ew * kSlabs * kSlab;
+    uint64_t* rb = r_full + ew * kSlabs;
+    float* bs = sBias + ew * 32;
+    unsigned r_ph = 0;  // phases of this warp's residual barriers
     bool ok = true;
     int nu = 0;
-    for (int u = blockIdx.x; ok && u < units; u += gridDim.x, ++nu) {
-      const int ab = nu & 1, m0 = u / p.nt * 128 + q * 32, n0 = u % p.nt * p.BN, m = m0 + lane;
-      ok = !*abort_flag && mbar_wait(&d_full[ab], (nu >> 1) & 1, p.err, DEVERR_WAIT_EPI);
+    pdl_wait();  // this grid is not over before lora_t_kernel is
+    for (int u = first; ok && u < units; u += step, ++nu) {
+      const int ab = nu & 1, m0 = u / p.nt * TM + rank * 128 + q * 32, n0 = u % p.nt * p.BN;
+      // 32-column chunks of this warp: half, half + 2, ...
+      const int all = (min(p.BN, p.N - n0) + 31) / 32, mine = m0 < p.M ? (all - half + 1) / 2 : 0;
+      auto fetch = [&](int i) {  // residual of chunk i into its slab (free: its last store has been read)
+        mbar_arrive_expect_tx(&rb[i % kSlabs], kSlab);
+        tma_load_2d(slabs + i % kSlabs * kSlab, &p.tmR, &rb[i % kSlabs], n0 + (half + 2 * i) * 32, m0);
+      };
+      if (p.R && lane == 0 && mine) {
+        bulk_wait_read0();
+        for (int i = 0; i < min(mine, kSlabs); ++i) fetch(i);
+      }
+      ok = !*abort_flag && mbar_wait<PAIR>(&d_full[ab], (nu >> 1) & 1, p.err, DEVERR_WAIT_EPI);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
       const uint32_t d = tmem + ab * 256 + (static_cast<uint32_t>(q * 32) << 16);
-      if (m0 < p.M) {
 #pragma unroll 1
-        for (int c = half * 32; c < p.BN; c += 64) {
-          const int nb = n0 + c;
-          if (nb >= p.N) break;
-          uint4 res[4];
-          if (p.R && m < p.M) {
-            const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.R) + m * p.ldr + nb);
+      for (int i = 0; i < mine; ++i) {
+        const int c = (half + 2 * i) * 32, nb = n0 + c, sl = i % kSlabs;
+        uint8_t* slab = slabs + sl * kSlab;
+        uint4* rp = reinterpret_cast<uint4*>(slab + lane * 64);  // 64-byte rows, 64-byte swizzle
+        uint32_t r[32];
+        tmem_ld32(d + c, r);
+        if (p.bias) bs[lane] = nb + lane < p.N ? __ldg(p.bias + nb + lane) : 0.f;
+        __syncwarp();
+        tmem_wait_ld();
+        float v[32];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (nb + k * 8 < p.N) res[k] = src[k];  // may be the output: not through the read-only path
+        for (int k = 0; k < 32; ++k) v[k] = __uint_as_float(r[k]);
+        if (p.bias) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float4 b = reinterpret_cast<const float4*>(bs)[k];
+            v[4 * k] += b.x; v[4 * k + 1] += b.y; v[4 * k + 2] += b.z; v[4 * k + 3] += b.w;
           }
-          const float bl = p.bias && nb + lane < p.N ? __ldg(p.bias + nb + lane) : 0.f;
-          uint32_t r[32];
-          tmem_ld32(d + c, r);
-          tmem_wait_ld();
-          float v[32];
+        }
+        if (p.act) {
 #pragma unroll
-          for (int k = 0; k < 32; ++k) v[k] = __uint_as_float(r[k]) + __shfl_sync(0xffffffffu, bl, k);
-          if (p.act) {
+          for (int k = 0; k < 32; ++k) v[k] = act_of(v[k], p.act);
+        }
+        if (p.R) {
+          ok = mbar_wait(&rb[sl], (r_ph >> sl) & 1, p.err, DEVERR_WAIT_EPI) && ok;
+          r_ph ^= 1u << sl;
 #pragma unroll
-            for (int k = 0; k < 32; ++k) v[k] = act_of(v[k], p.act);
-          }
-          if (p.R && m < p.M) {
+          for (int k = 0; k < 4; ++k) {
+            const uint4 t = rp[k ^ ((lane >> 1) & 3)];
+            const uint32_t w[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint32_t w[4] = {res[k].x, res[k].y, res[k].z, res[k].w};
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float2 f = unpack2<BF16>(w[e]);
-                v[8 * k + 2 * e] += f.x;
-                v[8 * k + 2 * e + 1] += f.y;
-              }
+            for (int e = 0; e < 4; ++e) {
+              const float2 f = unpack2<BF16>(w[e]);
+              v[8 * k + 2 * e] += f.x;
+              v[8 * k + 2 * e + 1] += f.y;
             }
           }
-          if (lane == 0) bulk_wait_read0();  // the previous chunk's store has read the slab
-          __syncwarp();
-          uint4* rp = reinterpret_cast<uint4*>(slab + lane * 64);  // 64-byte rows, 64-byte swizzle
+        } else {
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kSlabs - 1) : "memory");
+          __syncwarp();  // the store that last used this slab has read it
+        }
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            rp[k ^ ((lane >> 1) & 3)] = make_uint4(pack2<BF16>(v[8 * k], v[8 * k + 1]), pack2<BF16>(v[8 * k + 2], v[8 * k + 3]),
-                                                   pack2<BF16>(v[8 * k + 4], v[8 * k + 5]),
-                                                   pack2<BF16>(v[8 * k + 6], v[8 * k + 7]));
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            tma_store_2d(&p.tmY, slab, nb, m0);  // rows and columns outside Y are skipped
-            bulk_commit();
+        for (int k = 0; k < 4; ++k)
+          rp[k ^ ((lane >> 1) & 3)] = make_uint4(pack2<BF16>(v[8 * k], v[8 * k + 1]), pack2<BF16>(v[8 * k + 2], v[8 * k + 3]),
+                                                 pack2<BF16>(v[8 * k + 4], v[8 * k + 5]),
+                                                 pack2<BF16>(v[8 * k + 6], v[8 * k + 7]));
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_2d(&p.tmY, slab, nb, m0);  // rows and columns outside Y are skipped
+          bulk_commit();
+          if (p.R && i + kSlabs < mine) {
+            bulk_wait_read0();
+            fetch(i + kSlabs);
           }
         }
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&d_empty[ab]);
+      if (lane == 0) {
+        if (PAIR) mbar_arrive_cluster(d_empty0 + ab * 8);
+        else mbar_arrive(&d_empty[ab]);
+      }
     }
     if (!ok) *abort_flag = 1;
     if (lane == 0) bulk_wait0();
   }
   tc_fence_before();
-  __syncthreads();
+  if (PAIR) cluster_sync();
+  else __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    if (PAIR) tmem_dealloc_pair(tmem, 512);
+    else tmem_dealloc(tmem, 512);
   }
 }
 
@@ -509,16 +599,6 @@ __global__ void __launch_bounds__(256) lora_shrink_kernel(const __grid_constant_
 #pragma unroll
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (lane == 0) p.T[m * p.r + j] = __ldg(p.scale + a) * s;
-}
-
-template <bool BF16>
-__device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if (BF16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 // 16 columns of Y for MT * 8 rows per block; the 8 warps take 32-wide K blocks in turn and are summed in shared memory.
@@ -611,53 +691,95 @@ int launch_skinny(Ctx* c, const LoraParams& p) {
   return check_launch(c, "linear_lora");
 }
 
+// CTA pairs that can be resident at once (both SMs of a pair lie in one GPC), per device.
+template <bool BF16>
+int resident_pairs(Ctx* c) {
+  static int known[32] = {};
+  int& n = known[c->device & 31];
+  if (n) return n;
+  int got = 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * (c->num_sms / 2));
+  cfg.blockDim = dim3(kLThreads);
+  cfg.dynamicSmemBytes = 232448;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&got, lora_tile_kernel<BF16, true>, &cfg) != cudaSuccess || got < 1) got = c->num_sms / 4;
+  cudaGetLastError();
+  return n = std::min(got, c->num_sms / 2);
+}
+
 template <bool BF16>
 int launch_tiles(Ctx* c, LoraParams& p) {
-  p.rp = (p.r + 15) / 16 * 16;
-  p.slots = std::max(1, std::min(64 / p.rp, p.L));
-  p.mt = (p.M + 127) / 128;
-  const int t_cols = (p.slots * p.rp + 31) / 32 * 32;
-  // Column width: the K loop of a unit costs about its MMA columns or its stage's bytes over the shared-memory fill rate,
-  // whichever is more, and a unit some 2500 cycles besides; the widest tile does not always fill the SMs.
-  double best = 1e30;
-  for (int bn = 32; bn <= 192 && bn + t_cols <= 256; bn += 32) {
-    const int nt = (p.N + bn - 1) / bn;
-    const double rounds = (double)(((long long)p.mt * nt + c->num_sms - 1) / c->num_sms);
-    const double kb = std::max<double>(bn + p.rp, (16384 + (bn + p.rp) * 128) / 90.0);
-    const double cost = rounds * (p.K / 64 * kb + 500.0) + 2000.0;
-    if (cost < best * 0.999) {
-      best = cost;
-      p.BN = bn;
-      p.nt = nt;
-    }
-  }
-  p.stage_bytes = 16384 + (p.BN + p.slots * p.rp) * 128;
-  p.stage_bytes = (p.stage_bytes + 1023) / 1024 * 1024;
-  p.stages = (int)std::min<uint32_t>(kMaxStages, (232448 - kFixedSmem) / p.stage_bytes);
-  const uint32_t smem = kFixedSmem + p.stages * p.stage_bytes;
-  const CUtensorMapDataType dt = BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  const uint64_t xd[2] = {(uint64_t)p.K, (uint64_t)p.M}, wd[2] = {(uint64_t)p.K, (uint64_t)p.N};
-  const uint64_t ad[3] = {(uint64_t)p.K, (uint64_t)p.r, (uint64_t)p.L}, bd[3] = {(uint64_t)p.r, (uint64_t)p.N, (uint64_t)p.L};
-  const uint64_t yd[2] = {(uint64_t)p.N, (uint64_t)p.M};
-  const uint64_t xs[1] = {(uint64_t)p.ldx * 2}, wst[1] = {(uint64_t)p.K * 2}, ys[1] = {(uint64_t)p.ldy * 2};
-  const uint64_t as[2] = {(uint64_t)p.K * 2, (uint64_t)p.r * p.K * 2}, bs[2] = {(uint64_t)p.r * 2, (uint64_t)p.N * p.r * 2};
-  const uint32_t xb[2] = {64, 128}, wb[2] = {64, (uint32_t)p.BN}, ab[3] = {64, (uint32_t)p.rp, 1}, bb[3] = {64, (uint32_t)p.BN, 1},
-                 yb[2] = {32, 32};
-  std::string err;
-  if (!make_tmap(&p.tmX, dt, 2, p.X, xd, xs, xb, CU_TENSOR_MAP_SWIZZLE_128B, &err) ||
-      !make_tmap(&p.tmW, dt, 2, p.W, wd, wst, wb, CU_TENSOR_MAP_SWIZZLE_128B, &err) ||
-      !make_tmap(&p.tmA, dt, 3, p.A, ad, as, ab, CU_TENSOR_MAP_SWIZZLE_128B, &err) ||
-      !make_tmap(&p.tmB, dt, 3, p.B, bd, bs, bb, CU_TENSOR_MAP_SWIZZLE_128B, &err) ||
-      !make_tmap(&p.tmY, dt, 2, p.Y, yd, ys, yb, CU_TENSOR_MAP_SWIZZLE_64B, &err))
-    return set_error(c, DI_EINVAL, "linear_lora: " + err);
-  auto kern = lora_tile_kernel<BF16>;
   static unsigned attr_done = 0;
   if (!(attr_done & (1u << (c->device & 31)))) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448) != cudaSuccess)
+    if (cudaFuncSetAttribute(lora_tile_kernel<BF16, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448) != cudaSuccess ||
+        cudaFuncSetAttribute(lora_tile_kernel<BF16, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448) != cudaSuccess)
       return set_error(c, DI_ECUDA, "linear_lora: shared memory attribute");
     attr_done |= 1u << (c->device & 31);
   }
-  launch_k(kern, dim3((unsigned)std::min<long long>((long long)p.mt * p.nt, c->num_sms)), kLThreads, smem, c->stream, p);
+  // Column width and pairing: a K block takes 2 BN cycles of MMAs or its stage's bytes at some 45 bytes a cycle from L2,
+  // whichever is more; a tile's epilogue (about 9 cycles a column and CTA) runs under the next main loop; the last
+  // tile's and the first loads do not.
+  bool pair = false;
+  double best = 1e30;
+  const int pairs = resident_pairs<BF16>(c);
+  for (int pr = 0; pr < 2; ++pr) {
+    const int mt = pr ? (p.M + 255) / 256 : (p.M + 127) / 128;
+    for (int bn = 256; bn >= 32; bn -= 32) {
+      const int nt = (p.N + bn - 1) / bn, slots = pr ? pairs : c->num_sms;
+      const double rounds = (double)(((long long)mt * nt + slots - 1) / slots);
+      const double kb = std::max(2.0 * bn, (128 + (pr ? bn / 2 : bn)) * 128 / 45.0);
+      const double loop = (p.K / 64 + 1) * kb, epi = 9.0 * bn;
+      const double cost = rounds * std::max(loop, epi) + epi + 1500.0;
+      if (cost < best * 0.999) {
+        best = cost;
+        p.BN = bn;
+        p.nt = nt;
+        p.mt = mt;
+        pair = pr != 0;
+      }
+    }
+  }
+  const int b_rows = pair ? p.BN / 2 : p.BN;
+  p.stage_bytes = (16384 + b_rows * 128 + 1023) / 1024 * 1024;
+  p.stages = (int)std::min<uint32_t>(kMaxStages, (232448 - kFixedSmem) / p.stage_bytes);
+  const uint32_t smem = kFixedSmem + p.stages * p.stage_bytes;
+  p.t_ld = p.r <= 32 ? 64 : (p.r + 63) / 64 * 128;
+  const CUtensorMapDataType dt = BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const uint64_t M = p.M, N = p.N, K = p.K, r = p.r, tl = p.t_ld;
+  const uint64_t xd[2] = {K, M}, wd[2] = {K, N}, td[2] = {tl, M}, bd[3] = {r, N, (uint64_t)p.L}, yd[2] = {N, M};
+  const uint64_t xs[1] = {(uint64_t)p.ldx * 2}, ws[1] = {K * 2}, ts[1] = {tl * 2}, bs[2] = {r * 2, N * r * 2};
+  const uint64_t rs[1] = {(uint64_t)p.ldr * 2}, ys[1] = {(uint64_t)p.ldy * 2};
+  const uint32_t xb[2] = {64, 128}, wb[2] = {64, (uint32_t)b_rows}, bb[3] = {64, (uint32_t)b_rows, 1}, yb[2] = {32, 32};
+  std::string err;
+  if (!make_tmap(&p.tmX, dt, 2, p.X, xd, xs, xb, CU_TENSOR_MAP_SWIZZLE_128B, &err) ||
+      !make_tmap(&p.tmW, dt, 2, p.W, wd, ws, wb, CU_TENSOR_MAP_SWIZZLE_128B, &err) ||
+      !make_tmap(&p.tmT, dt, 2, p.T16, td, ts, xb, CU_TENSOR_MAP_SWIZZLE_128B, &err) ||
+      !make_tmap(&p.tmB, dt, 3, p.B, bd, bs, bb, CU_TENSOR_MAP_SWIZZLE_128B, &err) ||
+      (p.R && !make_tmap(&p.tmR, dt, 2, p.R, yd, rs, yb, CU_TENSOR_MAP_SWIZZLE_64B, &err)) ||
+      !make_tmap(&p.tmY, dt, 2, p.Y, yd, ys, yb, CU_TENSOR_MAP_SWIZZLE_64B, &err))
+    return set_error(c, DI_EINVAL, "linear_lora: " + err);
+  // 64 rows a block reads the adapters least often; few rows take 16 so that the SMs are filled
+  const int rg = (p.r + 31) / 32;
+  if ((long long)p.M * rg >= 128LL * c->num_sms)
+    launch_k(lora_t_kernel<BF16, 64, 32>, dim3(rg, (p.M + 63) / 64), 256, 0, c->stream, p);
+  else
+    launch_k(lora_t_kernel<BF16, 16, 16>, dim3(rg, (p.M + 15) / 16), 256, 0, c->stream, p);
+  const int rc = check_launch(c, "linear_lora");
+  if (rc != DI_OK) return rc;
+  const long long units = (long long)p.mt * p.nt;
+  if (pair)
+    launch_k_cluster(lora_tile_kernel<BF16, true>, dim3(2 * (unsigned)std::min<long long>(units, pairs)), dim3(kLThreads), smem,
+                     c->stream, 2, p);
+  else
+    launch_k(lora_tile_kernel<BF16, false>, dim3((unsigned)std::min<long long>(units, c->num_sms)), dim3(kLThreads), smem,
+             c->stream, p);
   return check_launch(c, "linear_lora");
 }
 
@@ -667,8 +789,9 @@ int launch_tiles(Ctx* c, LoraParams& p) {
 using namespace di;
 
 extern "C" size_t di_linear_lora_workspace(di_ctx_t h, int M, int N, int K, int rank, int n_adapters) {
-  if (!h || M <= 0 || rank <= 0 || M > kSkinnyRows) return 0;
-  return (size_t)M * rank * 4;
+  if (!h || M <= 0 || rank <= 0) return 0;
+  if (M <= kSkinnyRows) return (size_t)M * rank * 4;
+  return (size_t)M * (rank <= 32 ? 64 : (rank + 63) / 64 * 128) * 2;
 }
 
 extern "C" int di_linear_lora(di_ctx_t h, int dtype, const void* X, long long ldx, int M, int K, const void* W, int N,
@@ -688,7 +811,7 @@ extern "C" int di_linear_lora(di_ctx_t h, int dtype, const void* X, long long ld
   if (!aligned16(X) || !aligned16(W) || !aligned16(A) || !aligned16(B) || !aligned16(R) || !aligned16(Y) || ldx % 8 ||
       ldy % 8 || (R && ldr % 8))
     return set_error(c, DI_EINVAL, "linear_lora: pointers must be 16-byte aligned, row strides multiples of 8 elements");
-  if ((long long)((M + 127LL) / 128) * ((N + 31) / 32) > 0x7fffffffll)
+  if ((M + 127LL) / 128 * ((N + 31) / 32) > 0x7fffffffll || (M + 15LL) / 16 > 65535)
     return set_error(c, DI_EUNSUPPORTED, "linear_lora: too many rows and columns");
   const size_t need = di_linear_lora_workspace(h, M, N, K, rank, n_adapters);
   if (need && (!ws || ws_bytes < need || !aligned16(ws)))
@@ -701,6 +824,7 @@ extern "C" int di_linear_lora(di_ctx_t h, int dtype, const void* X, long long ld
   p.scale = scale; p.bias = bias; p.rows = row_adapter; p.act = act;
   p.err = c->d_err;
   p.T = static_cast<float*>(ws);
+  p.T16 = static_cast<uint16_t*>(ws);
   if (M <= kSkinnyRows) return dtype == DI_F16 ? launch_skinny<false>(c, p) : launch_skinny<true>(c, p);
   return dtype == DI_F16 ? launch_tiles<false>(c, p) : launch_tiles<true>(c, p);
 }
