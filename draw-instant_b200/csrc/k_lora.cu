@@ -11,13 +11,16 @@
 //
 // Tiles (M > kSkinnyRows): T is kept as two 16-bit parts, hi + lo (2^-17 relative for bf16), and is simply more of K:
 // after the K blocks of X and W come, for every adapter that the tile's rows name, a block of [T_hi | T_lo] against that
-// adapter's B.  Its MMAs write the accumulator rows that name the adapter and no others (the output-lane mask of
-// tcgen05.mma), so a tile may mix adapters at the price of a block each, and an adapter's infinities stay with its rows.
+// adapter's B, with the T rows of other adapters zeroed in shared memory.  A tile may so mix adapters at the price of a
+// block each.  (tcgen05.mma's own mask of output lanes would spare the zeroing, but a masked MMA took some 1000 cycles, whatever
+// its width, against 80 to 128 for a plain one.)  Zero times an infinity or NaN in another adapter's B is NaN: outputs
+// that are not finite in a tile of several adapters are computed again from their own row's terms alone.
 // One persistent CTA per SM, or CTA pair (cta_group::2: 256 rows, each CTA loads half of B):
 //   warp 0       TMA loads through one ring of stages
 //   warp 1       MMA issue (the pair's first CTA)
 //   warp 2       the tile's distinct adapters and the rows of each
-//   warps 4-11   epilogue: bias, activation, residual (fetched by TMA during the main loop), stores by TMA
+//   warp 3       zeroes other adapters' rows of a T block
+//   warps 4-15   epilogue: bias, activation, residual (fetched by TMA during the main loop), stores by TMA
 // The accumulator is double-buffered, so a tile's epilogue runs under the next one's main loop.
 //
 // Few rows (M <= kSkinnyRows): T in 32 bits; the second launch streams W once from memory into mma.sync fragments (16
@@ -31,7 +34,7 @@
 namespace di {
 
 struct LoraParams {
-  CUtensorMap tmX, tmW, tmT, tmB, tmR, tmY;
+  CUtensorMap tmX, tmW, tmA, tmT, tmB, tmR, tmY;
   const void *X, *W, *A, *B, *R;
   void* Y;
   long long ldx, ldr, ldy;
@@ -43,6 +46,8 @@ struct LoraParams {
   // tiles
   int BN, stages, mt, nt;
   uint32_t stage_bytes;
+  int tslots, tstages;  // first kernel: adapters per pass
+  uint32_t tstage_bytes;
   uint16_t* T16;  // [M][t_ld]: 64-column groups, hi and lo parts of 32 ranks (r <= 32) or of 64 in two groups
   int t_ld;
   // few rows
@@ -52,11 +57,12 @@ struct LoraParams {
 namespace {
 
 constexpr int kSkinnyRows = 128;
-constexpr int kLThreads = 384;
+constexpr int kEpi = 12;           // epilogue warps: three share a quarter of the rows, 32-column chunks in turn
+constexpr int kLThreads = 128 + 32 * kEpi, kTThreads = 256;
 constexpr int kMaxStages = 12;
 constexpr int kSlots = 32;        // adapters per list entry
 constexpr int kLists = 3;
-constexpr int kSlabs = 3;         // residual / output slabs per epilogue warp
+constexpr int kSlabs = 2;         // residual / output slabs per epilogue warp
 constexpr uint32_t kSlab = 2048;  // 32 x 32 16-bit values
 
 struct SlotList {
@@ -65,26 +71,16 @@ struct SlotList {
   uint32_t others[kSlots][8];  // rows of the tile (accumulator lanes) that do not name the adapter
 };
 constexpr uint32_t kListBytes = (kLists * sizeof(SlotList) + 15) / 16 * 16;
-constexpr uint32_t kBarBytes = 8 * (2 * kMaxStages + 2 * kLists + 4 + 8 * kSlabs) + 16;
-constexpr uint32_t kFixedSmem = 1024 + 8 * kSlabs * kSlab + 8 * 128 + kListBytes + (kBarBytes + 15) / 16 * 16;
+constexpr uint32_t kBarBytes = 8 * (4 * kMaxStages + 2 * kLists + 4 + kEpi * kSlabs) + 16;
+constexpr uint32_t kTFixedSmem = 1024 + kListBytes + 8 * (2 * kMaxStages + 2 * kLists + 4) + 32;
+constexpr uint32_t kFixedSmem = 1024 + kEpi * kSlabs * kSlab + kEpi * 384 + kListBytes + (kBarBytes + 15) / 16 * 16;
 
-// As umma_f16 / umma_f16_pair, adding to D in all lanes but those of `off` (bit l of word w: row 32 w + l).
-template <bool PAIR>
-__device__ __forceinline__ void umma_f16_rows(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                              const uint32_t* off) {
-  if (PAIR)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.eq.b32 p, 0, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, "
-        "{%4, %5, %6, %7, %8, %9, %10, %11}, p;\n\t}\n"
-        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3]), "r"(off[4]),
-          "r"(off[5]), "r"(off[6]), "r"(off[7])
-        : "memory");
-  else
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.eq.b32 p, 0, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, "
-        "{%4, %5, %6, %7}, p;\n\t}\n"
-        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3])
-        : "memory");
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
 }
 template <bool PAIR>
 __device__ __forceinline__ void load_2d(void* dst, const CUtensorMap* m, uint32_t bar, int c0, int c1) {
@@ -123,7 +119,18 @@ template <bool BF16>
 __device__ __forceinline__ float2 unpack2(uint32_t w) {
   return BF16 ? __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&w)) : __half22float2(*reinterpret_cast<__half2*>(&w));
 }
-__device__ __forceinline__ float act_of(float v, int act) { return act == 1 ? silu_f(v) : act == 2 ? gelu_erf(v) : v; }
+// SiLU and erf GELU (erf by Abramowitz & Stegun 7.1.26, as gelu_erf) with the approximate division: the exact one's
+// branches cost four times the rest of the epilogue.
+__device__ __forceinline__ float act_of(float v, int act) {
+  if (act == 1) return __fdividef(v, 1.0f + __expf(-v));
+  if (act == 2) {
+    const float x = v * 0.70710678f, a = fabsf(x), t = __fdividef(1.0f, fmaf(0.3275911f, a, 1.0f));
+    const float y = (((1.061405429f * t - 1.453152027f) * t + 1.421413741f) * t - 0.284496736f) * t + 0.254829592f;
+    const float e = 1.0f - y * t * __expf(-a * a);
+    return 0.5f * v * (1.0f + copysignf(e, x));
+  }
+  return v;
+}
 template <bool BF16>
 __device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if (BF16)
@@ -145,121 +152,299 @@ struct Ring {
   }
 };
 
+// K-major operand descriptor of a 128-byte-swizzled tile at shared address `a`; + 2 steps 16 values along K.
+__device__ __forceinline__ uint64_t kdesc(uint32_t a) { return sdesc_sw128(0, 16, 1024) | (a >> 4); }
+
+// Bounded wait that also ends when another role has given up; the flag is read only when the phase is not there yet.
+template <bool CLUSTER>
+__device__ __forceinline__ bool wait_on(uint64_t* bar, int ph, volatile int* abort_flag, int* err, int code) {
+  const uint32_t a = smem_u32(bar);
+  if (CLUSTER ? mbar_try_wait_cluster(a, ph) : mbar_try_wait(a, ph)) return true;
+  return !*abort_flag && mbar_wait<CLUSTER>(bar, ph, err, code);
+}
+
+// One warp lists a tile's adapters (rows m0 .. m0 + 32 RL - 1), at most `most` to an entry, with the rows that do not
+// name each.  Every tile has one entry at least.
+template <int RL>
+__device__ __forceinline__ void rows_of(const LoraParams& p, int m0, int lane, int (&a)[RL]) {
+#pragma unroll
+  for (int i = 0; i < RL; ++i) {
+    const int m = m0 + i * 32 + lane;
+    a[i] = m < p.M && m0 >= 0 ? __ldg(p.rows + m) : -1;
+  }
+}
+// `next` holds the rows' adapters on entry, and those of the tile at next_m0 (-1: none) on return: a load under the
+// traffic of the streams takes microseconds, so it is made a tile ahead.
+template <int RL>
+__device__ __forceinline__ bool list_adapters(const LoraParams& p, int next_m0, int (&next)[RL], int most, SlotList* lists,
+                                              uint64_t* list_full, uint64_t* list_empty, Ring& li,
+                                              volatile int* abort_flag, int lane) {
+  int a[RL];
+#pragma unroll
+  for (int i = 0; i < RL; ++i) {
+    a[i] = next[i];
+    if (a[i] >= p.L) {
+      atomicOr(p.err, DEVERR_BOUNDS);
+      a[i] = -1;
+    }
+  }
+  rows_of<RL>(p, next_m0, lane, next);
+  int n = 0;
+  auto open_entry = [&] {
+    n = 0;
+    return __all_sync(0xffffffffu, wait_on<false>(&list_empty[li.s], li.ph ^ 1, abort_flag, p.err, DEVERR_WAIT_EPI)) != 0;
+  };
+  auto close_entry = [&](int more) {
+    if (lane == 0) {
+      lists[li.s].n = n;
+      lists[li.s].more = more;
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&list_full[li.s]);
+    li.advance(kLists);
+  };
+  if (!open_entry()) return false;
+#pragma unroll
+  for (int i = 0; i < RL; ++i) {
+    unsigned open;
+    while ((open = __ballot_sync(0xffffffffu, a[i] >= 0)) != 0) {
+      if (n == most) {
+        close_entry(1);
+        if (!open_entry()) return false;
+      }
+      const int id = __shfl_sync(0xffffffffu, a[i], __ffs(open) - 1);
+#pragma unroll
+      for (int k = 0; k < RL; ++k) {
+        const unsigned o = __ballot_sync(0xffffffffu, a[k] != id);
+        if (a[k] == id) a[k] = -1;
+        if (lane == 0) lists[li.s].others[n][k] = o;
+      }
+      if (lane == 0) lists[li.s].ids[n] = id;
+      ++n;
+    }
+  }
+  close_entry(0);
+  return true;
+}
+
 // ---- tiles: T = scale X A^T in two 16-bit parts ----
 
-// ROWS rows of X by 32 ranks per block; the warps are KW shares of K by ROWS / RW groups of RW rows, summed in shared memory.
-// A lane's 16-byte loads of 8 consecutive k stand for two 16-wide MMA steps: both operands use the same order of k.
-// Bound: the bytes of X; the rows' adapters come from L2, once per block for each adapter its rows name.
-template <bool BF16, int ROWS, int RW>
-__global__ void __launch_bounds__(256) lora_t_kernel(const __grid_constant__ LoraParams p) {
-  constexpr int KW = 8 * RW / ROWS, MT = RW / 8;
-  __shared__ float red[KW][ROWS][33];
-  pdl_begin();
-  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-  const int m0 = blockIdx.y * ROWS, j0 = blockIdx.x * 32;
-  const int kw = warp % KW, rw = warp / KW * RW;
-  constexpr int IDS = (ROWS + 31) / 32;
-  int ids[IDS];
-#pragma unroll
-  for (int i = 0; i < IDS; ++i) {
-    const int l = i * 32 + lane;
-    ids[i] = l < ROWS && m0 + l < p.M ? __ldg(p.rows + m0 + l) : -1;
-    if (ids[i] >= p.L) ids[i] = -1;
+// One pass over X per entry of the tile's list (all of its adapters as a rule): the A rows of up to `tslots` adapters are
+// the B operand, side by side, and every row keeps its own adapter's columns.  Bound: the bytes of X, which five
+// stages per SM stream (more only lengthen the queue that every load waits in).
+//   warp 0 TMA loads, warp 1 MMA issue, warp 2 lists, warps 4-7 T out of TMEM, one row per thread
+template <bool BF16>
+__global__ void __launch_bounds__(kTThreads, 1) lora_t_kernel(const __grid_constant__ LoraParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sStage = smem;  // [tstages]: 128 rows of X, then the adapters' rows, 128 bytes each
+  SlotList* lists = reinterpret_cast<SlotList*>(smem + p.tstages * p.tstage_bytes);
+  uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(lists) + kListBytes);  // [kMaxStages]
+  uint64_t* empty = full + kMaxStages;         // [kMaxStages]
+  uint64_t* list_full = empty + kMaxStages;    // [kLists]
+  uint64_t* list_empty = list_full + kLists;   // [kLists]
+  uint64_t* d_full = list_empty + kLists;      // [2]
+  uint64_t* d_empty = d_full + 2;              // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(d_empty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < p.tstages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+    for (int i = 0; i < kLists; ++i) { mbar_init(&list_full[i], 1); mbar_init(&list_empty[i], 6); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&d_full[i], 1); mbar_init(&d_empty[i], 4); }
+    *abort_flag = 0;
+    fence_mbar_init();
   }
-  const uint16_t* xr[MT];
-#pragma unroll
-  for (int t = 0; t < MT; ++t)  // rows past the last are computed and not stored
-    xr[t] = static_cast<const uint16_t*>(p.X) + min(m0 + rw + t * 8 + lane / 4, p.M - 1) * p.ldx + (lane & 3) * 8;
-#pragma unroll
-  for (int i = 0; i < IDS; ++i) {
-    unsigned open;
-    while ((open = __ballot_sync(0xffffffffu, ids[i] >= 0)) != 0) {  // the same in every warp of the block
-      const int id = __shfl_sync(0xffffffffu, ids[i], __ffs(open) - 1);
-      unsigned mine[IDS];
-#pragma unroll
-      for (int k = 0; k < IDS; ++k) {
-        mine[k] = __ballot_sync(0xffffffffu, ids[k] == id);
-        if (ids[k] == id) ids[k] = -1;
-      }
-      float acc[2][MT][4] = {};
-      const uint16_t* ar[4];  // ranks j0 + 8 i + lane / 4; those past the last read the last and are dropped
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        ar[k] = static_cast<const uint16_t*>(p.A) + ((long long)id * p.r + min(j0 + k * 8 + lane / 4, p.r - 1)) * p.K +
-                (lane & 3) * 8;
-#pragma unroll 2
-      for (int k = kw * 32; k < p.K; k += KW * 32) {
-        uint4 a[4], b[MT];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) a[q] = __ldg(reinterpret_cast<const uint4*>(ar[q] + k));
-#pragma unroll
-        for (int t = 0; t < MT; ++t) b[t] = __ldg(reinterpret_cast<const uint4*>(xr[t] + k));
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const uint32_t f0[4] = {a[2 * q].x, a[2 * q + 1].x, a[2 * q].y, a[2 * q + 1].y};
-          const uint32_t f1[4] = {a[2 * q].z, a[2 * q + 1].z, a[2 * q].w, a[2 * q + 1].w};
-#pragma unroll
-          for (int t = 0; t < MT; ++t) {
-            mma_16x8x16<BF16>(acc[q][t], f0, b[t].x, b[t].y);
-            mma_16x8x16<BF16>(acc[q][t], f1, b[t].z, b[t].w);
+  if (warp == 1) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;  // accumulator ab at column 256 ab
+  pdl_begin();
+  const int tiles = (p.M + 127) / 128, nk = p.K / 64, rp = (p.r + 15) / 16 * 16;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      tma_prefetch_desc(&p.tmX);
+      tma_prefetch_desc(&p.tmA);
+      Ring st, li;
+      bool ok = true;
+      unsigned issued = 0;
+      for (int u = blockIdx.x; ok && u < tiles; u += gridDim.x)
+        for (bool more = true; ok && more;) {
+          if (!(ok = wait_on<false>(&list_full[li.s], li.ph, abort_flag, p.err, DEVERR_WAIT_TMA))) break;
+          const SlotList& l = lists[li.s];
+          more = l.more;
+          for (int kb = 0; l.n && kb < nk; ++kb) {
+            if (!(ok = wait_on<false>(&empty[st.s], st.ph ^ 1, abort_flag, p.err, DEVERR_WAIT_TMA))) break;
+            uint8_t* d = sStage + st.s * p.tstage_bytes;
+            mbar_arrive_expect_tx(&full[st.s], 16384u + (uint32_t)(l.n * rp) * 128u);
+            tma_load_2d(d, &p.tmX, &full[st.s], kb * 64, u * 128);
+            for (int g = 0; g < l.n; ++g)
+              load_3d<false>(d + 16384 + g * rp * 128, &p.tmA, smem_u32(&full[st.s]), kb * 64, 0, l.ids[g]);
+            st.advance(p.tstages);
+            ++issued;
           }
+          mbar_arrive(&list_empty[li.s]);
+          li.advance(kLists);
+        }
+      if (!ok) {  // leave no copy in flight behind
+        *abort_flag = 1;
+        for (unsigned i = 0; i < min(issued, (unsigned)p.tstages); ++i) {
+          st.back(p.tstages);
+          mbar_wait(&full[st.s], st.ph, p.err, DEVERR_WAIT_TMA);
         }
       }
-#pragma unroll
-      for (int q = 0; q < 2; ++q)
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {  // d[0..1]: rank lane / 4, rows 2 (lane & 3) + {0, 1}; d[2..3]: rank + 8
-          const int m = rw + t * 8 + (lane & 3) * 2, j = q * 16 + lane / 4;
-          red[kw][m][j] = acc[q][t][0];
-          red[kw][m + 1][j] = acc[q][t][1];
-          red[kw][m][j + 8] = acc[q][t][2];
-          red[kw][m + 1][j + 8] = acc[q][t][3];
-        }
-      __syncthreads();
-      const float sc = __ldg(p.scale + id);
-      for (int o = threadIdx.x; o < ROWS * 16; o += 256) {  // two ranks each
-        const int m = o / 16, j = o % 16 * 2;
-        if (!((mine[m / 32] >> (m % 32)) & 1)) continue;
-        const int rank = j0 + j;
-        if (rank >= (p.r + 15) / 16 * 16) continue;
-        float x = 0.f, y = 0.f;
-#pragma unroll
-        for (int k = 0; k < KW; ++k) { x += red[k][m][j]; y += red[k][m][j + 1]; }
-        x *= sc;
-        y *= sc;
-        if (rank >= p.r) x = y = 0.f;  // the last 16-wide step's empty half (r is a multiple of 8)
-        const uint32_t hi = pack2<BF16>(x, y);
-        const float2 h = unpack2<BF16>(hi);
-        // a part that is not finite stands alone (inf - inf would be NaN)
-        const uint32_t lo = pack2<BF16>(isinf(h.x) ? 0.f : x - h.x, isinf(h.y) ? 0.f : y - h.y);
-        const int half = p.r <= 32 ? 32 : 64;
-        uint16_t* t = p.T16 + (long long)(m0 + m) * p.t_ld + rank / half * (2 * half) + rank % half;
-        *reinterpret_cast<uint32_t*>(t) = hi;
-        *reinterpret_cast<uint32_t*>(t + half) = lo;
-      }
-      __syncthreads();
     }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      Ring st, li, ac;
+      bool ok = true;
+      for (int u = blockIdx.x; ok && u < tiles; u += gridDim.x)
+        for (bool more = true; ok && more;) {
+          if (!(ok = wait_on<false>(&list_full[li.s], li.ph, abort_flag, p.err, DEVERR_WAIT_MMA))) break;
+          const int n = lists[li.s].n;
+          more = lists[li.s].more;
+          mbar_arrive(&list_empty[li.s]);
+          li.advance(kLists);
+          if (!n) continue;
+          ok = wait_on<false>(&d_empty[ac.s], ac.ph ^ 1, abort_flag, p.err, DEVERR_WAIT_MMA);
+          const uint32_t d = tmem + ac.s * 256, id = idesc_f16(128, 0, BF16) | ((uint32_t)(n * rp >> 3) << 17);
+          for (int kb = 0; ok && kb < nk; ++kb) {
+            if (!(ok = wait_on<false>(&full[st.s], st.ph, abort_flag, p.err, DEVERR_WAIT_MMA))) break;
+            tc_fence_after();
+            const uint64_t x = kdesc(smem_u32(sStage + st.s * p.tstage_bytes)), w = x + (16384 >> 4);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) umma_f16(d, x + 2 * k, w + 2 * k, id, (kb | k) != 0);
+            umma_commit(&empty[st.s]);
+            st.advance(p.tstages);
+          }
+          if (ok) umma_commit(&d_full[ac.s]);
+          ac.advance(2);
+        }
+      if (!ok) *abort_flag = 1;
+    }
+  } else if (warp == 2) {
+    Ring li;
+    bool ok = true;
+    int rows[4];
+    rows_of<4>(p, blockIdx.x * 128, lane, rows);
+    for (int u = blockIdx.x; ok && u < tiles; u += gridDim.x)
+      ok = list_adapters<4>(p, u + (int)gridDim.x < tiles ? (u + (int)gridDim.x) * 128 : -1, rows, p.tslots, lists,
+                            list_full, list_empty, li, abort_flag, lane);
+    if (!ok) *abort_flag = 1;
+  } else if (warp >= 4) {
+    const int q = warp & 3;
+    const int half = p.r <= 32 ? 32 : 64;
+    Ring li, ac;
+    bool ok = true;
+    for (int u = blockIdx.x; ok && u < tiles; u += gridDim.x) {
+      const int m = u * 128 + q * 32 + lane;
+      for (bool more = true; ok && more;) {
+        ok = wait_on<false>(&list_full[li.s], li.ph, abort_flag, p.err, DEVERR_WAIT_EPI);
+        if (!(ok = __all_sync(0xffffffffu, ok))) break;
+        const SlotList& l = lists[li.s];
+        const int n = l.n;
+        more = l.more;
+        if (n) {
+          ok = wait_on<false>(&d_full[ac.s], ac.ph, abort_flag, p.err, DEVERR_WAIT_EPI);
+          if (!(ok = __all_sync(0xffffffffu, ok))) break;
+          tc_fence_after();
+          const uint32_t d = tmem + ac.s * 256 + (static_cast<uint32_t>(q * 32) << 16);
+          for (int g = 0; g < n; ++g) {
+            const uint32_t others = l.others[g][q];
+            if (others == 0xffffffffu) continue;  // none of this warp's rows
+            const bool mine = m < p.M && !((others >> lane) & 1);
+            const float sc = __ldg(p.scale + l.ids[g]);
+            for (int c = 0; c < rp; c += 16) {
+              uint32_t r[16];
+              tmem_ld16(d + g * rp + c, r);
+              tmem_wait_ld();
+              if (mine) {
+                uint32_t hi[8], lo[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                  const float x = sc * __uint_as_float(r[2 * k]), y = sc * __uint_as_float(r[2 * k + 1]);
+                  hi[k] = pack2<BF16>(x, y);
+                  const float2 h = unpack2<BF16>(hi[k]);
+                  // a part that is not finite stands alone (inf - inf would be NaN)
+                  lo[k] = pack2<BF16>(isinf(h.x) ? 0.f : x - h.x, isinf(h.y) ? 0.f : y - h.y);
+                }
+                uint4* t = reinterpret_cast<uint4*>(p.T16 + (long long)m * p.t_ld + c / half * (2 * half) + c % half);
+                t[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                t[1] = make_uint4(hi[4], hi[5], hi[6], hi[7]);
+                t[half / 8] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                t[half / 8 + 1] = make_uint4(lo[4], lo[5], lo[6], lo[7]);
+              }
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&d_empty[ac.s]);
+          ac.advance(2);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&list_empty[li.s]);
+        li.advance(kLists);
+      }
+    }
+    if (!ok) *abort_flag = 1;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
   }
 }
 
 // ---- tiles: Y ----
+
+// X[m] . W[n] + T[m] . B[a][n] of one row, from its own terms: lane l returns column n0 + l.
+template <bool BF16>
+__device__ __noinline__ float own_terms(const LoraParams& p, int m, int n0, int lane) {
+  const int n = n0 + lane, a = __ldg(p.rows + m);
+  if (n >= p.N) return 0.f;
+  const uint16_t* x = static_cast<const uint16_t*>(p.X) + m * p.ldx;
+  const uint16_t* w = static_cast<const uint16_t*>(p.W) + (long long)n * p.K;
+  float s = 0.f;
+  for (int k = 0; k < p.K; k += 2) {
+    const float2 f = unpack2<BF16>(*reinterpret_cast<const uint32_t*>(x + k));
+    const float2 g = unpack2<BF16>(*reinterpret_cast<const uint32_t*>(w + k));
+    s = fmaf(f.x, g.x, fmaf(f.y, g.y, s));
+  }
+  if (a >= 0 && a < p.L) {
+    const int half = p.r <= 32 ? 32 : 64;
+    const uint16_t* t = p.T16 + (long long)m * p.t_ld;
+    const uint16_t* b = static_cast<const uint16_t*>(p.B) + ((long long)a * p.N + n) * p.r;
+    for (int j = 0; j < p.r; ++j) {
+      const int at = j / half * (2 * half) + j % half;
+      const float tj = unpack2<BF16>(t[at]).x + unpack2<BF16>(t[at + half]).x;
+      s = fmaf(tj, unpack2<BF16>(b[j]).x, s);
+    }
+  }
+  return s;
+}
+
 
 template <bool BF16, bool PAIR>
 __global__ void __launch_bounds__(kLThreads, 1) lora_tile_kernel(const __grid_constant__ LoraParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sStage = smem;                            // [stages]: 128 rows of X or T, then rows of W or B, 128 bytes each
-  uint8_t* sSlab = smem + p.stages * p.stage_bytes;  // [8][kSlabs]
-  float* sBias = reinterpret_cast<float*>(sSlab + 8 * kSlabs * kSlab);  // [8][32]
-  SlotList* lists = reinterpret_cast<SlotList*>(sBias + 8 * 32);
+  uint8_t* sSlab = smem + p.stages * p.stage_bytes;  // [kEpi][kSlabs]
+  float* sBias = reinterpret_cast<float*>(sSlab + kEpi * kSlabs * kSlab);  // [kEpi][3 chunks][32]
+  SlotList* lists = reinterpret_cast<SlotList*>(sBias + kEpi * 96);
   uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(lists) + kListBytes);  // [kMaxStages]
   uint64_t* empty = full + kMaxStages;         // [kMaxStages]
-  uint64_t* list_full = empty + kMaxStages;    // [kLists]
+  uint64_t* t_full = empty + kMaxStages;       // [kMaxStages] this CTA's T rows landed
+  uint64_t* t_clean = t_full + kMaxStages;     // [kMaxStages] other adapters' rows zeroed (a pair: both CTAs', on the first's)
+  uint64_t* list_full = t_clean + kMaxStages;  // [kLists]
   uint64_t* list_empty = list_full + kLists;   // [kLists]
   uint64_t* d_full = list_empty + kLists;      // [2] accumulator complete
   uint64_t* d_empty = d_full + 2;              // [2] accumulator read (a pair: by both, on the first CTA's)
-  uint64_t* r_full = d_empty + 2;              // [8][kSlabs] residual landed
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(r_full + 8 * kSlabs);
+  uint64_t* r_full = d_empty + 2;              // [kEpi][kSlabs] residual landed
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(r_full + kEpi * kSlabs);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -267,10 +452,16 @@ __global__ void __launch_bounds__(kLThreads, 1) lora_tile_kernel(const __grid_co
   const int first = PAIR ? (int)blockIdx.x / 2 : (int)blockIdx.x, step = PAIR ? (int)gridDim.x / 2 : (int)gridDim.x;
   const bool issues = rank == 0;  // this CTA's warp 1 issues the MMAs
   if (threadIdx.x == 0) {
-    for (int i = 0; i < p.stages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
-    for (int i = 0; i < kLists; ++i) { mbar_init(&list_full[i], 1); mbar_init(&list_empty[i], issues ? 2 : 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&d_full[i], 1); mbar_init(&d_empty[i], PAIR ? 16 : 8); }
-    for (int i = 0; i < 8 * kSlabs; ++i) mbar_init(&r_full[i], 1);
+    for (int i = 0; i < p.stages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+      mbar_init(&t_full[i], 1);
+      mbar_init(&t_clean[i], PAIR ? 2 : 1);
+    }
+    // readers of a list entry: loads, MMAs (where they are issued), zeroing, epilogue
+    for (int i = 0; i < kLists; ++i) { mbar_init(&list_full[i], 1); mbar_init(&list_empty[i], (issues ? 3 : 2) + kEpi); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&d_full[i], 1); mbar_init(&d_empty[i], (PAIR ? 2 : 1) * kEpi); }
+    for (int i = 0; i < kEpi * kSlabs; ++i) mbar_init(&r_full[i], 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -284,6 +475,7 @@ __global__ void __launch_bounds__(kLThreads, 1) lora_tile_kernel(const __grid_co
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const uint32_t full0 = PAIR ? mapa_shared(smem_u32(full), 0) : smem_u32(full);
+  const uint32_t t_clean0 = PAIR ? mapa_shared(smem_u32(t_clean), 0) : smem_u32(t_clean);
   const uint32_t d_empty0 = PAIR ? mapa_shared(smem_u32(d_empty), 0) : smem_u32(d_empty);
   pdl_trigger();
   // lora_t_kernel let this one start after its own wait for earlier kernels: X, W, the indices, R and Y are safe to use
@@ -301,10 +493,16 @@ __global__ void __launch_bounds__(kLThreads, 1) lora_tile_kernel(const __grid_co
       tma_prefetch_desc(&p.tmB);
       Ring st, li;
       bool ok = true, waited = false;
-      unsigned issued = 0;
+      unsigned issued = 0, t_any = 0, t_ph = 0;  // t_ph: phase that the last T copy into a stage completes
+      auto load_t = [&](int col, int m0) {
+        t_ph ^= ((t_any >> st.s) & 1) << st.s;
+        t_any |= 1u << st.s;
+        mbar_arrive_expect_tx(&t_full[st.s], 16384u);
+        tma_load_2d(sStage + st.s * p.stage_bytes, &p.tmT, &t_full[st.s], col, m0);
+      };
       auto stage = [&](uint32_t bytes) {  // the next free stage, armed for `bytes` of each CTA
-        if (*abort_flag || !mbar_wait<PAIR>(&empty[st.s], st.ph ^ 1, p.err, DEVERR_WAIT_TMA)) return false;
-        if (issues) mbar_arrive_expect_tx(&full[st.s], PAIR ? 2 * bytes : bytes);
+        if (!wait_on<PAIR>(&empty[st.s], st.ph ^ 1, abort_flag, p.err, DEVERR_WAIT_TMA)) return false;
+        if (issues) mbar_arrive_expect_tx(&full[st.s], PAIR ? 2 * bytes : bytes);  // 0: nothing but T, on t_full
         ++issued;
         return true;
       };
@@ -318,7 +516,7 @@ __global__ void __launch_bounds__(kLThreads, 1) lora_tile_kernel(const __grid_co
           st.advance(p.stages);
         }
         for (bool more = true; ok && more;) {
-          if (!(ok = !*abort_flag && mbar_wait(&list_full[li.s], li.ph, p.err, DEVERR_WAIT_TMA))) break;
+          if (!(ok = wait_on<false>(&list_full[li.s], li.ph, abort_flag, p.err, DEVERR_WAIT_TMA))) break;
           const SlotList& l = lists[li.s];
           more = l.more;
           if (l.n && !waited) {
@@ -327,14 +525,14 @@ __global__ void __launch_bounds__(kLThreads, 1) lora_tile_kernel(const __grid_co
           }
           for (int g = 0; ok && g < l.n; ++g)
             for (int c = 0; ok && c < groups; ++c) {
-              if (!(ok = stage(16384u + b_rows * 128u))) break;
+              if (!(ok = stage(b_rows * 128u))) break;
               uint8_t* d = sStage + st.s * p.stage_bytes;
-              load_2d<PAIR>(d, &p.tmT, full0 + st.s * 8, c * 128, m0);
+              load_t(c * 128, m0);
               load_3d<PAIR>(d + 16384, &p.tmB, full0 + st.s * 8, c * 64, n0, l.ids[g]);
               st.advance(p.stages);
               if (p.r > 32) {  // the lo parts, against the same B
-                if (!(ok = stage(16384u))) break;
-                load_2d<PAIR>(sStage + st.s * p.stage_bytes, &p.tmT, full0 + st.s * 8, c * 128 + 64, m0);
+                if (!(ok = stage(0u))) break;
+                load_t(c * 128 + 64, m0);
                 st.advance(p.stages);
               }
             }
@@ -348,6 +546,8 @@ __global__ void __launch_bounds__(kLThreads, 1) lora_tile_kernel(const __grid_co
           st.back(p.stages);
           mbar_wait<PAIR>(&full[st.s], st.ph, p.err, DEVERR_WAIT_TMA);
         }
+        for (int i = 0; i < p.stages; ++i)
+          if ((t_any >> i) & 1) mbar_wait(&t_full[i], (t_ph >> i) & 1, p.err, DEVERR_WAIT_TMA);
       }
     }
   } else if (warp == 1) {
@@ -361,45 +561,60 @@ __global__ void __launch_bounds__(kLThreads, 1) lora_tile_kernel(const __grid_co
         else umma_commit(bar);
       };
       auto stage = [&]() {
-        const bool r = !*abort_flag && mbar_wait<PAIR>(&full[st.s], st.ph, p.err, DEVERR_WAIT_MMA);
+        const bool r = wait_on<PAIR>(&full[st.s], st.ph, abort_flag, p.err, DEVERR_WAIT_MMA);
         tc_fence_after();
         return r;
+      };
+      unsigned ph_c = 0;  // phases of t_clean, one bit per stage
+      auto t_stage = [&]() {
+        if (!stage()) return false;
+        const bool r = wait_on<PAIR>(&t_clean[st.s], (ph_c >> st.s) & 1, abort_flag, p.err, DEVERR_WAIT_MMA);
+        ph_c ^= 1u << st.s;
+        tc_fence_after();
+        return r;
+      };
+      auto add = [&](uint32_t d, uint64_t a, uint64_t b) {
+        if (PAIR) umma_f16_pair(d, a, b, id, 1);
+        else umma_f16(d, a, b, id, 1);
       };
       for (int u = first; ok && u < units; u += step, ++nu) {
         const int ab = nu & 1;
         const uint32_t d = tmem + ab * 256;
-        ok = !*abort_flag && mbar_wait<PAIR>(&d_empty[ab], ((nu >> 1) & 1) ^ 1, p.err, DEVERR_WAIT_MMA);
+        ok = wait_on<PAIR>(&d_empty[ab], ((nu >> 1) & 1) ^ 1, abort_flag, p.err, DEVERR_WAIT_MMA);
         for (int kb = 0; ok && kb < nk; ++kb) {
           if (!(ok = stage())) break;
-          const uint32_t a = smem_u32(sStage + st.s * p.stage_bytes);
+          const uint64_t ad = kdesc(smem_u32(sStage + st.s * p.stage_bytes)), bd = ad + (16384 >> 4);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint64_t ad = sdesc_sw128(a + k * 32, 16, 1024), bd = sdesc_sw128(a + 16384 + k * 32, 16, 1024);
-            if (PAIR) umma_f16_pair(d, ad, bd, id, (kb | k) != 0);
-            else umma_f16(d, ad, bd, id, (kb | k) != 0);
+            if (PAIR) umma_f16_pair(d, ad + 2 * k, bd + 2 * k, id, (kb | k) != 0);
+            else umma_f16(d, ad + 2 * k, bd + 2 * k, id, (kb | k) != 0);
           }
           commit(&empty[st.s]);
           st.advance(p.stages);
         }
         for (bool more = true; ok && more;) {
-          if (!(ok = !*abort_flag && mbar_wait(&list_full[li.s], li.ph, p.err, DEVERR_WAIT_MMA))) break;
+          if (!(ok = wait_on<false>(&list_full[li.s], li.ph, abort_flag, p.err, DEVERR_WAIT_MMA))) break;
           const SlotList& l = lists[li.s];
           more = l.more;
-          for (int g = 0; ok && g < l.n; ++g)
+          const int n = l.n;
+          for (int g = 0; ok && g < n; ++g)
             for (int c = 0; ok && c < groups; ++c) {
-              if (!(ok = stage())) break;
-              const uint32_t t = smem_u32(sStage + st.s * p.stage_bytes), b = t + 16384;
-              const int s0 = st.s, steps = (min(p.r - c * 64, 64) + 15) / 16;
-              for (int k = 0; k < steps; ++k)
-                umma_f16_rows<PAIR>(d, sdesc_sw128(t + k * 32, 16, 1024), sdesc_sw128(b + k * 32, 16, 1024), id, l.others[g]);
+              const int steps = (min(p.r - c * 64, 64) + 15) / 16;
+              if (!(ok = t_stage())) break;
+              const uint64_t hi = kdesc(smem_u32(sStage + st.s * p.stage_bytes)), bd = hi + (16384 >> 4);
+              const int s0 = st.s;
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if (k < steps) add(d, hi + 2 * k, bd + 2 * k);
               st.advance(p.stages);
-              uint32_t lo = t + 64;
+              uint64_t lo = hi + 4;  // r <= 32: the same block's second half
               if (p.r > 32) {
-                if (!(ok = stage())) break;
-                lo = smem_u32(sStage + st.s * p.stage_bytes);
+                if (!(ok = t_stage())) break;
+                lo = kdesc(smem_u32(sStage + st.s * p.stage_bytes));
               }
-              for (int k = 0; k < steps; ++k)
-                umma_f16_rows<PAIR>(d, sdesc_sw128(lo + k * 32, 16, 1024), sdesc_sw128(b + k * 32, 16, 1024), id, l.others[g]);
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if (k < steps) add(d, lo + 2 * k, bd + 2 * k);
               commit(&empty[s0]);
               if (p.r > 32) {
                 commit(&empty[st.s]);
@@ -416,99 +631,136 @@ __global__ void __launch_bounds__(kLThreads, 1) lora_tile_kernel(const __grid_co
   } else if (warp == 2) {
     Ring li;
     bool ok = true;
+    int rows[TM / 32];
+    rows_of<TM / 32>(p, first / p.nt * TM, lane, rows);
+    for (int u = first; ok && u < units; u += step)
+      ok = list_adapters<TM / 32>(p, u + step < units ? (u + step) / p.nt * TM : -1, rows, kSlots, lists, list_full,
+                                  list_empty, li, abort_flag, lane);
+    if (!ok) *abort_flag = 1;
+  } else if (warp == 3) {
+    Ring st, li;
+    unsigned ph = 0;  // phases of t_full
+    bool ok = true;
     for (int u = first; ok && u < units; u += step) {
-      constexpr int RL = TM / 32;  // rows per lane
-      int a[RL];
+      for (int kb = 0; kb < nk; ++kb) st.advance(p.stages);
+      for (bool more = true; ok && more;) {
+        ok = __all_sync(0xffffffffu, wait_on<false>(&list_full[li.s], li.ph, abort_flag, p.err, DEVERR_WAIT_EPI));
+        if (!ok) break;
+        const SlotList& l = lists[li.s];
+        const int n = l.n;
+        more = l.more;
+        for (int g = 0; ok && g < n; ++g) {
+          uint32_t others[4];
 #pragma unroll
-      for (int i = 0; i < RL; ++i) {
-        const int m = u / p.nt * TM + i * 32 + lane;
-        a[i] = m < p.M ? __ldg(p.rows + m) : -1;
-        if (a[i] >= p.L) {
-          atomicOr(p.err, DEVERR_BOUNDS);
-          a[i] = -1;
-        }
-      }
-      int n = -1;  // adapters in the open list entry, -1: none open
-      auto open_entry = [&] {
-        const bool w = !*abort_flag && mbar_wait(&list_empty[li.s], li.ph ^ 1, p.err, DEVERR_WAIT_EPI);
-        n = 0;
-        return __all_sync(0xffffffffu, w) != 0;
-      };
-      auto close_entry = [&](int more) {
-        if (lane == 0) {
-          lists[li.s].n = n;
-          lists[li.s].more = more;
+          for (int i = 0; i < 4; ++i) others[i] = l.others[g][rank * 4 + i];
+          for (int c = 0; ok && c < groups * (p.r <= 32 ? 1 : 2); ++c) {
+            ok = __all_sync(0xffffffffu, wait_on<false>(&t_full[st.s], (ph >> st.s) & 1, abort_flag, p.err, DEVERR_WAIT_EPI));
+            if (!ok) break;
+            ph ^= 1u << st.s;
+            if (others[0] | others[1] | others[2] | others[3]) {
+              // a warp's stores cover four whole rows: lane / 8 the row, lane % 8 its 16-byte piece
+              uint4* t = reinterpret_cast<uint4*>(sStage + st.s * p.stage_bytes);
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (others[i]) {  // warp-uniform
+#pragma unroll
+                  for (int k = 0; k < 8; ++k)
+                    if ((others[i] >> (k * 4 + lane / 8)) & 1) t[(i * 32 + k * 4) * 8 + lane] = make_uint4(0, 0, 0, 0);
+                }
+              fence_async_smem();
+              __syncwarp();
+            }
+            if (lane == 0) {
+              if (PAIR) mbar_arrive_cluster(t_clean0 + st.s * 8);
+              else mbar_arrive(&t_clean[st.s]);
+            }
+            st.advance(p.stages);
+          }
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&list_full[li.s]);
+        if (lane == 0) mbar_arrive(&list_empty[li.s]);
         li.advance(kLists);
-      };
-      ok = open_entry();
-#pragma unroll
-      for (int i = 0; i < RL; ++i) {
-        unsigned open;
-        while (ok && (open = __ballot_sync(0xffffffffu, a[i] >= 0)) != 0) {
-          if (n == kSlots) {
-            close_entry(1);
-            if (!(ok = open_entry())) break;
-          }
-          const int id = __shfl_sync(0xffffffffu, a[i], __ffs(open) - 1);
-#pragma unroll
-          for (int k = 0; k < RL; ++k) {
-            const unsigned o = __ballot_sync(0xffffffffu, a[k] != id);
-            if (a[k] == id) a[k] = -1;
-            if (lane == 0) lists[li.s].others[n][k] = o;
-          }
-          if (lane == 0) lists[li.s].ids[n] = id;
-          ++n;
-        }
       }
-      if (ok) close_entry(0);
     }
     if (!ok) *abort_flag = 1;
-  } else if (warp >= 4) {
-    const int ew = warp - 4, q = warp & 3, half = ew / 4;
+  } else {
+    const int ew = warp - 4, q = warp & 3, third = ew / 4;
     uint8_t* slabs = sSlab + ew * kSlabs * kSlab;
     uint64_t* rb = r_full + ew * kSlabs;
-    float* bs = sBias + ew * 32;
+    float* bs = sBias + ew * 96;
+    Ring li;
     unsigned r_ph = 0;  // phases of this warp's residual barriers
     bool ok = true;
     int nu = 0;
     pdl_wait();  // this grid is not over before lora_t_kernel is
     for (int u = first; ok && u < units; u += step, ++nu) {
       const int ab = nu & 1, m0 = u / p.nt * TM + rank * 128 + q * 32, n0 = u % p.nt * p.BN;
-      // 32-column chunks of this warp: half, half + 2, ...
-      const int all = (min(p.BN, p.N - n0) + 31) / 32, mine = m0 < p.M ? (all - half + 1) / 2 : 0;
+      // 32-column chunks of this warp: third, third + 3, ...
+      const int all = (min(p.BN, p.N - n0) + 31) / 32, mine = m0 < p.M ? (all - third + 2) / 3 : 0;
       auto fetch = [&](int i) {  // residual of chunk i into its slab (free: its last store has been read)
         mbar_arrive_expect_tx(&rb[i % kSlabs], kSlab);
-        tma_load_2d(slabs + i % kSlabs * kSlab, &p.tmR, &rb[i % kSlabs], n0 + (half + 2 * i) * 32, m0);
+        tma_load_2d(slabs + i % kSlabs * kSlab, &p.tmR, &rb[i % kSlabs], n0 + (third + 3 * i) * 32, m0);
       };
-      if (p.R && lane == 0 && mine) {
+      if (p.R && lane == 0 && mine > 0) {
         bulk_wait_read0();
         for (int i = 0; i < min(mine, kSlabs); ++i) fetch(i);
       }
-      ok = !*abort_flag && mbar_wait<PAIR>(&d_full[ab], (nu >> 1) & 1, p.err, DEVERR_WAIT_EPI);
+      if (p.bias) {
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          const int n = n0 + (third + 3 * i) * 32 + lane;
+          if (i < mine) bs[i * 32 + lane] = n < p.N ? __ldg(p.bias + n) : 0.f;
+        }
+        __syncwarp();
+      }
+      bool mixed = false;  // some of the tile's rows do not take its first adapter
+      for (bool more = true; ok && more;) {
+        ok = __all_sync(0xffffffffu, wait_on<false>(&list_full[li.s], li.ph, abort_flag, p.err, DEVERR_WAIT_EPI));
+        if (!ok) break;
+        const SlotList& l = lists[li.s];
+        more = l.more;
+        mixed = mixed || l.n > 1 || more || (l.n && __any_sync(0xffffffffu, lane < TM / 32 && l.others[0][lane % 8]));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&list_empty[li.s]);
+        li.advance(kLists);
+      }
+      ok = ok && wait_on<PAIR>(&d_full[ab], (nu >> 1) & 1, abort_flag, p.err, DEVERR_WAIT_EPI);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
       const uint32_t d = tmem + ab * 256 + (static_cast<uint32_t>(q * 32) << 16);
+      uint32_t r[32];
+      if (mine > 0) tmem_ld32(d + third * 32, r);
 #pragma unroll 1
       for (int i = 0; i < mine; ++i) {
-        const int c = (half + 2 * i) * 32, nb = n0 + c, sl = i % kSlabs;
+        const int c = (third + 3 * i) * 32, nb = n0 + c, sl = i % kSlabs;
         uint8_t* slab = slabs + sl * kSlab;
         uint4* rp = reinterpret_cast<uint4*>(slab + lane * 64);  // 64-byte rows, 64-byte swizzle
-        uint32_t r[32];
-        tmem_ld32(d + c, r);
-        if (p.bias) bs[lane] = nb + lane < p.N ? __ldg(p.bias + nb + lane) : 0.f;
-        __syncwarp();
         tmem_wait_ld();
         float v[32];
 #pragma unroll
         for (int k = 0; k < 32; ++k) v[k] = __uint_as_float(r[k]);
+        if (i + 1 < mine) tmem_ld32(d + c + 96, r);  // the next chunk arrives under this one's arithmetic
+        if (mixed) {
+          float z = 0.f;
+#pragma unroll
+          for (int k = 0; k < 32; ++k) z = fmaf(v[k], 0.f, z);  // NaN if any value is not finite
+          unsigned bad = __ballot_sync(0xffffffffu, z != 0.f && m0 + lane < p.M);
+          while (bad) {
+            const int row = __ffs(bad) - 1;
+            bad &= bad - 1;
+            const float own = own_terms<BF16>(p, m0 + row, nb, lane);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              const float t = __shfl_sync(0xffffffffu, own, k);
+              if (lane == row) v[k] = t;
+            }
+          }
+        }
         if (p.bias) {
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            const float4 b = reinterpret_cast<const float4*>(bs)[k];
+            const float4 b = reinterpret_cast<const float4*>(bs + i * 32)[k];
             v[4 * k] += b.x; v[4 * k + 1] += b.y; v[4 * k + 2] += b.z; v[4 * k + 3] += b.w;
           }
         }
@@ -553,8 +805,11 @@ __global__ void __launch_bounds__(kLThreads, 1) lora_tile_kernel(const __grid_co
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        if (PAIR) mbar_arrive_cluster(d_empty0 + ab * 8);
-        else mbar_arrive(&d_empty[ab]);
+        // the reads are complete (tcgen05.wait): nothing else is handed over, so no release
+        if (PAIR)
+          asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(d_empty0 + ab * 8) : "memory");
+        else
+          mbar_arrive(&d_empty[ab]);
       }
     }
     if (!ok) *abort_flag = 1;
@@ -718,7 +973,8 @@ template <bool BF16>
 int launch_tiles(Ctx* c, LoraParams& p) {
   static unsigned attr_done = 0;
   if (!(attr_done & (1u << (c->device & 31)))) {
-    if (cudaFuncSetAttribute(lora_tile_kernel<BF16, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448) != cudaSuccess ||
+    if (cudaFuncSetAttribute(lora_t_kernel<BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448) != cudaSuccess ||
+        cudaFuncSetAttribute(lora_tile_kernel<BF16, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448) != cudaSuccess ||
         cudaFuncSetAttribute(lora_tile_kernel<BF16, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448) != cudaSuccess)
       return set_error(c, DI_ECUDA, "linear_lora: shared memory attribute");
     attr_done |= 1u << (c->device & 31);
@@ -765,12 +1021,16 @@ int launch_tiles(Ctx* c, LoraParams& p) {
       (p.R && !make_tmap(&p.tmR, dt, 2, p.R, yd, rs, yb, CU_TENSOR_MAP_SWIZZLE_64B, &err)) ||
       !make_tmap(&p.tmY, dt, 2, p.Y, yd, ys, yb, CU_TENSOR_MAP_SWIZZLE_64B, &err))
     return set_error(c, DI_EINVAL, "linear_lora: " + err);
-  // 64 rows a block reads the adapters least often; few rows take 16 so that the SMs are filled
-  const int rg = (p.r + 31) / 32;
-  if ((long long)p.M * rg >= 128LL * c->num_sms)
-    launch_k(lora_t_kernel<BF16, 64, 32>, dim3(rg, (p.M + 63) / 64), 256, 0, c->stream, p);
-  else
-    launch_k(lora_t_kernel<BF16, 16, 16>, dim3(rg, (p.M + 15) / 16), 256, 0, c->stream, p);
+  const int rp = (p.r + 15) / 16 * 16;
+  p.tslots = std::max(1, std::min({p.L, kSlots, 256 / rp}));
+  p.tstage_bytes = 16384 + p.tslots * rp * 128;
+  p.tstages = (int)std::min<uint32_t>(5, (232448 - kTFixedSmem) / p.tstage_bytes);
+  const uint64_t ad[3] = {K, r, (uint64_t)p.L}, as[2] = {K * 2, r * K * 2};
+  const uint32_t ab[3] = {64, (uint32_t)rp, 1};
+  if (!make_tmap(&p.tmA, dt, 3, p.A, ad, as, ab, CU_TENSOR_MAP_SWIZZLE_128B, &err))
+    return set_error(c, DI_EINVAL, "linear_lora: " + err);
+  launch_k(lora_t_kernel<BF16>, dim3((unsigned)std::min<long long>((p.M + 127LL) / 128, c->num_sms)), dim3(kTThreads),
+           kTFixedSmem + p.tstages * p.tstage_bytes, c->stream, p);
   const int rc = check_launch(c, "linear_lora");
   if (rc != DI_OK) return rc;
   const long long units = (long long)p.mt * p.nt;
@@ -811,7 +1071,7 @@ extern "C" int di_linear_lora(di_ctx_t h, int dtype, const void* X, long long ld
   if (!aligned16(X) || !aligned16(W) || !aligned16(A) || !aligned16(B) || !aligned16(R) || !aligned16(Y) || ldx % 8 ||
       ldy % 8 || (R && ldr % 8))
     return set_error(c, DI_EINVAL, "linear_lora: pointers must be 16-byte aligned, row strides multiples of 8 elements");
-  if ((M + 127LL) / 128 * ((N + 31) / 32) > 0x7fffffffll || (M + 15LL) / 16 > 65535)
+  if (M > (1 << 30) || N > (1 << 30) || (M + 127LL) / 128 * ((N + 31) / 32) > 0x7fffffffll)
     return set_error(c, DI_EUNSUPPORTED, "linear_lora: too many rows and columns");
   const size_t need = di_linear_lora_workspace(h, M, N, K, rank, n_adapters);
   if (need && (!ws || ws_bytes < need || !aligned16(ws)))
