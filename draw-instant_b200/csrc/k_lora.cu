@@ -976,7 +976,7 @@ int launch_tiles(Ctx* c, LoraParams& p) {
     if (cudaFuncSetAttribute(lora_t_kernel<BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448) != cudaSuccess ||
         cudaFuncSetAttribute(lora_tile_kernel<BF16, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448) != cudaSuccess ||
         cudaFuncSetAttribute(lora_tile_kernel<BF16, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448) != cudaSuccess)
-      return set_error(c, DI_ECUDA, "linear_lora: shared memory attribute");
+      return cudaGetLastError(), set_error(c, DI_ECUDA, "linear_lora: shared memory attribute");
     attr_done |= 1u << (c->device & 31);
   }
   // Column width and pairing: a K block takes 2 BN cycles of MMAs or its stage's bytes at some 45 bytes a cycle from L2,

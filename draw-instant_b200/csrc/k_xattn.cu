@@ -6,26 +6,30 @@
 // A request without valid keys gives zero rows; query rows from q_len[b] on are not written.
 //
 // One pass over the keys with a running maximum and sum per row.  Query heads that share a key head are
-// packed as rows of one tile (row t = token * GP + head, GP the power of two in the group), so a
-// key tile is read once for all of them and single-token queries fill rows that would be padding.  A work unit is 256
-// packed rows of one (request, head group) and a range of 128-key tiles; one persistent CTA per SM walks its units:
+// packed as rows (row t = token * GP + head, GP the power of two in the group), so a key tile is read once for all of
+// them and single-token queries fill rows that would be padding.  One persistent CTA per SM:
 //
-//   warps 0-3, 4-7  softmax of rows 0..127 and 128..255, one row per thread (= one TMEM lane)
-//   warp 8          MMA issue: S = Q K^T into TMEM, O += P V with P read from TMEM
-//   warp 9          TMA loads: Q tiles of the next unit while this one runs, K and V tiles through one ring
+//   4 NW warps  softmax: NW groups of 128 rows, one row per thread (= one TMEM lane)
+//   MMA warp    S = Q K^T into TMEM, O += P V with P read from TMEM
+//   TMA warp    Q tiles of the next work item while this one runs, K and V tiles through one ring
+//   clean warp  zeroes the V rows of masked keys in shared memory (their P is 0, but 0 * inf is not)
+//   item warp   works out the items ahead of the others and hands them over through shared memory
 //
-// P (16-bit) overwrites the columns of the scores it came from; the two row tiles alternate on the tensor
-// pipe, so one tile's products run while the other's exponentials do.  MMAs of the one issuing thread
-// execute in order: S of tile j + 1 may follow P V of tile j into the same columns, and its commit also tells that
-// P V of tile j is complete.  The running maximum only moves when a row's true maximum passes it by 2^8, so O is rarely
-// rescaled and P stays below 2^8 in range of both types; O / l is exact under the stale maximum.
-// P is rounded to the inputs' 16-bit type for the second product (half a step per probability, averaged over the
-// keys); scores, maxima, sums and O are 32-bit.
+// P (16-bit) overwrites the columns of the scores it came from.  The groups take turns on the tensor pipe, so one
+// group's products run while the others' exponentials do.  MMAs of the one issuing thread execute in order: S of the next
+// key tile may follow P V into the same columns, and its commit also tells that P V is complete.  The running maximum
+// only moves when a row's true maximum passes it by 2^8, so O is rarely rescaled and P stays below 2^8, in range of both
+// types; O / l is exact under the stale maximum.  P is rounded to the inputs' 16-bit type for the second product (half a
+// step per probability, averaged over the keys); scores, maxima, sums and O are 32-bit.
 //
-// Masked keys: scores become -inf before the maximum, and the V rows of masked keys are zeroed in shared memory before
-// the product, so nothing they hold reaches O.
-// Few units: the key tiles of a unit are split over CTAs, each writing (O, max, sum) in 32 bits to the
-// workspace, and a second kernel joins them in split order.
+// Work, by rows: an item is up to NW tiles of 128 rows of one (request, head group), which share its key tiles.
+// Work, by keys (too few rows for the SMs): an item is a range of key tiles of one tile of rows; the key tiles of all
+// requests are laid end to end and cut into as many equal ranges as there are CTAs, whatever the lengths, and the
+// groups of a CTA take its key tiles in turn.  Each group writes (O, max, sum) in 32 bits to the workspace and a second
+// kernel joins them in key order.
+//
+// Head dim 64: 4 groups, key tiles of 64; up to 128 keys one tile of 128, whose O then lies over the spent scores.
+// Head dim 128: 2 groups, key tiles of 128 (the 512 columns of TMEM hold two O and two S).
 #include <algorithm>
 #include <cstring>
 
@@ -37,33 +41,42 @@ struct XattnParams {
   CUtensorMap tmQ, tmK, tmV;
   void* O;
   long long osb, oss, osh;  // output strides in elements
-  int kvb_mul, kvh_mul, vb_mul, vh_mul, qb_mul, qh_mul;  // 0: the tensor is expanded over that axis
+  int kb_mul, kh_mul, vb_mul, vh_mul, qb_mul, qh_mul;  // 0: the tensor is expanded over that axis
   int B, HG, GP, gps, G;    // head groups of GP = 2^gps query heads; G query heads per key head
-  int Sq, Skv, RT, NS;      // row tiles (256 rows) per group, key splits
+  int Sq, Skv, RT, tpi;     // row blocks per group, row tiles per item
+  int by_keys;
+  unsigned items;           // by rows: B * HG * RT
+  int d_rt, d_hg, d_b;      // gridDim.x in units of the item order (b, hg, rt)
   int nq, ring;             // Q buffers, K/V ring tiles
   int wide;                 // output rows take 32-byte stores
   const int *q_len, *kv_len;
   const unsigned char* mask;
   float scale_log2;
-  float* part;              // [NS][B * HG * R][D] partial O, then [NS][B * HG * R][2] (max, sum)
+  float* part;              // by keys: [slots][NW][128][D] partial O, then [slots][NW][128][2] (max, sum)
+  int slots, grid;
   int* err;
 };
 
 namespace {
 
-constexpr int QT = 128, KT = 128;
-constexpr int kXThreads = 384;
-// Registers: three warpgroups launch with 168 each; the softmax warpgroups (a row of 128 scores per thread) take
-// 216, the third gives up its own down to 64: 256 * 216 + 128 * 64 <= 384 * 168.
 constexpr float kRescale = 8.0f;  // log2 units
+constexpr int kItems = 4;         // work items worked out ahead
+constexpr int kMaxByKeys = 256;   // requests whose key tiles are laid end to end
 
-template <int D>
-struct XSmem {
-  static constexpr uint32_t TILE = 128 * D * 2;       // one Q, K or V tile
-  static constexpr uint32_t HALF = 128 * 128;         // 64 columns of it, 128-byte rows
-  static constexpr int SLOTS = D == 64 ? 13 : 7;
-  static constexpr int MAXRING = SLOTS - 2;
-  static constexpr uint32_t TOTAL = 1024 + SLOTS * TILE + 1024;
+template <int D, bool SHORT>
+struct XCfg {
+  static constexpr int NW = D == 64 ? 4 : 2;
+  static constexpr int KT = D == 64 && !SHORT ? 64 : 128;       // keys per tile
+  static constexpr int THREADS = 128 * NW + 128;
+  static constexpr int TCOLS = 512 / NW;                        // TMEM columns of a group: S (P over it), O
+  static constexpr int TO = D == 64 ? 64 : 128;                 // first column of O
+  static constexpr uint32_t QTILE = 128 * D * 2, QHALF = 128 * 128;  // Q tile; 64 columns of it (128-byte rows)
+  static constexpr uint32_t KTILE = KT * D * 2, KHALF = KT * 128;
+  static constexpr uint32_t DATA = D == 64 ? 13 * 16384 : 7 * 32768;
+  static constexpr int MAXRING = D == 64 ? 20 : 6;
+  static constexpr uint32_t BARS = 8 * (4 + 3 * MAXRING + 4 * NW + 2 * kItems) + 16 + kItems * 64;
+  static constexpr uint32_t TOTAL = 1024 + DATA + (BARS + 15) / 16 * 16 + (kMaxByKeys + 4) * 4;
+  static_assert(TOTAL <= 232448, "shared memory of one CTA");
 };
 
 __device__ __forceinline__ uint64_t f2_pack(float a, float b) {
@@ -77,6 +90,11 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t d;
   asm("add.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
 __device__ __forceinline__ float lo_f(uint64_t v) { return __uint_as_float((uint32_t)v); }
@@ -107,7 +125,7 @@ __device__ __forceinline__ void umma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, ui
       ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
       ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
@@ -123,440 +141,701 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   __half2 v = __floats2half2_rn(a, b);
   return *reinterpret_cast<uint32_t*>(&v);
 }
+__device__ __forceinline__ uint64_t kdesc(uint32_t a) { return sdesc_sw128(0, 16, 1024) | (a >> 4); }  // K-major tile
+
+// Bounded wait that also ends when another role has given up; the flag is read only when the phase is not there yet.
+__device__ __forceinline__ bool wait_on(uint64_t* bar, int ph, volatile int* abort_flag, int* err, int code) {
+  if (mbar_try_wait(smem_u32(bar), ph)) return true;
+  return !*abort_flag && mbar_wait(bar, ph, err, code);
+}
 
 // Position in a ring of n buffers: entry e lies in buffer e % n and completes its barrier's phase (e / n) & 1.
 struct RingPos {
   int s = 0, ph = 0;
-  __device__ __forceinline__ void advance(int n, int by = 1) {
-    s += by;
-    if (s >= n) { s -= n; ph ^= 1; }
+  __device__ __forceinline__ void advance(int n) {
+    if (++s == n) { s = 0; ph ^= 1; }
   }
   __device__ __forceinline__ RingPos next(int n) const {
     RingPos r = *this;
     r.advance(n);
     return r;
   }
+  __device__ __forceinline__ void back(int n) {
+    if (--s < 0) { s = n - 1; ph ^= 1; }
+  }
 };
 
-// One work unit: packed rows [row0, row0 + rows) of (b, hg), key tiles [t0, t1) of n valid-range keys.
-struct Unit {
-  int b, hg, sp, row0, rows, n, t0, t1;
+// A work item: packed rows [row0, row0 + rows) of (b, hg), key tiles [t0, t1) of its n keys in reach.
+struct Item {
+  int b, hg, row0, rows, n, t0, t1, slot;  // rows 0: no more items
 };
-__device__ __forceinline__ bool unit_of(const XattnParams& p, unsigned u, Unit& w) {
-  w.sp = (int)(u % p.NS);
-  u /= p.NS;
-  const int rt = (int)(u % p.RT);
-  u /= p.RT;
-  w.hg = (int)(u % p.HG);
-  w.b = (int)(u / p.HG);
-  w.row0 = rt * 2 * QT;
-  const int q = p.q_len ? min(max(__ldg(p.q_len + w.b), 0), p.Sq) : p.Sq;
-  w.rows = min(q * p.GP - w.row0, 2 * QT);
-  w.n = p.kv_len ? min(max(__ldg(p.kv_len + w.b), 0), p.Skv) : p.Skv;
-  const int nt = (w.n + KT - 1) / KT;
-  w.t0 = (int)((long long)nt * w.sp / p.NS);
-  w.t1 = (int)((long long)nt * (w.sp + 1) / p.NS);
-  return w.rows > 0;
-}
+// The items of one CTA.  Items without rows are left out; those without keys are kept when they are by rows (their
+// outputs are zeros).
+template <int KT>
+struct Items {
+  const XattnParams& p;
+  const int* ends;  // by keys: key tiles of the requests before and with b, times row blocks and head groups
+  unsigned u;       // by rows
+  int b, hg, rt;
+  int g, g1, bb;    // by keys: this CTA's range of the tiles laid end to end, request of tile g
+  __device__ __forceinline__ Items(const XattnParams& p_, const int* e) : p(p_), ends(e) {
+    if (p.by_keys) {
+      const long long total = ends[p.B - 1];
+      g = (int)(total * blockIdx.x / p.grid);
+      g1 = (int)(total * (blockIdx.x + 1) / p.grid);
+      bb = 0;
+    } else {
+      u = blockIdx.x;
+      rt = (int)(u % p.RT);
+      hg = (int)(u / p.RT % p.HG);
+      b = (int)(u / p.RT / p.HG);
+    }
+  }
+  __device__ __forceinline__ bool next(Item& w) {
+    if (p.by_keys) {
+      while (g < g1) {
+        while (ends[bb] <= g) ++bb;
+        w.b = bb;
+        w.n = p.kv_len ? min(max(__ldg(p.kv_len + bb), 0), p.Skv) : p.Skv;
+        const int nt = (w.n + KT - 1) / KT, at = g - (bb ? ends[bb - 1] : 0);
+        const int blk = at / nt;
+        w.t0 = at - blk * nt;
+        w.t1 = min(nt, w.t0 + g1 - g);
+        w.hg = blk / p.RT;
+        const int r = blk - w.hg * p.RT;
+        w.slot = (int)blockIdx.x + (bb * p.HG + w.hg) * p.RT + r;  // grows by one with each CTA and each block of rows
+        g += w.t1 - w.t0;
+        if (rows_of(w, r)) return true;
+      }
+      return false;
+    }
+    while (u < p.items) {
+      w.b = b;
+      w.hg = hg;
+      const int r = rt;
+      u += gridDim.x;
+      rt += p.d_rt;
+      hg += p.d_hg;
+      b += p.d_b;
+      if (rt >= p.RT) { rt -= p.RT; ++hg; }
+      if (hg >= p.HG) { hg -= p.HG; ++b; }
+      if (!rows_of(w, r)) continue;
+      w.n = p.kv_len ? min(max(__ldg(p.kv_len + w.b), 0), p.Skv) : p.Skv;
+      w.t0 = 0;
+      w.t1 = (w.n + KT - 1) / KT;
+      w.slot = 0;
+      return true;
+    }
+    return false;
+  }
+  __device__ __forceinline__ bool rows_of(Item& w, int r) {
+    w.row0 = r * p.tpi * 128;
+    const int q = p.q_len ? min(max(__ldg(p.q_len + w.b), 0), p.Sq) : p.Sq;
+    w.rows = min((q << p.gps) - w.row0, p.tpi * 128);
+    return w.rows > 0;
+  }
+};
 
-template <bool BF16, int D>
-__global__ void __launch_bounds__(kXThreads, 1) xattn_kernel(const __grid_constant__ XattnParams p) {
-  using S = XSmem<D>;
+template <bool BF16, int D, bool SHORT>
+__global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const __grid_constant__ XattnParams p) {
+  using C = XCfg<D, SHORT>;
+  constexpr int NW = C::NW, KT = C::KT;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sQ = smem;                             // [nq][2] tiles
-  uint8_t* sKV = smem + p.nq * 2 * S::TILE;       // [ring] tiles
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::SLOTS * S::TILE);
-  uint64_t* q_full = bars;                        // [2]
-  uint64_t* q_empty = bars + 2;                   // [2]
-  uint64_t* kv_full = bars + 4;                   // [ring]
-  uint64_t* kv_empty = kv_full + S::MAXRING;      // [ring]
-  uint64_t* s_full = kv_empty + S::MAXRING;       // [2] scores of row tile w ready
-  uint64_t* p_full = s_full + 2;                  // [2] probabilities of row tile w written
-  uint64_t* o_full = p_full + 2;                  // [2] O of row tile w complete
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
+  const int qtiles = p.by_keys ? 1 : p.tpi;        // Q tiles of an item
+  uint8_t* sQ = smem;                              // [nq][qtiles]
+  uint8_t* sKV = smem + p.nq * qtiles * C::QTILE;  // [ring]
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + C::DATA);  // [2]
+  uint64_t* q_empty = q_full + 2;                  // [2]
+  uint64_t* kv_full = q_empty + 2;                 // [ring]
+  uint64_t* kv_empty = kv_full + C::MAXRING;       // [ring]
+  uint64_t* v_clean = kv_empty + C::MAXRING;       // [ring] V rows of masked keys zeroed
+  uint64_t* s_full = v_clean + C::MAXRING;         // [NW] scores ready
+  uint64_t* p_full = s_full + NW;                  // [NW] probabilities written
+  uint64_t* o_full = p_full + NW;                  // [NW] O complete
+  uint64_t* o_read = o_full + NW;                  // [NW] O read (SHORT: the next scores may overwrite it)
+  uint64_t* item_full = o_read + NW;               // [kItems]
+  uint64_t* item_empty = item_full + kItems;       // [kItems]
+  Item* items = reinterpret_cast<Item*>(item_empty + kItems);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(items) + kItems * 64);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* ends = reinterpret_cast<int*>(smem + C::DATA + (C::BARS + 15) / 16 * 16);  // [B] by keys
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int svc = warp - 4 * NW;  // service warps: 0 MMA, 1 TMA, 2 clean, 3 items
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], 1);
-      mbar_init(&q_empty[i], 1);
+    for (int i = 0; i < 2; ++i) { mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], 1); }
+    for (int i = 0; i < p.ring; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); mbar_init(&v_clean[i], 1); }
+    for (int i = 0; i < NW; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 128);
       mbar_init(&o_full[i], 1);
+      mbar_init(&o_read[i], 4);
     }
-    for (int i = 0; i < p.ring; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); }
+    for (int i = 0; i < kItems; ++i) { mbar_init(&item_full[i], 1); mbar_init(&item_empty[i], 3 + 4 * NW); }
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 8) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  if (svc == 0) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  pdl_begin();
+  if (p.by_keys && svc == 3) {  // running sums of the requests' key tiles
+    int sum = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 32) {
+      const int b = b0 + lane;
+      int n = 0;
+      if (b < p.B) n = ((p.kv_len ? min(max(__ldg(p.kv_len + b), 0), p.Skv) : p.Skv) + KT - 1) / KT * p.HG * p.RT;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, n, o);
+        if (lane >= o) n += x;
+      }
+      if (b < p.B) ends[b] = sum + n;
+      sum += __shfl_sync(0xffffffffu, n, 31);
+    }
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  pdl_begin();
-  const unsigned units = (unsigned)p.B * p.HG * p.RT * p.NS;
-  // TMEM columns: scores of row tile w at 128 w (its probabilities over their first half), O at 256 + D w
+  // a tile needs its V rows cleaned when it has masked keys inside the tensor (rows past Skv are zero already)
+  auto cleaned = [&](const Item& w, int t) { return p.mask || (w.n < p.Skv && w.n - t * KT < KT); };
+  // The next item, or nothing: one thread (or one per warp, the rest following) takes it, done() gives its place back.
+  RingPos ip;
+  auto next = [&](int code) -> const Item* {
+    if (!wait_on(&item_full[ip.s], ip.ph, abort_flag, p.err, code)) {
+      *abort_flag = 1;
+      return nullptr;
+    }
+    return items[ip.s].rows ? &items[ip.s] : nullptr;
+  };
+  auto done = [&] {
+    mbar_arrive(&item_empty[ip.s]);
+    ip.advance(kItems);
+  };
 
-  if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-  if (warp == 9) {
+  if (svc == 1) {
     if (elect_one()) {
       tma_prefetch_desc(&p.tmQ);
       tma_prefetch_desc(&p.tmK);
       tma_prefetch_desc(&p.tmV);
       RingPos kv, q;
-      unsigned nkv = 0, nq = 0;  // copies issued, up to the buffers there are
-      for (unsigned u = blockIdx.x; u < units && !*abort_flag; u += gridDim.x) {
-        Unit w;
-        if (!unit_of(p, u, w) || w.t0 >= w.t1) continue;
-        const int nw = w.rows > QT ? 2 : 1;
-        if (!mbar_wait(&q_empty[q.s], q.ph ^ 1, p.err, DEVERR_WAIT_TMA)) { *abort_flag = 1; break; }
-        mbar_arrive_expect_tx(&q_full[q.s], nw * S::TILE);
-        for (int i = 0; i < nw; ++i)
+      unsigned nkv = 0, nq = 0;  // copies issued
+      bool ok = true;
+      for (const Item* item; ok && (item = next(DEVERR_WAIT_TMA)); done()) {
+        const Item w = *item;
+        if (w.t0 >= w.t1) continue;
+        if (!(ok = wait_on(&q_empty[q.s], q.ph ^ 1, abort_flag, p.err, DEVERR_WAIT_TMA))) break;
+        const int nt = (w.rows + 127) / 128;
+        mbar_arrive_expect_tx(&q_full[q.s], nt * C::QTILE);
+        for (int i = 0; i < nt; ++i)
           for (int c = 0; c < D / 64; ++c)
-            tma_load_5d(sQ + (q.s * 2 + i) * S::TILE + c * S::HALF, &p.tmQ, &q_full[q.s], c * 64, 0,
-                        (w.row0 + i * QT) >> p.gps, w.hg * p.qh_mul, w.b * p.qb_mul);
+            tma_load_5d(sQ + (q.s * qtiles + i) * C::QTILE + c * C::QHALF, &p.tmQ, &q_full[q.s], c * 64, 0,
+                        (w.row0 + i * 128) >> p.gps, w.hg * p.qh_mul, w.b * p.qb_mul);
         q.advance(p.nq);
         ++nq;
-        const int hk = w.hg * p.GP / p.G;
-        for (int t = w.t0; t < w.t1; ++t)
+        const int hk = (w.hg << p.gps) / p.G;
+        for (int t = w.t0; ok && t < w.t1; ++t)
           for (int v = 0; v < 2; ++v) {
-            if (*abort_flag || !mbar_wait(&kv_empty[kv.s], kv.ph ^ 1, p.err, DEVERR_WAIT_TMA)) {
-              *abort_flag = 1;
-              t = w.t1;
-              break;
-            }
-            mbar_arrive_expect_tx(&kv_full[kv.s], S::TILE);
+            if (!(ok = wait_on(&kv_empty[kv.s], kv.ph ^ 1, abort_flag, p.err, DEVERR_WAIT_TMA))) break;
+            mbar_arrive_expect_tx(&kv_full[kv.s], C::KTILE);
             for (int c = 0; c < D / 64; ++c)
-              tma_load_4d(sKV + kv.s * S::TILE + c * S::HALF, v ? &p.tmV : &p.tmK, &kv_full[kv.s], c * 64, t * KT,
-                          hk * (v ? p.vh_mul : p.kvh_mul), w.b * (v ? p.vb_mul : p.kvb_mul));
+              tma_load_4d(sKV + kv.s * C::KTILE + c * C::KHALF, v ? &p.tmV : &p.tmK, &kv_full[kv.s], c * 64, t * KT,
+                          hk * (v ? p.vh_mul : p.kh_mul), w.b * (v ? p.vb_mul : p.kb_mul));
             kv.advance(p.ring);
             ++nkv;
           }
       }
-      if (*abort_flag) {  // leave no copy in flight behind: the last ones issued into each buffer
+      if (!ok || *abort_flag) {  // leave no copy in flight behind: the last ones issued into each buffer
+        *abort_flag = 1;
         for (unsigned i = 0; i < min(nkv, (unsigned)p.ring); ++i) {
-          kv.s = kv.s ? kv.s - 1 : (kv.ph ^= 1, p.ring - 1);
+          kv.back(p.ring);
           mbar_wait(&kv_full[kv.s], kv.ph, p.err, DEVERR_WAIT_TMA);
         }
         for (unsigned i = 0; i < min(nq, (unsigned)p.nq); ++i) {
-          q.s = q.s ? q.s - 1 : (q.ph ^= 1, p.nq - 1);
+          q.back(p.nq);
           mbar_wait(&q_full[q.s], q.ph, p.err, DEVERR_WAIT_TMA);
         }
       }
     }
-  } else if (warp == 8) {
+  } else if (svc == 0) {
     if (elect_one()) {
       RingPos kv, q;
       bool ok = true;
-      int ph_p[2] = {0, 0};
-      for (unsigned u = blockIdx.x; ok && u < units; u += gridDim.x) {
-        Unit w;
-        if (!unit_of(p, u, w) || w.t0 >= w.t1) continue;
-        const int nw = w.rows > QT ? 2 : 1, qb = q.s;
-        ok = !*abort_flag && mbar_wait(&q_full[q.s], q.ph, p.err, DEVERR_WAIT_MMA);
-        q.advance(p.nq);
-        auto kv_wait = [&](const RingPos& r) {
-          return !*abort_flag && mbar_wait(&kv_full[r.s], r.ph, p.err, DEVERR_WAIT_MMA);
-        };
-        auto keys16 = [&](int t) { return (min(w.n - t * KT, KT) + 15) / 16; };  // 16-key steps of tile t
-        auto issue_s = [&](int i, int t, int slot) {
-          const uint32_t aQ = smem_u32(sQ + (qb * 2 + i) * S::TILE), aK = smem_u32(sKV + slot * S::TILE);
-          // the score tile is as wide as the softmax reads it: 32-key chunks
-          const uint32_t id = idesc_f16(128, 0, BF16) | ((uint32_t)(((keys16(t) + 1) / 2 * 32) >> 3) << 17);
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (kk / 4) * S::HALF + (kk % 4) * 32;
-            umma_f16(tmem + i * 128, sdesc_sw128(aQ + off, 16, 1024), sdesc_sw128(aK + off, 16, 1024), id, kk != 0);
+      unsigned ph_p = 0, ph_c = 0, ph_r = 0;  // phases of p_full, v_clean, o_read, one bit each
+      unsigned used = 0;                      // groups whose O has to be read before new scores (SHORT)
+      auto wait = [&](uint64_t* b, int ph) { return wait_on(b, ph, abort_flag, p.err, DEVERR_WAIT_MMA); };
+      for (const Item* item; ok && (item = next(DEVERR_WAIT_MMA)); done()) {
+        const Item w = *item;
+        if (w.t0 >= w.t1) continue;
+        const int nw = (w.rows + 127) / 128, qb = q.s * qtiles;
+        auto issue_s = [&](int i, int qt, int t, int slot) {
+          if (SHORT) {
+            if ((used >> i) & 1) {
+              ok = wait(&o_read[i], (ph_r >> i) & 1);
+              ph_r ^= 1u << i;
+              tc_fence_after();
+            }
+            used |= 1u << i;
           }
+          const uint64_t dq = kdesc(smem_u32(sQ + (qb + qt) * C::QTILE)), dk = kdesc(smem_u32(sKV + slot * C::KTILE));
+          // the score tile is as wide as the softmax reads it: 32-key chunks
+          const int n = min((w.n - t * KT + 31) / 32, KT / 32) * 32;
+          const uint32_t id = idesc_f16(128, 0, BF16) | ((uint32_t)(n >> 3) << 17);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+            umma_f16(tmem + i * C::TCOLS, dq + ((kk / 4) * C::QHALF + (kk % 4) * 32) / 16,
+                     dk + ((kk / 4) * C::KHALF + (kk % 4) * 32) / 16, id, kk != 0);
           umma_commit(&s_full[i]);
         };
-        auto issue_pv = [&](int i, int t, int slot) {
-          const uint32_t aV = smem_u32(sKV + slot * S::TILE);
+        auto issue_pv = [&](int i, int t, int slot, bool first) {
+          const uint64_t dv = sdesc_sw128(0, C::KHALF, 1024) | (smem_u32(sKV + slot * C::KTILE) >> 4);
           constexpr uint32_t id = idesc_f16(128, D, BF16, false, true);  // V is MN-major (d contiguous)
-          const int steps = keys16(t);
-          for (int kk = 0; kk < steps; ++kk)
-            umma_f16_ta(tmem + 256 + i * D, tmem + i * 128 + kk * 8, sdesc_sw128(aV + kk * 2048, S::HALF, 1024), id,
-                        t != w.t0 || kk != 0);
+          const int steps = min((w.n - t * KT + 15) / 16, KT / 16);
+#pragma unroll
+          for (int kk = 0; kk < KT / 16; ++kk)
+            if (kk < steps)
+              umma_f16_ta(tmem + i * C::TCOLS + C::TO, tmem + i * C::TCOLS + kk * 8, dv + kk * 2048 / 16, id,
+                          !first || kk != 0);
         };
-        if (ok && (ok = kv_wait(kv))) {
-          tc_fence_after();
-          for (int i = 0; i < nw; ++i) issue_s(i, w.t0, kv.s);
-          umma_commit(&kv_empty[kv.s]);
-        }
-        for (int t = w.t0; ok && t < w.t1; ++t) {  // kv: the K tile of t, then its V tile, then the next K tile
-          const bool more = t + 1 < w.t1;
-          const RingPos v = kv.next(p.ring), k2 = v.next(p.ring);
-          ok = kv_wait(v) && (!more || kv_wait(k2));
-          for (int i = 0; ok && i < nw; ++i) {
-            ok = !*abort_flag && mbar_wait(&p_full[i], ph_p[i], p.err, DEVERR_WAIT_MMA);
-            ph_p[i] ^= 1;
-            if (!ok) break;
-            tc_fence_after();
-            issue_pv(i, t, v.s);
-            if (more) issue_s(i, t + 1, k2.s);
-            else umma_commit(&o_full[i]);
+        auto v_wait = [&](const RingPos& v, int t) {
+          if (!wait(&kv_full[v.s], v.ph)) return false;
+          if (cleaned(w, t)) {
+            if (!wait(&v_clean[v.s], (ph_c >> v.s) & 1)) return false;
+            ph_c ^= 1u << v.s;
           }
-          if (!ok) break;
-          umma_commit(&kv_empty[v.s]);
-          if (more) umma_commit(&kv_empty[k2.s]);
-          else umma_commit(&q_empty[qb]);
-          kv = k2;
+          return true;
+        };
+        auto p_wait = [&](int i) {
+          const bool r = wait(&p_full[i], (ph_p >> i) & 1);
+          ph_p ^= 1u << i;
+          tc_fence_after();
+          return r;
+        };
+        ok = wait(&q_full[q.s], q.ph);
+        const int qs = q.s;
+        q.advance(p.nq);
+        if (!p.by_keys) {
+          if (ok && (ok = wait(&kv_full[kv.s], kv.ph))) {
+            tc_fence_after();
+            for (int i = 0; ok && i < nw; ++i) issue_s(i, i, w.t0, kv.s);
+            umma_commit(&kv_empty[kv.s]);
+          }
+          for (int t = w.t0; ok && t < w.t1; ++t) {  // kv: the K tile of t, then its V tile, then the next K tile
+            const bool more = t + 1 < w.t1;
+            const RingPos v = kv.next(p.ring), k2 = v.next(p.ring);
+            ok = v_wait(v, t) && (!more || wait(&kv_full[k2.s], k2.ph));
+            for (int i = 0; ok && i < nw; ++i) {
+              if (!(ok = p_wait(i))) break;
+              issue_pv(i, t, v.s, t == w.t0);
+              if (more) issue_s(i, i, t + 1, k2.s);
+              else umma_commit(&o_full[i]);
+            }
+            if (!ok) break;
+            umma_commit(&kv_empty[v.s]);
+            umma_commit(more ? &kv_empty[k2.s] : &q_empty[qs]);
+            kv = k2;
+          }
+        } else {
+          // group i takes tiles t0 + i, t0 + i + NW, ...: P V of a tile, then S of the group's next one
+          RingPos v = kv.next(p.ring);  // V tile of `t`; kv: K tile of `t + NW`
+          for (int t = w.t0 - NW; ok && t < w.t1; ++t) {
+            if (t >= w.t0) {
+              const int i = (t - w.t0) % NW;
+              if (!(ok = v_wait(v, t) && p_wait(i))) break;
+              issue_pv(i, t, v.s, t - w.t0 < NW);
+              if (t + NW >= w.t1) umma_commit(&o_full[i]);
+              umma_commit(&kv_empty[v.s]);
+              v = v.next(p.ring).next(p.ring);
+            }
+            if (t + NW < w.t1) {
+              if (!(ok = wait(&kv_full[kv.s], kv.ph))) break;
+              tc_fence_after();
+              issue_s((t + NW - w.t0) % NW, 0, t + NW, kv.s);
+              umma_commit(t + NW == w.t1 - 1 ? &q_empty[qs] : &kv_empty[kv.s]);
+              if (t + NW == w.t1 - 1) umma_commit(&kv_empty[kv.s]);
+              kv = kv.next(p.ring).next(p.ring);
+            }
+          }
         }
       }
       if (!ok) *abort_flag = 1;
     }
-  }
+  } else if (svc == 2) {
+    RingPos kv;
+    bool ok = true;
+    for (const Item* item; ok && (item = next(DEVERR_WAIT_SOFTMAX));) {
+      const Item w = *item;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[ip.s]);
+      ip.advance(kItems);
+      for (int t = w.t0; ok && t < w.t1; ++t) {
+        // every tile is waited for, cleaned or not: a wait that runs a whole ring ahead would find the phase before it
+        const RingPos k = kv, v = kv.next(p.ring);
+        kv = v.next(p.ring);
+        ok = wait_on(&kv_full[k.s], k.ph, abort_flag, p.err, DEVERR_WAIT_SOFTMAX);
+        if (!cleaned(w, t)) {
+          ok = __all_sync(0xffffffffu, ok && wait_on(&kv_full[v.s], v.ph, abort_flag, p.err, DEVERR_WAIT_SOFTMAX));
+          continue;
+        }
+        const int left = min(w.n - t * KT, KT), reach = (left + 15) / 16 * 16;  // rows that P V reads
+        uint32_t off[KT / 32];
+#pragma unroll
+        for (int c = 0; c < KT / 32; ++c) {
+          const int j = c * 32 + lane;
+          off[c] = __ballot_sync(0xffffffffu, j < reach && (j >= left || (p.mask && !__ldg(p.mask + (long long)w.b * p.Skv + t * KT + j))));
+        }
+        ok = __all_sync(0xffffffffu, ok && wait_on(&kv_full[v.s], v.ph, abort_flag, p.err, DEVERR_WAIT_SOFTMAX));
+        if (!ok) break;
+        uint4* vt = reinterpret_cast<uint4*>(sKV + v.s * C::KTILE);
+#pragma unroll
+        for (int c = 0; c < KT / 32; ++c)
+          if (off[c]) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)  // four rows at a time: lane / 8 the row, lane % 8 its 16-byte piece
+              if ((off[c] >> (k * 4 + lane / 8)) & 1) {
+#pragma unroll
+                for (int h = 0; h < D / 64; ++h) vt[h * (C::KHALF / 16) + (c * 32 + k * 4) * 8 + lane] = make_uint4(0, 0, 0, 0);
+              }
+          }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_clean[v.s]);
+      }
+    }
+    if (!ok) *abort_flag = 1;
+  } else if (svc == 3) {
+    if (elect_one()) {
+      Items<KT> it(p, ends);
+      for (Item w = {}; w.rows >= 0; ip.advance(kItems)) {
+        const bool more = it.next(w);
+        if (!wait_on(&item_empty[ip.s], ip.ph ^ 1, abort_flag, p.err, DEVERR_WAIT_EPI)) {
+          *abort_flag = 1;
+          break;
+        }
+        if (!more) w.rows = 0;
+        items[ip.s] = w;
+        mbar_arrive(&item_full[ip.s]);
+        if (!more) break;
+      }
+    }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // ---------------- softmax warps: one packed row per thread ----------------
     const int i = warp / 4, wq = warp & 3;
     const int lrow = wq * 32 + lane;  // row of the tile = TMEM lane
-    const uint32_t lane_off = static_cast<uint32_t>(wq * 32) << 16;
-    const uint32_t tS = tmem + i * 128 + lane_off, tO = tmem + 256 + i * D + lane_off;
-    const long long R = (long long)p.Sq * p.GP;
+    const uint32_t tS = tmem + i * C::TCOLS + (static_cast<uint32_t>(wq * 32) << 16), tO = tS + C::TO;
+    const int row = p.by_keys ? lrow : i * 128 + lrow;               // row of the item
+    const int warp_row = p.by_keys ? wq * 32 : i * 128 + wq * 32;
+    const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2);
     int ph_s = 0, ph_o = 0;
-    RingPos v;  // the V tile of the current key tile (first row tile's warps only: every unit has that one)
-    v.advance(p.ring);
     bool ok = true;
-    for (unsigned u = blockIdx.x; ok && u < units; u += gridDim.x) {
-      Unit w;
-      if (!unit_of(p, u, w)) continue;
-      const int row = i * QT + lrow;               // row of the unit
-      const bool mine = row < w.rows;
-      const bool warp_on = i * QT + wq * 32 < w.rows;
+    for (const Item* item; ok && (item = next(DEVERR_WAIT_SOFTMAX)) != nullptr;) {
+      const Item& w = *item;  // read again where it is used: registers are short here
+      const int slot = ip.s;
+      ip.advance(kItems);
+      if (!p.by_keys && i * 128 >= w.rows) {
+        if (lane == 0) mbar_arrive(&item_empty[slot]);
+        continue;
+      }
+      const bool mine = row < w.rows, warp_on = warp_row < w.rows;
+      const int ta = p.by_keys ? w.t0 + i : w.t0, tstep = p.by_keys ? NW : 1;  // this group's key tiles
+      const bool any = ta < w.t1;
       float m_run = -INFINITY, l_run = 0.f;
-      if (i * QT < w.rows) {
-        for (int t = w.t0; ok && t < w.t1; ++t) {
-          ok = !*abort_flag && mbar_wait(&s_full[i], ph_s, p.err, DEVERR_WAIT_SOFTMAX);
-          ok = __all_sync(0xffffffffu, ok);
-          ph_s ^= 1;
-          if (!ok) break;
-          tc_fence_after();
-          const int left = w.n - t * KT;  // > 0; keys of this tile inside the length
-          const int nc = min(4, (left + 31) / 32);
-          uint32_t bits[4];
-          const bool partial = left < KT || p.mask;
-          if (partial) {
+      for (int t = ta; t < w.t1; t += tstep) {
+        const int left = w.n - t * KT;  // > 0; keys of this tile inside the length
+        const int nc = min(KT / 32, (left + 31) / 32);
+        const bool partial = left < KT || p.mask;
+        uint32_t bits[KT / 32];
+        if (partial) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const int j = t * KT + c * 32 + lane;
-              bits[c] = __ballot_sync(0xffffffffu, j < w.n && (!p.mask || __ldg(p.mask + (long long)w.b * p.Skv + j)));
-            }
-            // V rows of masked keys inside the tensor are zeroed (one key per thread of the first row tile; keys
-            // past Skv are zero already)
-            if (i == 0) {
-              ok = mbar_wait(&kv_full[v.s], v.ph, p.err, DEVERR_WAIT_SOFTMAX);
-              const uint32_t mine_bits = wq == 0 ? bits[0] : wq == 1 ? bits[1] : wq == 2 ? bits[2] : bits[3];
-              if (ok && !((mine_bits >> lane) & 1) && lrow < (left + 15) / 16 * 16) {
-                uint8_t* vrow = sKV + v.s * S::TILE + lrow * 128;
-#pragma unroll
-                for (int c = 0; c < D / 8; ++c)
-                  *reinterpret_cast<uint4*>(vrow + (c / 8) * S::HALF + (c % 8) * 16) = make_uint4(0, 0, 0, 0);
-                fence_async_smem();
-              }
-              __syncwarp();
-            }
+          for (int c = 0; c < KT / 32; ++c) {
+            const int j = c * 32 + lane;
+            bits[c] = __ballot_sync(0xffffffffu, j < left && (!p.mask || __ldg(p.mask + (long long)w.b * p.Skv + t * KT + j)));
           }
-          if (warp_on) {
-            float s[KT];
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-              if (c < nc) tmem_ld32(tS + c * 32, reinterpret_cast<uint32_t(&)[32]>(s[c * 32]));
+        }
+        ok = wait_on(&s_full[i], ph_s, abort_flag, p.err, DEVERR_WAIT_SOFTMAX);
+        ok = __all_sync(0xffffffffu, ok);
+        ph_s ^= 1;
+        if (!ok) break;
+        tc_fence_after();
+        if (warp_on) {
+          // two passes over the scores in TMEM, 32 at a time: the maximum, then the exponentials
+          float s[32];
+          auto load = [&](int c) {
+            tmem_ld32(tS + c * 32, reinterpret_cast<uint32_t(&)[32]>(s));
             tmem_wait_ld();
-            float mx = -INFINITY;
+            if (partial && bits[c] != 0xffffffffu) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-              if (c < nc) {
-                if (partial && bits[c] != 0xffffffffu) {
-#pragma unroll
-                  for (int k = 0; k < 32; ++k)
-                    if (!((bits[c] >> k) & 1)) s[c * 32 + k] = -INFINITY;
-                }
-                float a = -INFINITY, b = -INFINITY;
-#pragma unroll
-                for (int k = 0; k < 32; k += 4) {
-                  a = max3f(a, s[c * 32 + k], s[c * 32 + k + 1]);
-                  b = max3f(b, s[c * 32 + k + 2], s[c * 32 + k + 3]);
-                }
-                mx = max3f(mx, a, b);
-              }
-            mx *= p.scale_log2;  // the scale is positive
-            const bool move = mx > m_run + kRescale;
-            const float m_new = move ? mx : m_run;
-            const float alpha = move ? ex2_approx(m_run - m_new) : 1.0f;
-            const float m_sub = m_new == -INFINITY ? 0.f : m_new;  // no valid key yet: every p is 2^-inf = 0
-            const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2), nm2 = f2_pack(-m_sub, -m_sub);
-            uint64_t acc2 = 0;
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-              if (c < nc) {
-                uint32_t pk[16];
-#pragma unroll
-                for (int k = 0; k < 32; k += 2) {
-                  const uint64_t x = fma2(f2_pack(s[c * 32 + k], s[c * 32 + k + 1]), sc2, nm2);
-                  const float a = ex2_approx(lo_f(x)), b = ex2_approx(hi_f(x));
-                  acc2 = add2(acc2, f2_pack(a, b));
-                  pk[k / 2] = pack2<BF16>(a, b);
-                }
-                tmem_st16(tS + c * 16, pk);
-              }
-            l_run = l_run * alpha + (lo_f(acc2) + hi_f(acc2));
-            m_run = m_new;
-            if (t != w.t0 && __any_sync(0xffffffffu, move)) {
-              // this tile's scores follow the previous P V on the tensor pipe: O is complete
-#pragma unroll
-              for (int c = 0; c < D / 32; ++c) {
-                uint32_t r[32];
-                tmem_ld32(tO + c * 32, r);
-                tmem_wait_ld();
-#pragma unroll
-                for (int k = 0; k < 32; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * alpha);
-                tmem_st32(tO + c * 32, r);
-              }
+              for (int k = 0; k < 32; ++k)
+                if (!((bits[c] >> k) & 1)) s[k] = -INFINITY;
             }
-            tmem_wait_st();
-          }
-          tc_fence_before();
-          mbar_arrive(&p_full[i]);
-          v.advance(p.ring, 2);
-        }
-        if (ok && w.t1 > w.t0) {
-          ok = !*abort_flag && mbar_wait(&o_full[i], ph_o, p.err, DEVERR_WAIT_SOFTMAX);
-          ok = __all_sync(0xffffffffu, ok);
-          ph_o ^= 1;
-          tc_fence_after();
-        }
-        if (ok && warp_on) {
-          const long long tr = w.row0 + row;  // packed row of the group
-          const long long pr = ((long long)w.b * p.HG + w.hg) * R + tr + (long long)w.sp * p.B * p.HG * R;
-          const bool any = w.t1 > w.t0;
-          const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;
-          uint16_t* o = static_cast<uint16_t*>(p.O) + w.b * p.osb + (tr >> p.gps) * p.oss +
-                        (w.hg * p.GP + (tr & (p.GP - 1))) * p.osh;
+          };
+          float mx = -INFINITY;
 #pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t r[32];
-            if (any) {  // warp-uniform
+          for (int c = 0; c < KT / 32; ++c)
+            if (c < nc) {
+              load(c);
+              float a = mx, b = -INFINITY;
+#pragma unroll
+              for (int k = 0; k < 32; k += 4) {
+                a = max3f(a, s[k], s[k + 1]);
+                b = max3f(b, s[k + 2], s[k + 3]);
+              }
+              mx = fmaxf(a, b);
+            }
+          mx *= p.scale_log2;  // the scale is positive
+          const bool move = mx > m_run + kRescale;
+          const float m_new = move ? mx : m_run;
+          const float alpha = move ? ex2_approx(m_run - m_new) : 1.0f;
+          const float m_sub = m_new == -INFINITY ? 0.f : m_new;  // no valid key yet: every p is 2^-inf = 0
+          const uint64_t nm2 = f2_pack(-m_sub, -m_sub);
+          uint64_t acc[4] = {0, 0, 0, 0};
+          // P of chunk c lies over the scores of chunk c / 2, which have been read again by then
+#pragma unroll
+          for (int c = 0; c < KT / 32; ++c)
+            if (c < nc) {
+              load(c);
+              uint32_t* w32 = reinterpret_cast<uint32_t*>(s);  // 32 scores -> 16 words of probabilities, in place
+#pragma unroll
+              for (int k = 0; k < 32; k += 2) {
+                const uint64_t x = fma2(f2_pack(s[k], s[k + 1]), sc2, nm2);
+                const float a = ex2_approx(lo_f(x)), b = ex2_approx(hi_f(x));
+                acc[k / 2 % 4] = add2(acc[k / 2 % 4], f2_pack(a, b));
+                w32[k / 2] = pack2<BF16>(a, b);
+              }
+              tmem_st16(tS + c * 16, w32);
+            }
+          const uint64_t sum = add2(add2(acc[0], acc[1]), add2(acc[2], acc[3]));
+          l_run = l_run * alpha + (lo_f(sum) + hi_f(sum));
+          m_run = m_new;
+          if (t != ta && __any_sync(0xffffffffu, move)) {
+            // this tile's scores follow the previous P V on the tensor pipe: O is complete
+            const uint64_t al2 = f2_pack(alpha, alpha);
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t r[32];
               tmem_ld32(tO + c * 32, r);
               tmem_wait_ld();
-            }
-            if (p.NS > 1) {
-              if (mine && any) {
-                float4* d = reinterpret_cast<float4*>(p.part + pr * D + c * 32);
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                  d[k] = make_float4(__uint_as_float(r[4 * k]), __uint_as_float(r[4 * k + 1]),
-                                     __uint_as_float(r[4 * k + 2]), __uint_as_float(r[4 * k + 3]));
+              for (int k = 0; k < 32; k += 2) {
+                const uint64_t x = mul2(f2_pack(__uint_as_float(r[k]), __uint_as_float(r[k + 1])), al2);
+                r[k] = (uint32_t)x;
+                r[k + 1] = (uint32_t)(x >> 32);
               }
-            } else if (mine) {
-              uint32_t h[16];
-#pragma unroll
-              for (int k = 0; k < 16; ++k)  // no valid key: zeros, whatever O holds
-                h[k] = l_run == 0.f ? 0u : pack2<BF16>(__uint_as_float(r[2 * k]) * inv, __uint_as_float(r[2 * k + 1]) * inv);
-              if (p.wide) {
-#pragma unroll
-                for (int k = 0; k < 2; ++k)
-                  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(o + c * 32 + k * 16),
-                               "r"(h[8 * k]), "r"(h[8 * k + 1]), "r"(h[8 * k + 2]), "r"(h[8 * k + 3]), "r"(h[8 * k + 4]),
-                               "r"(h[8 * k + 5]), "r"(h[8 * k + 6]), "r"(h[8 * k + 7])
-                               : "memory");
-              } else {
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  reinterpret_cast<uint4*>(o + c * 32)[k] = make_uint4(h[4 * k], h[4 * k + 1], h[4 * k + 2], h[4 * k + 3]);
-              }
+              tmem_st32(tO + c * 32, r);
             }
           }
-          if (p.NS > 1 && mine)
-            reinterpret_cast<float2*>(p.part + (long long)p.NS * p.B * p.HG * R * D)[pr] = make_float2(m_run, l_run);
+          tmem_wait_st();
         }
-        tc_fence_before();  // O is read before the next unit's first P V, which waits for this warp's p_full
+        tc_fence_before();
+        mbar_arrive(&p_full[i]);
       }
+      if (ok && any) {
+        ok = wait_on(&o_full[i], ph_o, abort_flag, p.err, DEVERR_WAIT_SOFTMAX);
+        ok = __all_sync(0xffffffffu, ok);
+        ph_o ^= 1;
+        tc_fence_after();
+      }
+      if (!ok) break;
+      const long long pr = ((long long)w.slot * NW + i) * 128 + lrow;  // by keys: the row's partial
+      const int tr = w.row0 + row;                                     // packed row of the group
+      const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;
+      const uint64_t inv2 = f2_pack(inv, inv);
+      uint16_t* o = static_cast<uint16_t*>(p.O) + w.b * p.osb + (tr >> p.gps) * p.oss +
+                    ((w.hg << p.gps) + (tr & (p.GP - 1))) * p.osh;
+      if (warp_on) {
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t r[32];
+          if (any) {  // warp-uniform
+            tmem_ld32(tO + c * 32, r);
+            tmem_wait_ld();
+          }
+          if (SHORT && c == D / 32 - 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (any && lane == 0) mbar_arrive(&o_read[i]);
+          }
+          if (p.by_keys) {
+            if (mine && any) {
+              float4* d = reinterpret_cast<float4*>(p.part + pr * D + c * 32);
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                d[k] = make_float4(__uint_as_float(r[4 * k]), __uint_as_float(r[4 * k + 1]),
+                                   __uint_as_float(r[4 * k + 2]), __uint_as_float(r[4 * k + 3]));
+            }
+          } else if (mine) {
+            uint32_t h[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {  // no valid key: zeros, whatever O holds
+              const uint64_t x = mul2(f2_pack(__uint_as_float(r[2 * k]), __uint_as_float(r[2 * k + 1])), inv2);
+              h[k] = l_run == 0.f ? 0u : pack2<BF16>(lo_f(x), hi_f(x));
+            }
+            if (p.wide) {
+#pragma unroll
+              for (int k = 0; k < 2; ++k)
+                asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(o + c * 32 + k * 16),
+                             "r"(h[8 * k]), "r"(h[8 * k + 1]), "r"(h[8 * k + 2]), "r"(h[8 * k + 3]), "r"(h[8 * k + 4]),
+                             "r"(h[8 * k + 5]), "r"(h[8 * k + 6]), "r"(h[8 * k + 7])
+                             : "memory");
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                reinterpret_cast<uint4*>(o + c * 32)[k] = make_uint4(h[4 * k], h[4 * k + 1], h[4 * k + 2], h[4 * k + 3]);
+            }
+          }
+        }
+        if (p.by_keys && mine)
+          reinterpret_cast<float2*>(p.part + (long long)p.slots * NW * 128 * D)[pr] = make_float2(m_run, l_run);
+        tc_fence_before();  // O is read before the next item's first P V, which waits for this warp's p_full
+      } else if (SHORT && any && lane == 0) {
+        mbar_arrive(&o_read[i]);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[slot]);
     }
     if (!ok) *abort_flag = 1;
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (svc == 0) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
 }
 
-// Joins the key splits: one warp per packed row.
+// Joins the parts of the keys: one warp per packed row.
 template <bool BF16, int D>
 __global__ void __launch_bounds__(128) xattn_join_kernel(const __grid_constant__ XattnParams p) {
+  constexpr int NW = XCfg<D, false>::NW, KT = XCfg<D, false>::KT;
   pdl_begin();
-  const long long R = (long long)p.Sq * p.GP, NR = (long long)p.B * p.HG * R;
-  const long long r = (long long)blockIdx.x * 4 + threadIdx.x / 32;
   const int lane = threadIdx.x & 31;
-  if (r >= NR) return;
-  const int b = (int)(r / R / p.HG), hg = (int)(r / R % p.HG);
-  const long long t = r % R;
-  if (p.q_len && t / p.GP >= __ldg(p.q_len + b)) return;
-  const float2* ml = reinterpret_cast<const float2*>(p.part + p.NS * NR * D);
-  float m = -INFINITY;
-  for (int s = lane; s < p.NS; s += 32) {
-    const float2 v = ml[s * NR + r];
-    if (v.y != 0.f) m = fmaxf(m, v.x);
+  const int pair = (int)(blockIdx.y);  // (b, hg, row block)
+  const int b = pair / p.RT / p.HG, hg = pair / p.RT % p.HG, rt = pair % p.RT;
+  const int lrow = blockIdx.x * 4 + threadIdx.x / 32, t = rt * 128 + lrow;
+  const int q = p.q_len ? min(max(__ldg(p.q_len + b), 0), p.Sq) : p.Sq;
+  if (t >= q << p.gps) return;
+  // this block's place in the key tiles laid end to end, and the CTAs that share it
+  int before = 0, total = 0, nt = 0;
+  for (int x = lane; x < p.B; x += 32) {
+    const int n = ((p.kv_len ? min(max(__ldg(p.kv_len + x), 0), p.Skv) : p.Skv) + KT - 1) / KT;
+    total += n;
+    if (x < b) before += n;
+    if (x == b) nt = n;
   }
-  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  constexpr int W = D / 32;
-  float acc[W] = {}, l = 0.f;
-  for (int s = 0; s < p.NS; ++s) {
-    const float2 v = ml[s * NR + r];
-    if (v.y == 0.f) continue;  // nothing valid in this split (its O may not even be written); NaN passes
-    const float f = ex2_approx(v.x - m);
-    l = fmaf(v.y, f, l);
-    const float* o = p.part + (s * NR + r) * D + lane * W;
 #pragma unroll
-    for (int k = 0; k < W; ++k) acc[k] = fmaf(o[k], f, acc[k]);
+  for (int o = 16; o; o >>= 1) {
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+    nt += __shfl_xor_sync(0xffffffffu, nt, o);
+  }
+  const long long all = (long long)total * p.HG * p.RT;
+  const long long g0 = (long long)before * p.HG * p.RT + (long long)(pair - b * p.HG * p.RT) * nt, g1 = g0 + nt;
+  float m = -INFINITY, l = 0.f;
+  constexpr int W = D / 32;
+  float acc[W] = {};
+  if (nt) {
+    // CTA c has tiles [all c / grid, all (c + 1) / grid): the first and last that meet [g0, g1)
+    const int c0 = (int)(((g0 + 1) * p.grid - 1) / all), c1 = (int)((g1 * p.grid - 1) / all);
+    const float2* ml = reinterpret_cast<const float2*>(p.part + (long long)p.slots * NW * 128 * D);
+    const int n = (c1 - c0 + 1) * NW;
+    const long long base = ((long long)(c0 + pair) * NW) * 128 + lrow;
+    auto part_of = [&](int s) {  // (max, sum) of part s; sum 0: nothing valid there, its O may not even be written
+      if (s >= n) return make_float2(-INFINITY, 0.f);
+      const long long c = c0 + s / NW;  // fewer tiles than CTAs: some have none
+      if (all < p.grid && all * c / p.grid == all * (c + 1) / p.grid) return make_float2(-INFINITY, 0.f);
+      return ml[base + s * 128];
+    };
+    for (int s = lane; s < n; s += 32) {
+      const float2 v = part_of(s);
+      if (v.y != 0.f) m = fmaxf(m, v.x);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int s0 = 0; s0 < n; s0 += 32) {
+      const float2 v = part_of(s0 + lane);
+      const float mine = v.y != 0.f ? ex2_approx(v.x - m) : 0.f;  // NaN passes
+      if (v.y != 0.f) l = fmaf(v.y, mine, l);
+      unsigned with = __ballot_sync(0xffffffffu, v.y != 0.f);
+      while (with) {
+        const int j = __ffs(with) - 1;
+        with &= with - 1;
+        const float f = __shfl_sync(0xffffffffu, mine, j);
+        const float* o = p.part + (base + (s0 + j) * 128) * D + lane * W;
+#pragma unroll
+        for (int k = 0; k < W; ++k) acc[k] = fmaf(o[k], f, acc[k]);
+      }
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
   }
   const float inv = l == 0.f ? 0.f : 1.0f / l;
-  uint16_t* o = static_cast<uint16_t*>(p.O) + b * p.osb + t / p.GP * p.oss + (hg * p.GP + t % p.GP) * p.osh + lane * W;
+  uint16_t* o = static_cast<uint16_t*>(p.O) + b * p.osb + (t >> p.gps) * p.oss +
+                ((hg << p.gps) + (t & (p.GP - 1))) * p.osh + lane * W;
 #pragma unroll
   for (int k = 0; k < W; k += 2) reinterpret_cast<uint32_t*>(o)[k / 2] = pack2<BF16>(acc[k] * inv, acc[k + 1] * inv);
 }
 
 struct XPlan {
-  int GP, HG, RT, NS;
+  int GP, HG, RT, tpi, by_keys, grid, slots;
 };
-XPlan xattn_plan(const Ctx* c, int B, int H, int Hkv, int Sq, int Skv) {
-  XPlan x;
-  const int G = H / Hkv;
+XPlan xattn_plan(const Ctx* c, int B, int H, int Hkv, int Sq, int Skv, int D) {
+  XPlan x = {};
+  const int G = H / Hkv, NW = D == 64 ? 4 : 2, KT = D == 64 && Skv > 128 ? 64 : 128;
   x.GP = G & -G;  // packed heads: the power of two in the group (tiles of 128 rows hold whole tokens)
-  if (x.GP > QT) x.GP = QT;
+  if (x.GP > 128) x.GP = 128;
   x.HG = H / x.GP;
-  x.RT = (int)(((long long)Sq * x.GP + 2 * QT - 1) / (2 * QT));
-  const long long units = (long long)B * x.HG * x.RT;
-  const int nt = (Skv + KT - 1) / KT;
-  x.NS = 1;
-  if (units * 2 <= c->num_sms) x.NS = (int)std::max<long long>(1, std::min<long long>(nt, 2 * c->num_sms / units));
+  const long long rows = (long long)Sq * x.GP, tiles = (rows + 127) / 128, nt = ((long long)Skv + KT - 1) / KT;
+  // By keys: when the row tiles leave most SMs idle and there are key tiles to share out.
+  if ((long long)B * x.HG * tiles * 2 <= c->num_sms && nt >= 4 && B <= kMaxByKeys &&
+      nt * B * x.HG * tiles < (1ll << 30)) {
+    x.by_keys = 1;
+    x.tpi = 1;
+    x.RT = (int)tiles;
+    x.grid = (int)std::min<long long>(c->num_sms, std::max<long long>(1, B * x.HG * tiles * nt / 2));
+    x.slots = x.grid + B * x.HG * x.RT;
+    return x;
+  }
+  // By rows: as many row tiles per item as fill the SMs in the fewest rounds (an item costs a share of its
+  // latency however many tiles it has).
+  double best = 1e30;
+  for (int n = 1; n <= NW; ++n) {
+    const long long items = (long long)B * x.HG * ((tiles + n - 1) / n);
+    const double cost = (double)((items + c->num_sms - 1) / c->num_sms) * (2.0 + n);
+    if (cost <= best) {
+      best = cost;
+      x.tpi = n;
+    }
+  }
+  x.RT = (int)((tiles + x.tpi - 1) / x.tpi);
   return x;
 }
 
-template <bool BF16, int D>
-int launch_xattn(Ctx* c, XattnParams& p, int nt) {
-  using S = XSmem<D>;
-  auto kern = xattn_kernel<BF16, D>;
+template <bool BF16, int D, bool SHORT>
+int launch_xattn(Ctx* c, XattnParams& p) {
+  using C = XCfg<D, SHORT>;
+  auto kern = xattn_kernel<BF16, D, SHORT>;
   static unsigned attr_done = 0;
   if (!(attr_done & (1u << (c->device & 31)))) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::TOTAL) != cudaSuccess)
-      return set_error(c, DI_ECUDA, "cross_attention: shared memory attribute");
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::TOTAL) != cudaSuccess)
+      return cudaGetLastError(), set_error(c, DI_ECUDA, "cross_attention: shared memory attribute");
     attr_done |= 1u << (c->device & 31);
   }
-  p.nq = D == 64 || nt <= 2 ? 2 : 1;
-  p.ring = S::SLOTS - 2 * p.nq;
-  const long long units = (long long)p.B * p.HG * p.RT * p.NS;
-  launch_k(kern, dim3((unsigned)std::min<long long>(units, c->num_sms)), kXThreads, S::TOTAL, c->stream, p);
-  if (p.NS > 1) {
+  const int qtiles = p.by_keys ? 1 : p.tpi;
+  // Q of the next item is fetched under this one; long key sequences leave that for a longer K/V ring (head dim 128)
+  p.nq = D == 64 || qtiles == 1 || p.Skv <= 2 * C::KT ? 2 : 1;
+  p.ring = (int)std::min<uint32_t>(C::MAXRING, (C::DATA - p.nq * qtiles * C::QTILE) / C::KTILE);
+  const unsigned grid = p.by_keys ? p.grid : std::min<unsigned>(p.items, c->num_sms);
+  if (!p.by_keys) {
+    p.d_rt = (int)(grid % p.RT);
+    p.d_hg = (int)(grid / p.RT % p.HG);
+    p.d_b = (int)(grid / p.RT / p.HG);
+  }
+  launch_k(kern, dim3(grid), C::THREADS, C::TOTAL, c->stream, p);
+  if (p.by_keys) {
     const int rc = check_launch(c, "cross_attention");
     if (rc != DI_OK) return rc;
-    const long long rows = (long long)p.B * p.HG * p.Sq * p.GP;
-    launch_k(xattn_join_kernel<BF16, D>, dim3((unsigned)((rows + 3) / 4)), 128, 0, c->stream, p);
+    const int rows = (int)std::min<long long>(128, (long long)p.Sq << p.gps);
+    launch_k(xattn_join_kernel<BF16, D>, dim3((rows + 3) / 4, p.B * p.HG * p.RT), 128, 0, c->stream, p);
   }
   return check_launch(c, "cross_attention");
 }
@@ -568,8 +847,9 @@ using namespace di;
 
 extern "C" size_t di_cross_attention_workspace(di_ctx_t h, int B, int H, int Hkv, int Sq, int Skv, int D) {
   if (!h || B <= 0 || H <= 0 || Hkv <= 0 || Sq <= 0 || Skv <= 0 || D <= 0 || H % Hkv) return 0;
-  const XPlan x = xattn_plan(ctx_of(h), B, H, Hkv, Sq, Skv);
-  return x.NS > 1 ? (size_t)x.NS * B * H * Sq * (D + 2) * 4 : 0;
+  if (D != 64 && D != 128) return 0;
+  const XPlan x = xattn_plan(ctx_of(h), B, H, Hkv, Sq, Skv, D);
+  return (size_t)x.slots * (D == 64 ? 4 : 2) * 128 * (D + 2) * 4;
 }
 
 extern "C" int di_cross_attention(di_ctx_t h, int dtype, const void* Q, const long long q_strides[3], const void* K,
@@ -587,8 +867,8 @@ extern "C" int di_cross_attention(di_ctx_t h, int dtype, const void* Q, const lo
   if (D != 64 && D != 128) return set_error(c, DI_EUNSUPPORTED, "cross_attention: head dim must be 64 or 128");
   if (!aligned16(Q) || !aligned16(K) || !aligned16(V) || !aligned16(O))
     return set_error(c, DI_EINVAL, "cross_attention: pointers must be 16-byte aligned");
-  const XPlan x = xattn_plan(c, B, H, Hkv, Sq, Skv);
-  if ((long long)Sq * x.GP > (1 << 30) || Skv > (1 << 30) || (long long)B * x.HG * x.RT * x.NS > 0x7fffffffll)
+  const XPlan x = xattn_plan(c, B, H, Hkv, Sq, Skv, D);
+  if ((long long)Sq * x.GP > (1 << 30) || Skv > (1 << 30) || (long long)B * x.HG * x.RT > 0x7fffffffll)
     return set_error(c, DI_EUNSUPPORTED, "cross_attention: too many tokens");
   // strides of axes of length one mean nothing: they are replaced by 8 elements (a valid tensor-map stride)
   long long qs[3], ks[3], vs[3], os[3];
@@ -617,8 +897,9 @@ extern "C" int di_cross_attention(di_ctx_t h, int dtype, const void* Q, const lo
   auto str = [](long long stride) { return (uint64_t)(stride ? stride : 8) * 2; };
   const uint64_t qd[5] = {(uint64_t)D, (uint64_t)x.GP, (uint64_t)Sq, len(qs[2], x.HG), len(qs[0], B)};
   const uint64_t qst[4] = {str(qs[2]), str(qs[1]), str(qs[2] * x.GP), str(qs[0])};
-  const uint32_t qbox[5] = {64, (uint32_t)x.GP, (uint32_t)(QT / x.GP), 1, 1};
-  const uint32_t kbox[4] = {64, KT, 1, 1};
+  const uint32_t qbox[5] = {64, (uint32_t)x.GP, (uint32_t)(128 / x.GP), 1, 1};
+  const bool is_short = D == 64 && Skv <= 128;
+  const uint32_t kbox[4] = {64, D == 64 && !is_short ? 64u : 128u, 1, 1};
   const uint64_t kd[4] = {(uint64_t)D, (uint64_t)Skv, len(ks[2], Hkv), len(ks[0], B)};
   const uint64_t vd[4] = {(uint64_t)D, (uint64_t)Skv, len(vs[2], Hkv), len(vs[0], B)};
   const uint64_t kst[3] = {str(ks[1]), str(ks[2]), str(ks[0])}, vst[3] = {str(vs[1]), str(vs[2]), str(vs[0])};
@@ -627,18 +908,23 @@ extern "C" int di_cross_attention(di_ctx_t h, int dtype, const void* Q, const lo
       !make_tmap(&p.tmV, dt, 4, V, vd, vst, kbox, CU_TENSOR_MAP_SWIZZLE_128B, &err))
     return set_error(c, DI_EINVAL, "cross_attention: " + err);
   p.qh_mul = qs[2] != 0; p.qb_mul = qs[0] != 0;
-  p.kvh_mul = ks[2] != 0; p.kvb_mul = ks[0] != 0;
+  p.kh_mul = ks[2] != 0; p.kb_mul = ks[0] != 0;
   p.vh_mul = vs[2] != 0; p.vb_mul = vs[0] != 0;
   p.O = O;
   p.osb = os[0]; p.oss = os[1]; p.osh = os[2];
   p.wide = (reinterpret_cast<uintptr_t>(O) & 31) == 0 && (os[0] | os[1] | os[2]) % 16 == 0;
   while ((1 << p.gps) < x.GP) ++p.gps;
-  p.B = B; p.HG = x.HG; p.GP = x.GP; p.G = H / Hkv; p.Sq = Sq; p.Skv = Skv; p.RT = x.RT; p.NS = x.NS;
+  p.B = B; p.HG = x.HG; p.GP = x.GP; p.G = H / Hkv; p.Sq = Sq; p.Skv = Skv; p.RT = x.RT; p.tpi = x.tpi;
+  p.by_keys = x.by_keys; p.grid = x.grid; p.slots = x.slots;
+  p.items = (unsigned)B * x.HG * x.RT;
   p.q_len = q_len; p.kv_len = kv_len; p.mask = key_mask;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.part = static_cast<float*>(ws);
   p.err = c->d_err;
-  const int nt = (Skv + KT - 1) / KT;
-  if (dtype == DI_F16) return D == 64 ? launch_xattn<false, 64>(c, p, nt) : launch_xattn<false, 128>(c, p, nt);
-  return D == 64 ? launch_xattn<true, 64>(c, p, nt) : launch_xattn<true, 128>(c, p, nt);
+  if (dtype == DI_F16) {
+    if (D == 128) return launch_xattn<false, 128, false>(c, p);
+    return is_short ? launch_xattn<false, 64, true>(c, p) : launch_xattn<false, 64, false>(c, p);
+  }
+  if (D == 128) return launch_xattn<true, 128, false>(c, p);
+  return is_short ? launch_xattn<true, 64, true>(c, p) : launch_xattn<true, 64, false>(c, p);
 }

@@ -201,6 +201,16 @@ def test_lora_repeats_bit_for_bit(ctx, layers, M):
         assert torch.equal(layers.linear_lora(ctx, **s, act="silu"), first)
 
 
+@pytest.mark.parametrize("M,per,K,N,r,L", [(1001, 77, 640, 1280, 64, 6), (3000, 50, 320, 320, 32, 9), (70, 1, 640, 640, 16, 70)])
+def test_lora_back_to_back(ctx, layers, M, per, K, N, r, L):
+    """Thirty calls queued at once: every one gives the same bits, and the right ones."""
+    s = lora_case(M, M, K, N, r, L, torch.float16, res=True, rows=[(m // per * 5) % (L + 1) - 1 for m in range(M)])
+    outs = [layers.linear_lora(ctx, **s, act="gelu") for _ in range(30)]
+    check(outs[0], *lora_ref(s, "gelu"))
+    for o in outs[1:]:
+        assert torch.equal(o, outs[0])
+
+
 def test_lora_c_entry_refusals(ctx, dib):
     L, s = dib.lib(), lora_case(1, 4, 64, 32, 8, 2, torch.float16)
     y = torch.empty(4, 32, dtype=torch.float16, device="cuda")
@@ -464,6 +474,19 @@ def test_cross_repeats_bit_for_bit(ctx, layers, Sq, Skv):
     first = layers.cross_attention(ctx, q, k, v)
     for _ in range(3):
         assert torch.equal(layers.cross_attention(ctx, q, k, v), first)
+
+
+@pytest.mark.parametrize("B,Sq,Skv,G,Hkv,D", [(3, 279, 371, 1, 2, 128), (4, 125, 328, 3, 1, 128), (2, 500, 700, 1, 3, 64), (6, 1, 900, 4, 2, 128),
+                                              (6, 3, 900, 2, 2, 64), (8, 600, 77, 1, 5, 64)])
+def test_cross_back_to_back(ctx, layers, B, Sq, Skv, G, Hkv, D):
+    """Thirty calls queued at once, ragged lengths: every one gives the same bits, and the right ones."""
+    g = gen(Sq)
+    q, k, v = normal(g, B, Sq, G * Hkv, D), normal(g, B, Skv, Hkv, D), normal(g, B, Skv, Hkv, D)
+    lens = torch.randint(0, Skv + 1, (B,), generator=g, device="cuda").int()
+    outs = [layers.cross_attention(ctx, q, k, v, kv_len=lens) for _ in range(30)]
+    check(outs[0], *cross_ref(q, k, v, lens))
+    for o in outs[1:]:
+        assert torch.equal(o, outs[0])
 
 
 @pytest.mark.parametrize("Sq", [1, 140])
