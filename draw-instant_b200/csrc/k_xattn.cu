@@ -28,8 +28,12 @@
 // groups of a CTA take its key tiles in turn.  Each group writes (O, max, sum) in 32 bits to the workspace and a second
 // kernel joins them in key order.
 //
-// Head dim 64: 4 groups, key tiles of 64; up to 128 keys one tile of 128, whose O then lies over the spent scores.
-// Head dim 128: 2 groups, key tiles of 128 (the 512 columns of TMEM hold two O and two S).
+// Key tiles are 128 keys.  Two groups (TMEM holds 128 columns of S and D of O for each); at head dim 64 with up to 128
+// keys three, whose O lies over the spent scores: an item is then one tile of keys, and S of the next item's group i is
+// issued behind P V of this item's group i + 1.
+//
+// O of a warp whose 32 rows are all to be written goes through shared memory (the group's Q tile, which is spent) and a TMA
+// store; ragged rows are stored from registers.
 #include <algorithm>
 #include <cstring>
 
@@ -38,7 +42,7 @@
 namespace di {
 
 struct XattnParams {
-  CUtensorMap tmQ, tmK, tmV;
+  CUtensorMap tmQ, tmK, tmV, tmO;
   void* O;
   long long osb, oss, osh;  // output strides in elements
   int kb_mul, kh_mul, vb_mul, vh_mul, qb_mul, qh_mul;  // 0: the tensor is expanded over that axis
@@ -60,21 +64,22 @@ struct XattnParams {
 namespace {
 
 constexpr float kRescale = 8.0f;  // log2 units
+constexpr int KT = 128;          // keys per tile
+constexpr int kQBufs = 3;         // most Q buffers
 constexpr int kItems = 4;         // work items worked out ahead
 constexpr int kMaxByKeys = 256;   // requests whose key tiles are laid end to end
 
 template <int D, bool SHORT>
 struct XCfg {
-  static constexpr int NW = D == 64 ? 4 : 2;
-  static constexpr int KT = D == 64 && !SHORT ? 64 : 128;       // keys per tile
-  static constexpr int THREADS = 128 * NW + 128;
-  static constexpr int TCOLS = 512 / NW;                        // TMEM columns of a group: S (P over it), O
-  static constexpr int TO = D == 64 ? 64 : 128;                 // first column of O
-  static constexpr uint32_t QTILE = 128 * D * 2, QHALF = 128 * 128;  // Q tile; 64 columns of it (128-byte rows)
-  static constexpr uint32_t KTILE = KT * D * 2, KHALF = KT * 128;
+  static constexpr int NW = SHORT ? 3 : 2;                      // groups of 128 rows
+  static constexpr int SW = 4 * NW;                             // softmax warps
+  static constexpr int THREADS = 32 * SW + 128;
+  static constexpr int TCOLS = SHORT ? 128 : 256;                    // TMEM columns of a group: S (P over it), O
+  static constexpr int TO = SHORT ? 64 : 128;                   // first column of O
+  static constexpr uint32_t TILE = 128 * D * 2, HALF = 128 * 128;  // Q, K or V tile; 64 columns of it (128-byte rows)
   static constexpr uint32_t DATA = D == 64 ? 13 * 16384 : 7 * 32768;
-  static constexpr int MAXRING = D == 64 ? 20 : 6;
-  static constexpr uint32_t BARS = 8 * (4 + 3 * MAXRING + 4 * NW + 2 * kItems) + 16 + kItems * 64;
+  static constexpr int MAXRING = 10;
+  static constexpr uint32_t BARS = 8 * (2 * kQBufs * NW + 3 * MAXRING + 4 * NW + 2 * kItems) + 16 + kItems * 64;
   static constexpr uint32_t TOTAL = 1024 + DATA + (BARS + 15) / 16 * 16 + (kMaxByKeys + 4) * 4;
   static_assert(TOTAL <= 232448, "shared memory of one CTA");
 };
@@ -132,6 +137,15 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
         "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+__device__ __forceinline__ void tma_store_5d(const CUtensorMap* m, const void* src, int c0, int c1, int c2, int c3, int c4) {
+  asm volatile("cp.async.bulk.tensor.5d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5, %6}], [%1];"
+               ::"l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
+               : "memory");
+}
+// Gives back something that was only read: nothing is published, so no release (which would wait for earlier stores).
+__device__ __forceinline__ void mbar_arrive_relaxed(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   if (BF16) {
@@ -171,7 +185,6 @@ struct Item {
 };
 // The items of one CTA.  Items without rows are left out; those without keys are kept when they are by rows (their
 // outputs are zeros).
-template <int KT>
 struct Items {
   const XattnParams& p;
   const int* ends;  // by keys: key tiles of the requests before and with b, times row blocks and head groups
@@ -239,15 +252,15 @@ struct Items {
 template <bool BF16, int D, bool SHORT>
 __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const __grid_constant__ XattnParams p) {
   using C = XCfg<D, SHORT>;
-  constexpr int NW = C::NW, KT = C::KT;
+  constexpr int NW = C::NW;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int qtiles = p.by_keys ? 1 : p.tpi;        // Q tiles of an item
   uint8_t* sQ = smem;                              // [nq][qtiles]
-  uint8_t* sKV = smem + p.nq * qtiles * C::QTILE;  // [ring]
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + C::DATA);  // [2]
-  uint64_t* q_empty = q_full + 2;                  // [2]
-  uint64_t* kv_full = q_empty + 2;                 // [ring]
+  uint8_t* sKV = smem + p.nq * qtiles * C::TILE;  // [ring]
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + C::DATA);  // [nq][NW] Q tile of group i
+  uint64_t* q_empty = q_full + kQBufs * NW;        // [nq][NW]
+  uint64_t* kv_full = q_empty + kQBufs * NW;       // [ring]
   uint64_t* kv_empty = kv_full + C::MAXRING;       // [ring]
   uint64_t* v_clean = kv_empty + C::MAXRING;       // [ring] V rows of masked keys zeroed
   uint64_t* s_full = v_clean + C::MAXRING;         // [NW] scores ready
@@ -262,17 +275,17 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
   int* ends = reinterpret_cast<int*>(smem + C::DATA + (C::BARS + 15) / 16 * 16);  // [B] by keys
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int svc = warp - 4 * NW;  // service warps: 0 MMA, 1 TMA, 2 clean, 3 items
+  const int svc = warp - C::SW;  // service warps: 0 MMA, 1 TMA, 2 clean, 3 items
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) { mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], 1); }
+    for (int i = 0; i < kQBufs * NW; ++i) { mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], p.by_keys ? C::SW : 4); }
     for (int i = 0; i < p.ring; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); mbar_init(&v_clean[i], 1); }
     for (int i = 0; i < NW; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 128);
+      mbar_init(&p_full[i], 4);
       mbar_init(&o_full[i], 1);
       mbar_init(&o_read[i], 4);
     }
-    for (int i = 0; i < kItems; ++i) { mbar_init(&item_full[i], 1); mbar_init(&item_empty[i], 3 + 4 * NW); }
+    for (int i = 0; i < kItems; ++i) { mbar_init(&item_full[i], 1); mbar_init(&item_empty[i], 3 + C::SW); }
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -309,7 +322,7 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
     return items[ip.s].rows ? &items[ip.s] : nullptr;
   };
   auto done = [&] {
-    mbar_arrive(&item_empty[ip.s]);
+    mbar_arrive_relaxed(&item_empty[ip.s]);
     ip.advance(kItems);
   };
 
@@ -319,27 +332,31 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
       tma_prefetch_desc(&p.tmK);
       tma_prefetch_desc(&p.tmV);
       RingPos kv, q;
-      unsigned nkv = 0, nq = 0;  // copies issued
+      unsigned nkv = 0;                // copies issued
+      unsigned q_used = 0, q_any = 0;  // Q tiles loaded, modulo 2, and at all
       bool ok = true;
       for (const Item* item; ok && (item = next(DEVERR_WAIT_TMA)); done()) {
         const Item w = *item;
         if (w.t0 >= w.t1) continue;
-        if (!(ok = wait_on(&q_empty[q.s], q.ph ^ 1, abort_flag, p.err, DEVERR_WAIT_TMA))) break;
-        const int nt = (w.rows + 127) / 128;
-        mbar_arrive_expect_tx(&q_full[q.s], nt * C::QTILE);
-        for (int i = 0; i < nt; ++i)
+        for (int i = 0; ok && i * 128 < w.rows; ++i) {
+          // a group that earlier items left out is behind: its buffer's phase has a count of its own
+          const int qi = q.s * NW + i;
+          if (!(ok = wait_on(&q_empty[qi], ((q_used >> qi) & 1) ^ 1, abort_flag, p.err, DEVERR_WAIT_TMA))) break;
+          q_used ^= 1u << qi;
+          q_any |= 1u << qi;
+          mbar_arrive_expect_tx(&q_full[qi], C::TILE);
           for (int c = 0; c < D / 64; ++c)
-            tma_load_5d(sQ + (q.s * qtiles + i) * C::QTILE + c * C::QHALF, &p.tmQ, &q_full[q.s], c * 64, 0,
+            tma_load_5d(sQ + (q.s * qtiles + i) * C::TILE + c * C::HALF, &p.tmQ, &q_full[qi], c * 64, 0,
                         (w.row0 + i * 128) >> p.gps, w.hg * p.qh_mul, w.b * p.qb_mul);
+        }
         q.advance(p.nq);
-        ++nq;
         const int hk = (w.hg << p.gps) / p.G;
         for (int t = w.t0; ok && t < w.t1; ++t)
           for (int v = 0; v < 2; ++v) {
             if (!(ok = wait_on(&kv_empty[kv.s], kv.ph ^ 1, abort_flag, p.err, DEVERR_WAIT_TMA))) break;
-            mbar_arrive_expect_tx(&kv_full[kv.s], C::KTILE);
+            mbar_arrive_expect_tx(&kv_full[kv.s], C::TILE);
             for (int c = 0; c < D / 64; ++c)
-              tma_load_4d(sKV + kv.s * C::KTILE + c * C::KHALF, v ? &p.tmV : &p.tmK, &kv_full[kv.s], c * 64, t * KT,
+              tma_load_4d(sKV + kv.s * C::TILE + c * C::HALF, v ? &p.tmV : &p.tmK, &kv_full[kv.s], c * 64, t * KT,
                           hk * (v ? p.vh_mul : p.kh_mul), w.b * (v ? p.vb_mul : p.kb_mul));
             kv.advance(p.ring);
             ++nkv;
@@ -351,10 +368,8 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
           kv.back(p.ring);
           mbar_wait(&kv_full[kv.s], kv.ph, p.err, DEVERR_WAIT_TMA);
         }
-        for (unsigned i = 0; i < min(nq, (unsigned)p.nq); ++i) {
-          q.back(p.nq);
-          mbar_wait(&q_full[q.s], q.ph, p.err, DEVERR_WAIT_TMA);
-        }
+        for (int i = 0; i < kQBufs * NW; ++i)
+          if ((q_any >> i) & 1) mbar_wait(&q_full[i], ((q_used >> i) & 1) ^ 1, p.err, DEVERR_WAIT_TMA);
       }
     }
   } else if (svc == 0) {
@@ -363,12 +378,11 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
       bool ok = true;
       unsigned ph_p = 0, ph_c = 0, ph_r = 0;  // phases of p_full, v_clean, o_read, one bit each
       unsigned used = 0;                      // groups whose O has to be read before new scores (SHORT)
+      unsigned ph_q = 0;                      // phases of q_full
       auto wait = [&](uint64_t* b, int ph) { return wait_on(b, ph, abort_flag, p.err, DEVERR_WAIT_MMA); };
-      for (const Item* item; ok && (item = next(DEVERR_WAIT_MMA)); done()) {
-        const Item w = *item;
-        if (w.t0 >= w.t1) continue;
-        const int nw = (w.rows + 127) / 128, qb = q.s * qtiles;
-        auto issue_s = [&](int i, int qt, int t, int slot) {
+      {
+        auto issue_s = [&](const Item& w, int i, int qt, int t, int slot) {  // qt: Q tile
+
           if (SHORT) {
             if ((used >> i) & 1) {
               ok = wait(&o_read[i], (ph_r >> i) & 1);
@@ -377,18 +391,18 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
             }
             used |= 1u << i;
           }
-          const uint64_t dq = kdesc(smem_u32(sQ + (qb + qt) * C::QTILE)), dk = kdesc(smem_u32(sKV + slot * C::KTILE));
+          const uint64_t dq = kdesc(smem_u32(sQ + qt * C::TILE)), dk = kdesc(smem_u32(sKV + slot * C::TILE));
           // the score tile is as wide as the softmax reads it: 32-key chunks
           const int n = min((w.n - t * KT + 31) / 32, KT / 32) * 32;
           const uint32_t id = idesc_f16(128, 0, BF16) | ((uint32_t)(n >> 3) << 17);
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk)
-            umma_f16(tmem + i * C::TCOLS, dq + ((kk / 4) * C::QHALF + (kk % 4) * 32) / 16,
-                     dk + ((kk / 4) * C::KHALF + (kk % 4) * 32) / 16, id, kk != 0);
+            umma_f16(tmem + i * C::TCOLS, dq + ((kk / 4) * C::HALF + (kk % 4) * 32) / 16,
+                     dk + ((kk / 4) * C::HALF + (kk % 4) * 32) / 16, id, kk != 0);
           umma_commit(&s_full[i]);
         };
-        auto issue_pv = [&](int i, int t, int slot, bool first) {
-          const uint64_t dv = sdesc_sw128(0, C::KHALF, 1024) | (smem_u32(sKV + slot * C::KTILE) >> 4);
+        auto issue_pv = [&](const Item& w, int i, int t, int slot, bool first) {
+          const uint64_t dv = sdesc_sw128(0, C::HALF, 1024) | (smem_u32(sKV + slot * C::TILE) >> 4);
           constexpr uint32_t id = idesc_f16(128, D, BF16, false, true);  // V is MN-major (d contiguous)
           const int steps = min((w.n - t * KT + 15) / 16, KT / 16);
 #pragma unroll
@@ -397,7 +411,7 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
               umma_f16_ta(tmem + i * C::TCOLS + C::TO, tmem + i * C::TCOLS + kk * 8, dv + kk * 2048 / 16, id,
                           !first || kk != 0);
         };
-        auto v_wait = [&](const RingPos& v, int t) {
+        auto v_wait = [&](const Item& w, const RingPos& v, int t) {
           if (!wait(&kv_full[v.s], v.ph)) return false;
           if (cleaned(w, t)) {
             if (!wait(&v_clean[v.s], (ph_c >> v.s) & 1)) return false;
@@ -411,50 +425,109 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
           tc_fence_after();
           return r;
         };
-        ok = wait(&q_full[q.s], q.ph);
-        const int qs = q.s;
-        q.advance(p.nq);
-        if (!p.by_keys) {
-          if (ok && (ok = wait(&kv_full[kv.s], kv.ph))) {
-            tc_fence_after();
-            for (int i = 0; ok && i < nw; ++i) issue_s(i, i, w.t0, kv.s);
-            umma_commit(&kv_empty[kv.s]);
+        auto q_wait = [&](int i) {  // Q tile of group i of the item at q
+          const int qi = q.s * NW + i;
+          const bool r = wait(&q_full[qi], (ph_q >> qi) & 1);
+          ph_q ^= 1u << qi;
+          tc_fence_after();
+          return r;
+        };
+        auto take = [&](Item& w) {  // the next item that has keys
+          const Item* item;
+          while ((item = next(DEVERR_WAIT_MMA)) != nullptr) {
+            w = *item;
+            done();
+            if (w.t0 < w.t1) return true;
           }
-          for (int t = w.t0; ok && t < w.t1; ++t) {  // kv: the K tile of t, then its V tile, then the next K tile
-            const bool more = t + 1 < w.t1;
+          return false;
+        };
+        Item w, w2;
+        if (SHORT) {
+          // kv: the K tile of w, then its V tile, then the K tile of w2
+          bool have = take(w), loaded = false;
+          auto start = [&](const Item& x, int i, const RingPos& k) {  // S of group i of an item
+            if (i * 128 >= x.rows) return;
+            if (!loaded) ok = wait(&kv_full[k.s], k.ph);
+            loaded = true;
+            ok = ok && q_wait(i);
+            if (ok) issue_s(x, i, q.s * qtiles + i, 0, k.s);
+          };
+          if (have) {
+            for (int i = 0; ok && i < NW; ++i) start(w, i, kv);
+            umma_commit(&kv_empty[kv.s]);
+            q.advance(p.nq);
+          }
+          while (ok && have) {
+            const bool more = take(w2);
             const RingPos v = kv.next(p.ring), k2 = v.next(p.ring);
-            ok = v_wait(v, t) && (!more || wait(&kv_full[k2.s], k2.ph));
-            for (int i = 0; ok && i < nw; ++i) {
-              if (!(ok = p_wait(i))) break;
-              issue_pv(i, t, v.s, t == w.t0);
-              if (more) issue_s(i, i, t + 1, k2.s);
-              else umma_commit(&o_full[i]);
+            loaded = false;
+            ok = v_wait(w, v, 0);
+            for (int i = 0; ok && i < NW; ++i) {
+              if (i * 128 < w.rows) {
+                if (!(ok = p_wait(i))) break;
+                issue_pv(w, i, 0, v.s, true);
+                umma_commit(&o_full[i]);
+              }
+              if (more && i > 0) start(w2, i - 1, k2);
             }
             if (!ok) break;
             umma_commit(&kv_empty[v.s]);
-            umma_commit(more ? &kv_empty[k2.s] : &q_empty[qs]);
+            if (more) {
+              start(w2, NW - 1, k2);
+              umma_commit(&kv_empty[k2.s]);
+              q.advance(p.nq);
+            }
             kv = k2;
+            w = w2;
+            have = more;
           }
         } else {
-          // group i takes tiles t0 + i, t0 + i + NW, ...: P V of a tile, then S of the group's next one
-          RingPos v = kv.next(p.ring);  // V tile of `t`; kv: K tile of `t + NW`
-          for (int t = w.t0 - NW; ok && t < w.t1; ++t) {
-            if (t >= w.t0) {
-              const int i = (t - w.t0) % NW;
-              if (!(ok = v_wait(v, t) && p_wait(i))) break;
-              issue_pv(i, t, v.s, t - w.t0 < NW);
-              if (t + NW >= w.t1) umma_commit(&o_full[i]);
-              umma_commit(&kv_empty[v.s]);
-              v = v.next(p.ring).next(p.ring);
+          while (ok && take(w)) {
+            const int nw = (w.rows + 127) / 128, qb = q.s * qtiles;
+            if (!p.by_keys) {
+              if ((ok = wait(&kv_full[kv.s], kv.ph))) {
+                for (int i = 0; ok && i < nw; ++i)
+                  if ((ok = q_wait(i))) issue_s(w, i, qb + i, w.t0, kv.s);
+                umma_commit(&kv_empty[kv.s]);
+              }
+              for (int t = w.t0; ok && t < w.t1; ++t) {  // kv: the K tile of t, then its V tile, then the next K tile
+                const bool more = t + 1 < w.t1;
+                const RingPos v = kv.next(p.ring), k2 = v.next(p.ring);
+                ok = v_wait(w, v, t) && (!more || wait(&kv_full[k2.s], k2.ph));
+                for (int i = 0; ok && i < nw; ++i) {
+                  if (!(ok = p_wait(i))) break;
+                  issue_pv(w, i, t, v.s, t == w.t0);
+                  if (more) issue_s(w, i, qb + i, t + 1, k2.s);
+                  else umma_commit(&o_full[i]);
+                }
+                if (!ok) break;
+                umma_commit(&kv_empty[v.s]);
+                if (more) umma_commit(&kv_empty[k2.s]);
+                kv = k2;
+              }
+            } else {
+              // group i takes tiles t0 + i, t0 + i + NW, ...: P V of a tile, then S of the group's next one
+              ok = q_wait(0);
+              RingPos v = kv.next(p.ring);  // V tile of `t`; kv: K tile of `t + NW`
+              for (int t = w.t0 - NW; ok && t < w.t1; ++t) {
+                if (t >= w.t0) {
+                  const int i = (t - w.t0) % NW;
+                  if (!(ok = v_wait(w, v, t) && p_wait(i))) break;
+                  issue_pv(w, i, t, v.s, t - w.t0 < NW);
+                  if (t + NW >= w.t1) umma_commit(&o_full[i]);
+                  umma_commit(&kv_empty[v.s]);
+                  v = v.next(p.ring).next(p.ring);
+                }
+                if (t + NW < w.t1) {
+                  if (!(ok = wait(&kv_full[kv.s], kv.ph))) break;
+                  tc_fence_after();
+                  issue_s(w, (t + NW - w.t0) % NW, qb, t + NW, kv.s);
+                  umma_commit(&kv_empty[kv.s]);
+                  kv = kv.next(p.ring).next(p.ring);
+                }
+              }
             }
-            if (t + NW < w.t1) {
-              if (!(ok = wait(&kv_full[kv.s], kv.ph))) break;
-              tc_fence_after();
-              issue_s((t + NW - w.t0) % NW, 0, t + NW, kv.s);
-              umma_commit(t + NW == w.t1 - 1 ? &q_empty[qs] : &kv_empty[kv.s]);
-              if (t + NW == w.t1 - 1) umma_commit(&kv_empty[kv.s]);
-              kv = kv.next(p.ring).next(p.ring);
-            }
+            q.advance(p.nq);
           }
         }
       }
@@ -466,7 +539,7 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
     for (const Item* item; ok && (item = next(DEVERR_WAIT_SOFTMAX));) {
       const Item w = *item;
       __syncwarp();
-      if (lane == 0) mbar_arrive(&item_empty[ip.s]);
+      if (lane == 0) mbar_arrive_relaxed(&item_empty[ip.s]);
       ip.advance(kItems);
       for (int t = w.t0; ok && t < w.t1; ++t) {
         // every tile is waited for, cleaned or not: a wait that runs a whole ring ahead would find the phase before it
@@ -486,7 +559,7 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
         }
         ok = __all_sync(0xffffffffu, ok && wait_on(&kv_full[v.s], v.ph, abort_flag, p.err, DEVERR_WAIT_SOFTMAX));
         if (!ok) break;
-        uint4* vt = reinterpret_cast<uint4*>(sKV + v.s * C::KTILE);
+        uint4* vt = reinterpret_cast<uint4*>(sKV + v.s * C::TILE);
 #pragma unroll
         for (int c = 0; c < KT / 32; ++c)
           if (off[c]) {
@@ -494,7 +567,7 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
             for (int k = 0; k < 8; ++k)  // four rows at a time: lane / 8 the row, lane % 8 its 16-byte piece
               if ((off[c] >> (k * 4 + lane / 8)) & 1) {
 #pragma unroll
-                for (int h = 0; h < D / 64; ++h) vt[h * (C::KHALF / 16) + (c * 32 + k * 4) * 8 + lane] = make_uint4(0, 0, 0, 0);
+                for (int h = 0; h < D / 64; ++h) vt[h * (C::HALF / 16) + (c * 32 + k * 4) * 8 + lane] = make_uint4(0, 0, 0, 0);
               }
           }
         fence_async_smem();
@@ -505,7 +578,7 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
     if (!ok) *abort_flag = 1;
   } else if (svc == 3) {
     if (elect_one()) {
-      Items<KT> it(p, ends);
+      Items it(p, ends);
       for (Item w = {}; w.rows >= 0; ip.advance(kItems)) {
         const bool more = it.next(w);
         if (!wait_on(&item_empty[ip.s], ip.ph ^ 1, abort_flag, p.err, DEVERR_WAIT_EPI)) {
@@ -519,21 +592,26 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
       }
     }
   } else {
-    // ---------------- softmax warps: one packed row per thread ----------------
+    // ---------------- softmax warps: one packed row per lane ----------------
     const int i = warp / 4, wq = warp & 3;
     const int lrow = wq * 32 + lane;  // row of the tile = TMEM lane
     const uint32_t tS = tmem + i * C::TCOLS + (static_cast<uint32_t>(wq * 32) << 16), tO = tS + C::TO;
     const int row = p.by_keys ? lrow : i * 128 + lrow;               // row of the item
     const int warp_row = p.by_keys ? wq * 32 : i * 128 + wq * 32;
     const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2);
+    RingPos q;
     int ph_s = 0, ph_o = 0;
     bool ok = true;
     for (const Item* item; ok && (item = next(DEVERR_WAIT_SOFTMAX)) != nullptr;) {
       const Item& w = *item;  // read again where it is used: registers are short here
       const int slot = ip.s;
       ip.advance(kItems);
+      const bool keys = w.t0 < w.t1;  // the item has a Q tile
+      uint8_t* stage = sQ + (q.s * qtiles + (p.by_keys ? 0 : i)) * C::TILE + wq * 4096;
+      uint64_t* q_done = &q_empty[q.s * NW + (p.by_keys ? 0 : i)];
+      if (keys) q.advance(p.nq);
       if (!p.by_keys && i * 128 >= w.rows) {
-        if (lane == 0) mbar_arrive(&item_empty[slot]);
+        if (lane == 0) mbar_arrive_relaxed(&item_empty[slot]);
         continue;
       }
       const bool mine = row < w.rows, warp_on = warp_row < w.rows;
@@ -627,7 +705,8 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
           tmem_wait_st();
         }
         tc_fence_before();
-        mbar_arrive(&p_full[i]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[i]);
       }
       if (ok && any) {
         ok = wait_on(&o_full[i], ph_o, abort_flag, p.err, DEVERR_WAIT_SOFTMAX);
@@ -636,13 +715,15 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
         tc_fence_after();
       }
       if (!ok) break;
-      const long long pr = ((long long)w.slot * NW + i) * 128 + lrow;  // by keys: the row's partial
-      const int tr = w.row0 + row;                                     // packed row of the group
-      const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;
-      const uint64_t inv2 = f2_pack(inv, inv);
-      uint16_t* o = static_cast<uint16_t*>(p.O) + w.b * p.osb + (tr >> p.gps) * p.oss +
-                    ((w.hg << p.gps) + (tr & (p.GP - 1))) * p.osh;
+      bool staged = false;
       if (warp_on) {
+        const long long pr = ((long long)w.slot * NW + i) * 128 + lrow;  // by keys: the row's partial
+        const int tr = w.row0 + row;                                     // packed row of the group
+        const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;
+        const uint64_t inv2 = f2_pack(inv, inv);
+        staged = !p.by_keys && any && warp_row + 32 <= w.rows;
+        uint16_t* o = static_cast<uint16_t*>(p.O) + w.b * p.osb + (tr >> p.gps) * p.oss +
+                      ((w.hg << p.gps) + (tr & (p.GP - 1))) * p.osh;
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t r[32];
@@ -653,7 +734,7 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
           if (SHORT && c == D / 32 - 1) {
             tc_fence_before();
             __syncwarp();
-            if (any && lane == 0) mbar_arrive(&o_read[i]);
+            if (any && lane == 0) mbar_arrive_relaxed(&o_read[i]);
           }
           if (p.by_keys) {
             if (mine && any) {
@@ -663,13 +744,20 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
                 d[k] = make_float4(__uint_as_float(r[4 * k]), __uint_as_float(r[4 * k + 1]),
                                    __uint_as_float(r[4 * k + 2]), __uint_as_float(r[4 * k + 3]));
             }
-          } else if (mine) {
-            uint32_t h[16];
+            continue;
+          }
+          uint32_t h[16];
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {  // no valid key: zeros, whatever O holds
-              const uint64_t x = mul2(f2_pack(__uint_as_float(r[2 * k]), __uint_as_float(r[2 * k + 1])), inv2);
-              h[k] = l_run == 0.f ? 0u : pack2<BF16>(lo_f(x), hi_f(x));
-            }
+          for (int k = 0; k < 16; ++k) {  // no valid key: zeros, whatever O holds
+            const uint64_t x = mul2(f2_pack(__uint_as_float(r[2 * k]), __uint_as_float(r[2 * k + 1])), inv2);
+            h[k] = l_run == 0.f ? 0u : pack2<BF16>(lo_f(x), hi_f(x));
+          }
+          if (staged) {  // 128-byte swizzled rows, 64 columns to a half tile
+            uint4* d = reinterpret_cast<uint4*>(stage + c / 2 * C::HALF + lane * 128);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              d[(c % 2 * 4 + k) ^ (lane & 7)] = make_uint4(h[4 * k], h[4 * k + 1], h[4 * k + 2], h[4 * k + 3]);
+          } else if (mine) {
             if (p.wide) {
 #pragma unroll
               for (int k = 0; k < 2; ++k)
@@ -686,14 +774,30 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
         }
         if (p.by_keys && mine)
           reinterpret_cast<float2*>(p.part + (long long)p.slots * NW * 128 * D)[pr] = make_float2(m_run, l_run);
-        tc_fence_before();  // O is read before the next item's first P V, which waits for this warp's p_full
+        if (staged) {
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            const int tr0 = w.row0 + warp_row;
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c)
+              tma_store_5d(&p.tmO, stage + c * C::HALF, c * 64, tr0 & (p.GP - 1), tr0 >> p.gps, w.hg, w.b);
+            bulk_commit();
+            bulk_wait_read0();
+          }
+        }
       } else if (SHORT && any && lane == 0) {
-        mbar_arrive(&o_read[i]);
+        mbar_arrive_relaxed(&o_read[i]);
       }
+      tc_fence_before();  // O is read before the next item's first P V, which waits for this warp's p_full
       __syncwarp();
-      if (lane == 0) mbar_arrive(&item_empty[slot]);
+      if (lane == 0) {
+        if (keys) mbar_arrive_relaxed(q_done);
+        mbar_arrive_relaxed(&item_empty[slot]);
+      }
     }
     if (!ok) *abort_flag = 1;
+    if (lane == 0) bulk_wait0();
   }
   tc_fence_before();
   __syncthreads();
@@ -706,7 +810,7 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
 // Joins the parts of the keys: one warp per packed row.
 template <bool BF16, int D>
 __global__ void __launch_bounds__(128) xattn_join_kernel(const __grid_constant__ XattnParams p) {
-  constexpr int NW = XCfg<D, false>::NW, KT = XCfg<D, false>::KT;
+  constexpr int NW = XCfg<D, false>::NW;
   pdl_begin();
   const int lane = threadIdx.x & 31;
   const int pair = (int)(blockIdx.y);  // (b, hg, row block)
@@ -780,7 +884,7 @@ struct XPlan {
 };
 XPlan xattn_plan(const Ctx* c, int B, int H, int Hkv, int Sq, int Skv, int D) {
   XPlan x = {};
-  const int G = H / Hkv, NW = D == 64 ? 4 : 2, KT = D == 64 && Skv > 128 ? 64 : 128;
+  const int G = H / Hkv, NW = D == 64 && Skv <= KT ? 3 : 2;
   x.GP = G & -G;  // packed heads: the power of two in the group (tiles of 128 rows hold whole tokens)
   if (x.GP > 128) x.GP = 128;
   x.HG = H / x.GP;
@@ -821,9 +925,9 @@ int launch_xattn(Ctx* c, XattnParams& p) {
     attr_done |= 1u << (c->device & 31);
   }
   const int qtiles = p.by_keys ? 1 : p.tpi;
-  // Q of the next item is fetched under this one; long key sequences leave that for a longer K/V ring (head dim 128)
-  p.nq = D == 64 || qtiles == 1 || p.Skv <= 2 * C::KT ? 2 : 1;
-  p.ring = (int)std::min<uint32_t>(C::MAXRING, (C::DATA - p.nq * qtiles * C::QTILE) / C::KTILE);
+  // Q of the next item is fetched under this one where a ring of four tiles remains
+  p.nq = std::max(1, std::min<int>(SHORT ? kQBufs : 2, (int)(C::DATA / C::TILE - 4) / qtiles));
+  p.ring = (int)std::min<uint32_t>(C::MAXRING, (C::DATA - p.nq * qtiles * C::TILE) / C::TILE);
   const unsigned grid = p.by_keys ? p.grid : std::min<unsigned>(p.items, c->num_sms);
   if (!p.by_keys) {
     p.d_rt = (int)(grid % p.RT);
@@ -849,7 +953,7 @@ extern "C" size_t di_cross_attention_workspace(di_ctx_t h, int B, int H, int Hkv
   if (!h || B <= 0 || H <= 0 || Hkv <= 0 || Sq <= 0 || Skv <= 0 || D <= 0 || H % Hkv) return 0;
   if (D != 64 && D != 128) return 0;
   const XPlan x = xattn_plan(ctx_of(h), B, H, Hkv, Sq, Skv, D);
-  return (size_t)x.slots * (D == 64 ? 4 : 2) * 128 * (D + 2) * 4;
+  return (size_t)x.slots * 2 * 128 * (D + 2) * 4;
 }
 
 extern "C" int di_cross_attention(di_ctx_t h, int dtype, const void* Q, const long long q_strides[3], const void* K,
@@ -898,14 +1002,19 @@ extern "C" int di_cross_attention(di_ctx_t h, int dtype, const void* Q, const lo
   const uint64_t qd[5] = {(uint64_t)D, (uint64_t)x.GP, (uint64_t)Sq, len(qs[2], x.HG), len(qs[0], B)};
   const uint64_t qst[4] = {str(qs[2]), str(qs[1]), str(qs[2] * x.GP), str(qs[0])};
   const uint32_t qbox[5] = {64, (uint32_t)x.GP, (uint32_t)(128 / x.GP), 1, 1};
-  const bool is_short = D == 64 && Skv <= 128;
-  const uint32_t kbox[4] = {64, D == 64 && !is_short ? 64u : 128u, 1, 1};
+  const bool is_short = D == 64 && Skv <= KT;
+  const uint32_t kbox[4] = {64, KT, 1, 1};
   const uint64_t kd[4] = {(uint64_t)D, (uint64_t)Skv, len(ks[2], Hkv), len(ks[0], B)};
   const uint64_t vd[4] = {(uint64_t)D, (uint64_t)Skv, len(vs[2], Hkv), len(vs[0], B)};
   const uint64_t kst[3] = {str(ks[1]), str(ks[2]), str(ks[0])}, vst[3] = {str(vs[1]), str(vs[2]), str(vs[0])};
+  const uint64_t od[5] = {(uint64_t)D, (uint64_t)x.GP, (uint64_t)Sq, (uint64_t)x.HG, (uint64_t)B};
+  const uint64_t ost[4] = {str(os[2]), str(os[1]), str(os[2] * x.GP), str(os[0])};
+  const uint32_t gbox = std::min(x.GP, 32);
+  const uint32_t obox[5] = {64, gbox, 32 / gbox, 1, 1};  // a warp's 32 rows
   if (!make_tmap(&p.tmQ, dt, 5, Q, qd, qst, qbox, CU_TENSOR_MAP_SWIZZLE_128B, &err) ||
       !make_tmap(&p.tmK, dt, 4, K, kd, kst, kbox, CU_TENSOR_MAP_SWIZZLE_128B, &err) ||
-      !make_tmap(&p.tmV, dt, 4, V, vd, vst, kbox, CU_TENSOR_MAP_SWIZZLE_128B, &err))
+      !make_tmap(&p.tmV, dt, 4, V, vd, vst, kbox, CU_TENSOR_MAP_SWIZZLE_128B, &err) ||
+      !make_tmap(&p.tmO, dt, 5, O, od, ost, obox, CU_TENSOR_MAP_SWIZZLE_128B, &err))
     return set_error(c, DI_EINVAL, "cross_attention: " + err);
   p.qh_mul = qs[2] != 0; p.qb_mul = qs[0] != 0;
   p.kh_mul = ks[2] != 0; p.kb_mul = ks[0] != 0;
