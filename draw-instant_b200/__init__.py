@@ -84,12 +84,11 @@ SIGNATURES = {
     "di_gn_table_nhwc": (_I, [_P, _I, _P, _I, _P, _I, _I, _I, _I, _F, _P, _P, _P]),
     "di_conv3x3_nhwc_gn": (_I, [_P, _I, _P, _I, _P, _I, _I, _I, _I, _P, _I, _P, _P, _P, _P, _I, _P]),
     "di_attention": (_I, [_P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I]),
-    "di_linear_lora_workspace": (_SZ, [_P, _I, _I, _I, _I, _I]),
-    "di_linear_lora": (_I, [_P, _I, _P, _LL, _I, _I, _P, _I, _P, _P, _I, _I, _P, _P, _P, _P, _LL, _I, _P, _LL, _P, _SZ]),
-    "di_qk_norm_rope": (_I, [_P, _I, _P, _LL, _I, _P, _LL, _I, _I, _I, _P, _P, _F, _P, _I, _I, _P, ctypes.c_double, _I, _P,
-                             _LL, _P, _LL]),
-    "di_cross_attention_workspace": (_SZ, [_P, _I, _I, _I, _I, _I, _I]),
-    "di_cross_attention": (_I, [_P, _I] + [_P, _P] * 4 + [_I] * 6 + [_P, _P, _P, _F, _P, _SZ]),
+    "di_linear_lora_workspace": (_SZ, [_P, _P]),
+    "di_linear_lora": (_I, [_P, _I] + [_P] * 11 + [_SZ]),
+    "di_qk_norm_rope": (_I, [_P, _I, _P, _F, ctypes.c_double] + [_P] * 7),
+    "di_cross_attention_workspace": (_SZ, [_P, _P]),
+    "di_cross_attention": (_I, [_P, _I, _P, _F] + [_P] * 8 + [_SZ]),
     "di_tembed": (_I, [_P, _P, _I, _P, _P, _P, _P, _I, _I, _P]),
     "di_synth_uniform": (None, [ctypes.c_uint64, ctypes.c_char_p, _SZ, _F, _P]),
     "di_synth_normal": (None, [ctypes.c_uint64, ctypes.c_char_p, _SZ, _F, _F, _P]),

@@ -23,7 +23,7 @@
 //   warps 4-15   epilogue: bias, activation, residual (fetched by TMA during the main loop), stores by TMA
 // The accumulator is double-buffered, so a tile's epilogue runs under the next one's main loop.
 //
-// Few rows (M <= kSkinnyRows): T in 32 bits; the second launch streams W once from memory into mma.sync fragments (16
+// Few rows (M <= kSkinnyRows): T in 32 bits (in shared memory, with no first launch, where that is less work); the second launch streams W once from memory into mma.sync fragments (16
 // weight rows by 8 rows of X) and adds the rows' own B products with plain FMAs: every byte of W, A and B is
 // read about once, whoever owns it.
 #include <algorithm>
@@ -827,6 +827,25 @@ __global__ void __launch_bounds__(kLThreads, 1) lora_tile_kernel(const __grid_co
 
 // ---- few rows ----
 
+// x . w over K values by one warp; every lane returns it.
+template <bool BF16>
+__device__ __forceinline__ float dot_k(const uint16_t* x, const uint16_t* w, int K, int lane) {
+  float s = 0.f;
+#pragma unroll 4
+  for (int k = lane * 8; k < K; k += 256) {
+    const uint4 u = __ldg(reinterpret_cast<const uint4*>(x + k)), v = __ldg(reinterpret_cast<const uint4*>(w + k));
+    const uint32_t uu[4] = {u.x, u.y, u.z, u.w}, vv[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = unpack2<BF16>(uu[e]), g = unpack2<BF16>(vv[e]);
+      s = fmaf(f.x, g.x, fmaf(f.y, g.y, s));
+    }
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
+
 // T[m][j] = scale[a] * X[m] . A[a][j]: one warp per value, eight of one row to a block.
 template <bool BF16>
 __global__ void __launch_bounds__(256) lora_shrink_kernel(const __grid_constant__ LoraParams p) {
@@ -838,111 +857,174 @@ __global__ void __launch_bounds__(256) lora_shrink_kernel(const __grid_constant_
     a = -1;
   }
   if (a < 0) return;  // nothing reads this row of T
-  const uint16_t* x = static_cast<const uint16_t*>(p.X) + m * p.ldx;
-  const uint16_t* w = static_cast<const uint16_t*>(p.A) + ((long long)a * p.r + j) * p.K;
-  float s = 0.f;
-#pragma unroll 4
-  for (int k = lane * 8; k < p.K; k += 256) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(x + k)), v = __ldg(reinterpret_cast<const uint4*>(w + k));
-    const uint32_t uu[4] = {u.x, u.y, u.z, u.w}, vv[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 f = unpack2<BF16>(uu[e]), g = unpack2<BF16>(vv[e]);
-      s = fmaf(f.x, g.x, fmaf(f.y, g.y, s));
-    }
-  }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  const float s = dot_k<BF16>(static_cast<const uint16_t*>(p.X) + m * p.ldx,
+                              static_cast<const uint16_t*>(p.A) + ((long long)a * p.r + j) * p.K, p.K, lane);
   if (lane == 0) p.T[m * p.r + j] = __ldg(p.scale + a) * s;
 }
 
-// 16 columns of Y for MT * 8 rows per block; the 8 warps take 32-wide K blocks in turn and are summed in shared memory.
-// A lane's 16-byte loads of 8 consecutive k stand for two 16-wide MMA steps: both operands use the same order of k.
-template <bool BF16, int MT>
-__global__ void __launch_bounds__(256) lora_skinny_kernel(const __grid_constant__ LoraParams p) {
-  __shared__ float red[8][MT * 8][17];
+// 16 columns of Y for 8 MT rows per block.  The 8 warps are KW shares of K (32-wide blocks in turn) by 8 / KW groups of
+// rows, summed in shared memory.  A lane's 16-byte loads of 8 consecutive k stand for two 16-wide MMA steps: both
+// operands use the same order of k.  Bound: the bytes of W and B, and from L2 those of X, which every block reads whole.
+// CLUSTER: no first launch; the eight blocks of a cluster share out the values of T, which eight more warps of each compute
+// and hand to all through distributed shared memory while the MMAs run.
+template <bool BF16, int MT, bool CLUSTER>
+__global__ void __launch_bounds__(CLUSTER ? 512 : 256) lora_skinny_kernel(const __grid_constant__ LoraParams p) {
+  constexpr int KW = MT == 8 ? 4 : 8, RT = MT * KW / 8;  // row tiles per warp
+  constexpr int ROWS = 8 * MT, COLS = 16, AHEAD = 4;
+  __shared__ float red[KW][ROWS][COLS + 1];
+  __shared__ __align__(16) float ts[ROWS * (MT == 8 ? 40 : 128)];  // T of the rows, up to that rank
+  __shared__ int as[ROWS];                                         // their adapters
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * MT * 8;
-  // The shrink kernel lets this one start after its own wait for earlier kernels: X, W and B may be read at once,
-  // T, R and Y only after it.
+  const int n0 = blockIdx.x * COLS, m0 = blockIdx.y * ROWS;
+  constexpr int THREADS = CLUSTER ? 512 : 256;
+  if (CLUSTER) {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // 1: this block has started
+    pdl_wait();
+  }
+  // The shrink kernel lets this one start after its own wait for earlier kernels: X, W, B and the indices may be read at
+  // once, T, R and Y only after it.
   pdl_trigger();
-  float acc[MT][4] = {};
-  const uint16_t* w0 = static_cast<const uint16_t*>(p.W) + (long long)(n0 + lane / 4) * p.K + (lane & 3) * 8;
-  const uint16_t* w1 = w0 + 8ll * p.K;
-  const uint16_t* x0 = static_cast<const uint16_t*>(p.X) + (lane & 3) * 8;
-#pragma unroll 4
-  for (int k = warp * 32; k < p.K; k += 256) {
-    const uint4 a0 = __ldg(reinterpret_cast<const uint4*>(w0 + k)), a1 = __ldg(reinterpret_cast<const uint4*>(w1 + k));
-    uint4 b[MT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      const int m = min(m0 + t * 8 + lane / 4, p.M - 1);  // rows past the last are computed and not stored
-      b[t] = __ldg(reinterpret_cast<const uint4*>(x0 + m * p.ldx + k));
+  for (int i = threadIdx.x; i < ROWS; i += THREADS) {
+    int a = m0 + i < p.M ? __ldg(p.rows + m0 + i) : -1;
+    if (a >= p.L) {
+      if (CLUSTER && blockIdx.x == 0) atomicOr(p.err, DEVERR_BOUNDS);
+      a = -1;
     }
+    as[i] = a;
+  }
+  if (CLUSTER && warp >= 8) {
+    const int n = min(ROWS, p.M - m0) * p.r;
+    bool waited = false;
+    for (int v = (int)cluster_ctarank() + 8 * (warp - 8); v < n; v += 64) {
+      const int m = v / p.r, a = __ldg(p.rows + m0 + m);
+      float s = 0.f;
+      if (a >= 0 && a < p.L)
+        s = __ldg(p.scale + a) * dot_k<BF16>(static_cast<const uint16_t*>(p.X) + (m0 + m) * p.ldx,
+                                             static_cast<const uint16_t*>(p.A) + ((long long)a * p.r + v % p.r) * p.K, p.K, lane);
+      if (!waited) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // 1: all eight have started
+      waited = true;
+      if (lane < 8)
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(smem_u32(ts + v), lane)), "f"(s) : "memory");
+    }
+    if (!waited) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  } else {
+  const int kw = warp % KW, rw = warp / KW * RT * 8;
+  float acc[RT][4] = {};
+  const uint16_t* wp[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    wp[i] = static_cast<const uint16_t*>(p.W) + (long long)min(n0 + i * 8 + lane / 4, p.N - 1) * p.K + (lane & 3) * 8;
+  const uint16_t* xp[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t)  // rows and columns past the last are computed and not stored
+    xp[t] = static_cast<const uint16_t*>(p.X) + min(m0 + rw + t * 8 + lane / 4, p.M - 1) * p.ldx + (lane & 3) * 8;
+#pragma unroll 4
+  for (int k = kw * 32; k < p.K; k += KW * 32) {
+    const uint4 a0 = __ldg(reinterpret_cast<const uint4*>(wp[0] + k)), a1 = __ldg(reinterpret_cast<const uint4*>(wp[1] + k));
+    uint4 b[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) b[t] = __ldg(reinterpret_cast<const uint4*>(xp[t] + k));
     const uint32_t f0[4] = {a0.x, a1.x, a0.y, a1.y}, f1[4] = {a0.z, a1.z, a0.w, a1.w};
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
+    for (int t = 0; t < RT; ++t) {
       mma_16x8x16<BF16>(acc[t], f0, b[t].x, b[t].y);
       mma_16x8x16<BF16>(acc[t], f1, b[t].z, b[t].w);
     }
   }
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {  // d[0..1]: column lane / 4, rows 2 (lane & 3) + {0, 1}; d[2..3]: column + 8
-    const int m = t * 8 + (lane & 3) * 2, n = lane / 4;
-    red[warp][m][n] = acc[t][0];
-    red[warp][m + 1][n] = acc[t][1];
-    red[warp][m][n + 8] = acc[t][2];
-    red[warp][m + 1][n + 8] = acc[t][3];
+  for (int t = 0; t < RT; ++t) {  // d[0..1]: column lane / 4, rows 2 (lane & 3) + {0, 1}; d[2..3]: column + 8
+    const int m = rw + t * 8 + (lane & 3) * 2, n = lane / 4;
+    red[kw][m][n] = acc[t][0];
+    red[kw][m + 1][n] = acc[t][1];
+    red[kw][m][n + 8] = acc[t][2];
+    red[kw][m + 1][n + 8] = acc[t][3];
   }
+  if (CLUSTER) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // 1
+  }
+  if (CLUSTER) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // 2: this warp's values of T are written
   __syncthreads();
-  pdl_wait();  // T is complete
-  // outputs: groups of 2^g lanes share one output's rank chunks of 8
-  int g = 0;
-  while ((8 << g) < p.r) ++g;
-  const int per = 256 >> g, sub = threadIdx.x & ((1 << g) - 1);
-  for (int o = threadIdx.x >> g; o < (MT * 128 + per - 1) / per * per; o += per) {  // whole warps stay for the shuffles
-    const int n = o & 15, ml = o >> 4, m = m0 + ml;
-    const bool on = ml < MT * 8 && m < p.M;
-    int a = on ? __ldg(p.rows + m) : -1;
-    if (a >= p.L) a = -1;
-    float s = 0.f;
-    if (a >= 0 && sub * 8 < p.r) {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.B) +
-                                                           ((long long)a * p.N + n0 + n) * p.r + sub * 8));
-      const float* t = p.T + m * p.r + sub * 8;
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  // One output per thread at a time, neighbours in a row: its B row in 16-byte pieces, the first AHEAD of the next output's
+  // already on their way.
+  constexpr int total = ROWS * COLS;
+  uint4 u[AHEAD];
+  auto b_row = [&](int o) -> const uint4* {  // null: no adapter, or outside Y
+    const int n = n0 + o % COLS, a = o < total ? as[o / COLS] : -1;
+    return a >= 0 && n < p.N ? reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.B) + ((long long)a * p.N + n) * p.r)
+                             : nullptr;
+  };
+  auto fetch = [&](const uint4* row) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 f = unpack2<BF16>(w[e]);
-        s = fmaf(t[2 * e], f.x, fmaf(t[2 * e + 1], f.y, s));
-      }
+    for (int i = 0; i < AHEAD; ++i) u[i] = row && i * 8 < p.r ? __ldg(row + i) : make_uint4(0, 0, 0, 0);
+  };
+  const uint4* row = b_row(threadIdx.x);
+  fetch(row);
+  const bool shared_t = CLUSTER || ROWS * p.r <= (int)(sizeof ts / 4);
+  if (CLUSTER) {
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  } else {
+    pdl_wait();  // T is complete
+  }
+  if (!CLUSTER && shared_t) {
+    for (int i = threadIdx.x; i < ROWS * p.r; i += THREADS) ts[i] = m0 * p.r + i < p.M * p.r ? p.T[(long long)m0 * p.r + i] : 0.f;
+    __syncthreads();
+  }
+  for (int o = threadIdx.x; o < total; o += THREADS) {
+    const int ml = o / COLS, n = n0 + o % COLS, m = m0 + ml;
+    const float4* t = reinterpret_cast<const float4*>(shared_t ? ts + ml * p.r : p.T + (long long)m * p.r);
+    float s = 0.f, s2 = 0.f;
+    auto dot = [&](const uint4& v, const float4* t) {
+      const float4 ta = t[0], tb = t[1];
+      const float2 f0 = unpack2<BF16>(v.x), f1 = unpack2<BF16>(v.y), f2 = unpack2<BF16>(v.z), f3 = unpack2<BF16>(v.w);
+      s = fmaf(ta.x, f0.x, fmaf(ta.y, f0.y, fmaf(ta.z, f1.x, fmaf(ta.w, f1.y, s))));
+      s2 = fmaf(tb.x, f2.x, fmaf(tb.y, f2.y, fmaf(tb.z, f3.x, fmaf(tb.w, f3.y, s2))));
+    };
+    uint4 now[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) now[i] = u[i];
+    const uint4* mine = row;
+    row = b_row(o + THREADS);
+    fetch(row);
+    if (mine) {
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i)
+        if (i * 8 < p.r) dot(now[i], t + 2 * i);
+      for (int i = AHEAD; i * 8 < p.r; ++i) dot(__ldg(mine + i), t + 2 * i);
     }
-    for (int x = 1; x < (1 << g); x <<= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    if (on && sub == 0) {
+    if (m < p.M && n < p.N) {
 #pragma unroll
-      for (int x = 0; x < 8; ++x) s += red[x][ml][n];
-      if (p.bias) s += __ldg(p.bias + n0 + n);
+      for (int x = 0; x < KW; ++x) s += red[x][ml][o % COLS];
+      s += s2;
+      if (p.bias) s += __ldg(p.bias + n);
       s = act_of(s, p.act);
-      if (p.R) {
-        const uint16_t v = static_cast<const uint16_t*>(p.R)[m * p.ldr + n0 + n];
-        s += unpack2<BF16>(v).x;
-      }
-      static_cast<uint16_t*>(p.Y)[m * p.ldy + n0 + n] = (uint16_t)pack2<BF16>(s, 0.f);
+      if (p.R) s += unpack2<BF16>(static_cast<const uint16_t*>(p.R)[m * p.ldr + n]).x;
+      static_cast<uint16_t*>(p.Y)[m * p.ldy + n] = (uint16_t)pack2<BF16>(s, 0.f);
     }
   }
 }
 
+// Whether few rows run in one launch: each cluster of eight blocks (128 columns) reads the rows' adapters itself, which
+// has to stay small next to a launch (2 us against the L2 traffic of 16 MB).
+bool one_launch(long long M, long long N, long long K, long long r) {
+  return M <= 32 && M * r * K * 2 * ((N + 127) / 128) <= (16 << 20);
+}
+
 template <bool BF16>
 int launch_skinny(Ctx* c, const LoraParams& p) {
+  const int tiles = (p.M + 7) / 8;
+  if (one_launch(p.M, p.N, p.K, p.r)) {
+    const dim3 grid((p.N + 127) / 128 * 8);
+    auto kern = tiles == 1 ? lora_skinny_kernel<BF16, 1, true> : tiles == 2 ? lora_skinny_kernel<BF16, 2, true> : lora_skinny_kernel<BF16, 4, true>;
+    launch_k_cluster(kern, grid, 512, 0, c->stream, 8, p);
+    return check_launch(c, "linear_lora");
+  }
   launch_k(lora_shrink_kernel<BF16>, dim3(p.r / 8, p.M), 256, 0, c->stream, p);
   const int rc = check_launch(c, "linear_lora");
   if (rc != DI_OK) return rc;
-  const int tiles = (p.M + 7) / 8;
   auto go = [&](auto kern, int mt) { launch_k(kern, dim3(p.N / 16, (tiles + mt - 1) / mt), 256, 0, c->stream, p); };
-  if (tiles == 1) go(lora_skinny_kernel<BF16, 1>, 1);
-  else if (tiles == 2) go(lora_skinny_kernel<BF16, 2>, 2);
-  else if (tiles <= 4) go(lora_skinny_kernel<BF16, 4>, 4);
-  else go(lora_skinny_kernel<BF16, 8>, 8);
+  if (tiles == 1) go(lora_skinny_kernel<BF16, 1, false>, 1);
+  else if (tiles == 2) go(lora_skinny_kernel<BF16, 2, false>, 2);
+  else if (tiles <= 4) go(lora_skinny_kernel<BF16, 4, false>, 4);
+  else go(lora_skinny_kernel<BF16, 8, false>, 8);
   return check_launch(c, "linear_lora");
 }
 
@@ -1048,21 +1130,32 @@ int launch_tiles(Ctx* c, LoraParams& p) {
 
 using namespace di;
 
-extern "C" size_t di_linear_lora_workspace(di_ctx_t h, int M, int N, int K, int rank, int n_adapters) {
-  if (!h || M <= 0 || rank <= 0) return 0;
-  if (M <= kSkinnyRows) return (size_t)M * rank * 4;
-  return (size_t)M * (rank <= 32 ? 64 : (rank + 63) / 64 * 128) * 2;
+namespace {
+bool fits_int(const long long* v, int n) {
+  for (int i = 0; i < n; ++i)
+    if (v[i] < 0 || v[i] > (1ll << 30)) return false;
+  return true;
+}
+}  // namespace
+
+extern "C" size_t di_linear_lora_workspace(di_ctx_t h, const long long cfg[9]) {
+  if (!h || !cfg || !fits_int(cfg, 5)) return 0;
+  const size_t M = cfg[0], rank = cfg[3];
+  if (M <= (size_t)kSkinnyRows) return one_launch(cfg[0], cfg[1], cfg[2], cfg[3]) ? 0 : M * rank * 4;
+  return M * (rank <= 32 ? 64 : (rank + 63) / 64 * 128) * 2;
 }
 
-extern "C" int di_linear_lora(di_ctx_t h, int dtype, const void* X, long long ldx, int M, int K, const void* W, int N,
-                              const void* A, const void* B, int rank, int n_adapters, const float* scale,
-                              const int* row_adapter, const float* bias, const void* R, long long ldr, int act, void* Y,
-                              long long ldy, void* ws, size_t ws_bytes) {
+extern "C" int di_linear_lora(di_ctx_t h, int dtype, const long long cfg[9], const void* X, const void* W, const void* A,
+                              const void* B, const float* scale, const int* row_adapter, const float* bias, const void* R,
+                              void* Y, void* ws, size_t ws_bytes) {
   Ctx* c = ctx_of(h);
   if (!c || (dtype != DI_F16 && dtype != DI_BF16)) return DI_EINVAL;
   DeviceGuard guard(c->device);
-  if (M <= 0 || N <= 0 || K <= 0 || n_adapters <= 0 || !X || !W || !A || !B || !scale || !row_adapter || !Y)
+  if (!cfg || !fits_int(cfg, 5) || !X || !W || !A || !B || !scale || !row_adapter || !Y)
     return set_error(c, DI_EINVAL, "linear_lora: bad shape or missing tensor");
+  const int M = (int)cfg[0], N = (int)cfg[1], K = (int)cfg[2], rank = (int)cfg[3], L = (int)cfg[4];
+  const long long ldx = cfg[5], ldr = cfg[6], ldy = cfg[7], act = cfg[8];
+  if (M <= 0 || N <= 0 || K <= 0 || L <= 0) return set_error(c, DI_EINVAL, "linear_lora: bad shape or missing tensor");
   if (K % 64 || N % 16) return set_error(c, DI_EUNSUPPORTED, "linear_lora: K must be a multiple of 64, N of 16");
   if (rank < 8 || rank > 128 || rank % 8)
     return set_error(c, DI_EUNSUPPORTED, "linear_lora: the rank must be a multiple of 8, 8 to 128");
@@ -1071,17 +1164,17 @@ extern "C" int di_linear_lora(di_ctx_t h, int dtype, const void* X, long long ld
   if (!aligned16(X) || !aligned16(W) || !aligned16(A) || !aligned16(B) || !aligned16(R) || !aligned16(Y) || ldx % 8 ||
       ldy % 8 || (R && ldr % 8))
     return set_error(c, DI_EINVAL, "linear_lora: pointers must be 16-byte aligned, row strides multiples of 8 elements");
-  if (M > (1 << 30) || N > (1 << 30) || (M + 127LL) / 128 * ((N + 31) / 32) > 0x7fffffffll)
+  if ((M + 127LL) / 128 * ((N + 31) / 32) > 0x7fffffffll)
     return set_error(c, DI_EUNSUPPORTED, "linear_lora: too many rows and columns");
-  const size_t need = di_linear_lora_workspace(h, M, N, K, rank, n_adapters);
+  const size_t need = di_linear_lora_workspace(h, cfg);
   if (need && (!ws || ws_bytes < need || !aligned16(ws)))
     return set_error(c, DI_EINVAL, "linear_lora: workspace missing, too small or not 16-byte aligned");
   LoraParams p;
   memset(&p, 0, sizeof p);
   p.X = X; p.W = W; p.A = A; p.B = B; p.R = R; p.Y = Y;
   p.ldx = ldx; p.ldr = ldr; p.ldy = ldy;
-  p.M = M; p.N = N; p.K = K; p.r = rank; p.L = n_adapters;
-  p.scale = scale; p.bias = bias; p.rows = row_adapter; p.act = act;
+  p.M = M; p.N = N; p.K = K; p.r = rank; p.L = L;
+  p.scale = scale; p.bias = bias; p.rows = row_adapter; p.act = (int)act;
   p.err = c->d_err;
   p.T = static_cast<float*>(ws);
   p.T16 = static_cast<uint16_t*>(ws);

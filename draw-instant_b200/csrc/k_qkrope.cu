@@ -6,11 +6,13 @@
 // (sum d_a = D) and pair j of axis a turns by pos[token][a] * theta^(-2j / d_a) radians.  A pair is two
 // neighbouring values (interleaved) or values i and i + D/2 (halves).
 //
-// Bound: HBM, every value read and written once.  One warp takes one token at a time: a lane owns the same
-// 8-value chunk of every head it meets, so the token's angles (one sine and cosine per pair, taken once per
-// token for all its heads) and the weights stay in its registers, and all traffic is 16-byte accesses.
-// The angle is the product of an integer position and a 64-bit frequency in turns, reduced to half a turn in 64
-// bits before the 32-bit sine: positions of any size keep the accuracy of position zero.
+// Bound: HBM, every value read and written once; at 23 bytes a cycle and SM that leaves some 170 instructions for the
+// 1 KB that a warp reads and writes per step, so the arithmetic is packed (two values per instruction) and the
+// angles are taken once per token for all its heads.  A warp takes four tokens (two at D = 128) side by side and walks their
+// heads, queries then keys: a lane owns the same 8-value chunk of every head of one token, with the weights times the
+// sines and cosines of its pairs in registers, and all traffic is whole 128-byte lines.  Loads run four steps ahead.
+// The angle is the product of an integer position and a 64-bit frequency in turns, reduced to half a turn in 64 bits
+// before the 32-bit sine (absolute error 2^-20.9): positions of any size keep the accuracy of position zero.
 // Sums and products are 32-bit; the result is rounded once.
 #include <algorithm>
 #include <cmath>
@@ -36,147 +38,194 @@ struct QkParams {
   const int* pos;         // null: no rotation
   float eps;
   int hsplit;             // warps that share a token's heads
-  int tokens;             // tokens per warp
   double freq[kMaxPairs];           // turns per position step
   unsigned char axis[kMaxPairs];
 };
 
-constexpr int kQkWarps = 4, kQkTokens = 4, kQkUnroll = 4;  // warps per block, most tokens per warp, chunks in flight
+constexpr int kQkWarps = 4, kQkAhead = 4;  // warps per block, steps in flight
 
-template <typename T>
-__device__ __forceinline__ void unpack8(const uint4& u, float (&f)[8]) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t v = w[i];
-    float2 t;
-    if (std::is_same<T, __half>::value) t = __half22float2(*reinterpret_cast<__half2*>(&v));
-    else t = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v));
-    f[2 * i] = t.x;
-    f[2 * i + 1] = t.y;
-  }
+__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
+  return (uint64_t)__float_as_uint(a) | ((uint64_t)__float_as_uint(b) << 32);
+}
+__device__ __forceinline__ float lo_f(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float hi_f(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
 }
 template <typename T>
-__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (std::is_same<T, __half>::value) {
-      __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-      w[i] = *reinterpret_cast<uint32_t*>(&h);
-    } else {
-      __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-      w[i] = *reinterpret_cast<uint32_t*>(&h);
-    }
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<__half2*>(&w));
+  return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&w));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if (std::is_same<T, __half>::value) {
+    __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
   }
-  return make_uint4(w[0], w[1], w[2], w[3]);
+  __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&h);
 }
 
 template <typename T, int D, bool HALVES>
-__global__ void __launch_bounds__(32 * kQkWarps) qk_norm_rope_kernel(const __grid_constant__ QkParams p) {
-  constexpr int LPH = D / 8;        // lanes per head
-  constexpr int HPW = 32 / LPH;     // heads per warp step
-  constexpr int PPL = D / 64;       // pairs whose angle a lane computes
-  constexpr int NP = HALVES ? 8 : 4;  // pairs that a lane's chunk meets
-  const int lane = threadIdx.x & 31;
-  const long long warp = (long long)blockIdx.x * kQkWarps + (threadIdx.x >> 5);
-  const int part = (int)(warp % p.hsplit);
-  const long long t0 = warp / p.hsplit * p.tokens;
-  const int chunk = lane % LPH, sub = lane / LPH;
-  double fr[PPL];
-  int ax[PPL];
-#pragma unroll
-  for (int i = 0; i < PPL; ++i) {
-    fr[i] = p.freq[lane + 32 * i];
-    ax[i] = p.axis[lane + 32 * i];
+__global__ void __launch_bounds__(32 * kQkWarps, 5) qk_norm_rope_kernel(const __grid_constant__ QkParams p) {
+  constexpr int LPH = D / 8;   // lanes per head
+  constexpr int TPW = 32 / LPH;  // tokens per warp
+  const int lane = threadIdx.x & 31, chunk = lane % LPH;
+  const int heads = p.H[0] + p.H[1];
+  unsigned group = blockIdx.x * kQkWarps + (threadIdx.x >> 5);
+  int h0 = 0, h1 = heads;
+  if (p.hsplit > 1) {  // divisions are dear next to a warp's work: 32 bits, and only where they are needed
+    const unsigned part = group % p.hsplit;
+    group /= p.hsplit;
+    h0 = (int)((unsigned)heads * part / p.hsplit);
+    h1 = (int)((unsigned)heads * (part + 1) / p.hsplit);
   }
+  const long long t = (long long)group * TPW + lane / LPH;
+  const bool on = t < p.T;
+  // A lane's 8 values are 4 pairs (interleaved), or one value each of 8 pairs whose other values lie LPH / 2 lanes on
+  // (halves); it takes the angles of 4 pairs, in the halves' case 4 of the 8 and the other lane the rest.
+  const int pair0 = HALVES ? chunk % (LPH / 2) * 8 + chunk / (LPH / 2) * 4 : chunk * 4;
   pdl_begin();
-  float wq[8], wk[8];
+  // This warp's query heads and key heads, each list padded to whole blocks of kQkAhead steps: step v of the two lists
+  // laid end to end uses buffer v % kQkAhead.
+  const int q0 = min(h0, p.H[0]), nq = min(h1, p.H[0]) - q0, k0 = max(h0 - p.H[0], 0), nk = max(h1 - p.H[0], 0) - k0;
+  const int qpad = (nq + kQkAhead - 1) / kQkAhead * kQkAhead, steps = qpad + nk;
+  const long long tt = on ? t : 0;
+  const T* xq = static_cast<const T*>(p.x[0]) + tt * p.ldx[0] + (long long)q0 * D + chunk * 8;
+  const T* xk = static_cast<const T*>(p.x[1]) + tt * p.ldx[1] + (long long)(k0 - qpad) * D + chunk * 8;
+  T* yq = static_cast<T*>(p.y[0]) + tt * p.ldy[0] + (long long)q0 * D + chunk * 8;
+  T* yk = static_cast<T*>(p.y[1]) + tt * p.ldy[1] + (long long)(k0 - qpad) * D + chunk * 8;
+  uint4 raw[kQkAhead];
+  auto fetch = [&](uint4& r, int v) {
+    if (on && (v < nq || (v >= qpad && v < steps))) r = *reinterpret_cast<const uint4*>((v < qpad ? xq : xk) + (long long)v * D);
+  };
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    wq[e] = p.w[0] ? __ldg(p.w[0] + chunk * 8 + e) : 1.f;
-    wk[e] = p.w[1] ? __ldg(p.w[1] + chunk * 8 + e) : 1.f;
-  }
-  const int heads = p.H[0] + p.H[1], steps = (heads + HPW - 1) / HPW;
-  const int s0 = (int)((long long)steps * part / p.hsplit), s1 = (int)((long long)steps * (part + 1) / p.hsplit);
-  for (long long t = t0; t < min(t0 + p.tokens, p.T); ++t) {
-    float c[NP], s[NP];
-    if (p.pos) {
-      float cl[PPL], sl[PPL];
+  for (int u = 0; u < kQkAhead; ++u) fetch(raw[u], u);
+  float co[HALVES ? 8 : 4], si[HALVES ? 8 : 4];
+  if (p.pos) {
+    const int* row = p.pos + (long long)(on ? (unsigned)t % (unsigned)p.P : 0u) * p.axes;
+    float c4[4], s4[4];
 #pragma unroll
-      for (int i = 0; i < PPL; ++i) {
-        const double turns = (double)__ldg(p.pos + (t % p.P) * p.axes + ax[i]) * fr[i];
-        sincospif(2.0f * (float)(turns - rint(turns)), &sl[i], &cl[i]);
+    for (int i = 0; i < 4; ++i) {
+      const double turns = (double)__ldg(row + p.axis[pair0 + i]) * p.freq[pair0 + i];
+      __sincosf(6.283185307f * (float)(turns - rint(turns)), &s4[i], &c4[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (HALVES) {
+        const float oc = __shfl_xor_sync(0xffffffffu, c4[i], LPH / 2), os = __shfl_xor_sync(0xffffffffu, s4[i], LPH / 2);
+        const bool low = chunk < LPH / 2;
+        co[i % (HALVES ? 8 : 4)] = low ? c4[i] : oc;
+        si[i % (HALVES ? 8 : 4)] = low ? s4[i] : os;
+        co[(i + 4) % (HALVES ? 8 : 4)] = low ? oc : c4[i];
+        si[(i + 4) % (HALVES ? 8 : 4)] = low ? os : s4[i];
+      } else {
+        co[i] = c4[i];
+        si[i] = s4[i];
       }
+    }
+  } else {
 #pragma unroll
-      for (int e = 0; e < NP; ++e) {
-        // pair of this chunk's e-th value (halves) or value pair (interleaved), held by lane pair % 32
-        const int pair = HALVES ? (chunk * 8 + e) % (D / 2) : chunk * 4 + e;
-        c[e] = __shfl_sync(0xffffffffu, cl[0], pair & 31);
-        s[e] = __shfl_sync(0xffffffffu, sl[0], pair & 31);
-        if (PPL == 2) {
-          const float c1 = __shfl_sync(0xffffffffu, cl[PPL - 1], pair & 31);
-          const float s1v = __shfl_sync(0xffffffffu, sl[PPL - 1], pair & 31);
-          if (pair >= 32) { c[e] = c1; s[e] = s1v; }
+    for (int i = 0; i < (HALVES ? 8 : 4); ++i) { co[i] = 1.f; si[i] = 0.f; }
+  }
+  // Values two and two: interleaved, the first and the second values of pairs 2 j and 2 j + 1; halves, values 2 j and 2 j + 1.
+  // With the weights folded in: first' = first * m1 + second * m2, second' = first * m3 + second * m4 (halves: own value
+  // and other value times m1 and m2).
+  uint64_t m1[HALVES ? 4 : 2], m2[HALVES ? 4 : 2], m3[2], m4[2];
+  bool norm = false;
+  for (int v = 0; v < steps; v += kQkAhead) {
+    if (v == 0 || v == qpad) {  // on to the queries, or the keys
+      const float* wp = v < qpad ? p.w[0] : p.w[1];
+      norm = wp != nullptr;
+      float w[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = wp ? __ldg(wp + chunk * 8 + e) : 1.f;
+#pragma unroll
+      for (int j = 0; j < (HALVES ? 4 : 2); ++j) {
+        if (HALVES) {
+          const float sign = chunk < LPH / 2 ? -1.f : 1.f;
+          const float o0 = __shfl_xor_sync(0xffffffffu, w[2 * j], LPH / 2), o1 = __shfl_xor_sync(0xffffffffu, w[2 * j + 1], LPH / 2);
+          m1[j] = f2_pack(w[2 * j] * co[2 * j], w[2 * j + 1] * co[2 * j + 1]);
+          m2[j] = f2_pack(sign * o0 * si[2 * j], sign * o1 * si[2 * j + 1]);
+        } else {
+          const float c0 = co[2 * j], c1 = co[2 * j + 1], s0 = si[2 * j], s1 = si[2 * j + 1];
+          m1[j] = f2_pack(w[4 * j] * c0, w[4 * j + 2] * c1);
+          m2[j] = f2_pack(-w[4 * j + 1] * s0, -w[4 * j + 3] * s1);
+          m3[j] = f2_pack(w[4 * j] * s0, w[4 * j + 2] * s1);
+          m4[j] = f2_pack(w[4 * j + 1] * c0, w[4 * j + 3] * c1);
         }
       }
     }
-    for (int st = s0; st < s1; st += kQkUnroll) {
-      uint4 raw[kQkUnroll];
+    T* y = v < qpad ? yq : yk;
+    const int left = (v < qpad ? nq : steps) - v;
 #pragma unroll
-      for (int u = 0; u < kQkUnroll; ++u) {
-        const int h = (st + u) * HPW + sub;
-        raw[u] = make_uint4(0, 0, 0, 0);
-        if (st + u < s1 && h < heads) {
-          const int k = h >= p.H[0];
-          raw[u] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.x[k]) + t * p.ldx[k] +
-                                                   (long long)(k ? h - p.H[0] : h) * D + chunk * 8);
-        }
+    for (int u = 0; u < kQkAhead; ++u) {
+      const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+      fetch(raw[u], v + u + kQkAhead);
+      if (u >= left) continue;  // warp-uniform
+      uint64_t x[4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float2 f = unpack2<T>(w[2 * j]), g = unpack2<T>(w[2 * j + 1]);
+        x[2 * j] = HALVES ? f2_pack(f.x, f.y) : f2_pack(f.x, g.x);
+        x[2 * j + 1] = HALVES ? f2_pack(g.x, g.y) : f2_pack(f.y, g.y);
       }
-#pragma unroll
-      for (int u = 0; u < kQkUnroll; ++u) {
-        if (st + u >= s1) break;  // warp-uniform
-        const int h = (st + u) * HPW + sub;
-        const int k = h >= p.H[0];
-        float f[8];
-        unpack8<T>(raw[u], f);
-        float ss = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(f[e], f[e], ss);
+      uint64_t r2 = f2_pack(1.f, 1.f);
+      if (norm) {
+        const uint64_t q = fma2(x[0], x[0], fma2(x[1], x[1], fma2(x[2], x[2], mul2(x[3], x[3]))));
+        float ss = lo_f(q) + hi_f(q);
 #pragma unroll
         for (int o = LPH / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (p.w[k]) {
-          const float r = 1.0f / sqrtf(ss * (1.0f / D) + p.eps);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] *= r * (k ? wk[e] : wq[e]);
-        }
-        if (p.pos) {
-          if (HALVES) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float o = __shfl_xor_sync(0xffffffffu, f[e], LPH / 2);  // the pair's other value
-              f[e] = chunk < LPH / 2 ? f[e] * c[e] - o * s[e] : o * s[e] + f[e] * c[e];
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float lo = f[2 * e], hi = f[2 * e + 1];
-              f[2 * e] = lo * c[e] - hi * s[e];
-              f[2 * e + 1] = lo * s[e] + hi * c[e];
-            }
-          }
-        }
-        if (h < heads)
-          *reinterpret_cast<uint4*>(static_cast<T*>(p.y[k]) + t * p.ldy[k] + (long long)(k ? h - p.H[0] : h) * D +
-                                    chunk * 8) = pack8<T>(f);
+        const float r = rsqrtf(fmaf(ss, 1.0f / D, p.eps));
+        r2 = f2_pack(r, r);
       }
+      uint32_t out[4];
+      if (HALVES) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint64_t z = mul2(x[j], m1[j]);
+          if (p.pos) {
+            const uint64_t o = f2_pack(__shfl_xor_sync(0xffffffffu, lo_f(x[j]), LPH / 2),
+                                       __shfl_xor_sync(0xffffffffu, hi_f(x[j]), LPH / 2));
+            z = fma2(o, m2[j], z);
+          }
+          z = mul2(z, r2);
+          out[j] = pack2<T>(lo_f(z), hi_f(z));
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint64_t f = x[2 * j], g = x[2 * j + 1];
+          uint64_t f1 = mul2(f, m1[j]), g1 = mul2(g, m4[j]);
+          if (p.pos) {
+            f1 = fma2(g, m2[j], f1);
+            g1 = fma2(f, m3[j], g1);
+          }
+          f1 = mul2(f1, r2);
+          g1 = mul2(g1, r2);
+          out[2 * j] = pack2<T>(lo_f(f1), lo_f(g1));
+          out[2 * j + 1] = pack2<T>(hi_f(f1), hi_f(g1));
+        }
+      }
+      if (on) *reinterpret_cast<uint4*>(y + (long long)(v + u) * D) = make_uint4(out[0], out[1], out[2], out[3]);
     }
   }
 }
 
 template <typename T, int D>
-int launch_qk(Ctx* c, const QkParams& p, int halves) {
-  const long long groups = (p.T + p.tokens - 1) / p.tokens;
+int launch_qk(Ctx* c, QkParams& p, int halves) {
+  constexpr int TPW = 256 / D;
+  // Few tokens: their heads are shared out over warps until the card has some 8 warps per SM.
+  const long long groups = (p.T + TPW - 1) / TPW;
+  p.hsplit = (int)std::max<long long>(1, std::min<long long>(p.H[0] + p.H[1], 8LL * c->num_sms / groups));
   const long long blocks = (groups * p.hsplit + kQkWarps - 1) / kQkWarps;
   auto kern = halves ? qk_norm_rope_kernel<T, D, true> : qk_norm_rope_kernel<T, D, false>;
   launch_k(kern, dim3((unsigned)blocks), dim3(32 * kQkWarps), 0, c->stream, p);
@@ -188,17 +237,19 @@ int launch_qk(Ctx* c, const QkParams& p, int halves) {
 
 using namespace di;
 
-extern "C" int di_qk_norm_rope(di_ctx_t h, int dtype, const void* Q, long long ldq, int Hq, const void* K,
-                               long long ldk, int Hk, int T, int D, const float* q_weight, const float* k_weight,
-                               float eps, const int* positions, int pos_rows, int n_axes, const int* axis_dims,
-                               double theta, int pairing, void* Qo, long long ldqo, void* Ko, long long ldko) {
+extern "C" int di_qk_norm_rope(di_ctx_t h, int dtype, const long long cfg[14], float eps, double theta, const void* Q,
+                               const void* K, const float* q_weight, const float* k_weight, const int* positions, void* Qo,
+                               void* Ko) {
   Ctx* c = ctx_of(h);
   if (!c || (dtype != DI_F16 && dtype != DI_BF16)) return DI_EINVAL;
   DeviceGuard guard(c->device);
-  if (T <= 0 || Hq <= 0 || Hk < 0 || !Q || !Qo || (Hk > 0) != (K != nullptr) || (Hk > 0) != (Ko != nullptr))
+  if (!cfg || cfg[0] <= 0 || cfg[0] > 0x7fffffff || cfg[1] <= 0 || cfg[1] > 16384 || cfg[2] < 0 || cfg[2] > 16384 || !Q || !Qo ||
+      (cfg[2] > 0) != (K != nullptr) || (cfg[2] > 0) != (Ko != nullptr))
     return set_error(c, DI_EINVAL, "qk_norm_rope: bad shape or missing tensor");
+  const int T = (int)cfg[0], Hq = (int)cfg[1], Hk = (int)cfg[2];
+  const long long D = cfg[3], ldq = cfg[4], ldk = cfg[5], ldqo = cfg[6], ldko = cfg[7];
+  const long long pos_rows = cfg[8], pairing = cfg[9], n_axes = cfg[10], *axis_dims = cfg + 11;
   if (D != 64 && D != 128) return set_error(c, DI_EUNSUPPORTED, "qk_norm_rope: head dim must be 64 or 128");
-  if (Hq + (long long)Hk > 65536) return set_error(c, DI_EINVAL, "qk_norm_rope: more than 65536 heads");
   if (ldq < (long long)Hq * D || ldqo < (long long)Hq * D || (Hk && (ldk < (long long)Hk * D || ldko < (long long)Hk * D)))
     return set_error(c, DI_EINVAL, "qk_norm_rope: a token stride is shorter than the token's heads");
   if (!aligned16(Q) || !aligned16(Qo) || !aligned16(K) || !aligned16(Ko) || ldq % 8 || ldqo % 8 ||
@@ -209,15 +260,17 @@ extern "C" int di_qk_norm_rope(di_ctx_t h, int dtype, const void* Q, long long l
   QkParams p;
   memset(&p, 0, sizeof p);
   if (positions) {
-    if (n_axes < 1 || n_axes > 3 || pos_rows < 1 || !axis_dims || !(theta > 0.0))
+    if (n_axes < 1 || n_axes > 3 || pos_rows < 1 || pos_rows > 0x7fffffff || !(theta > 0.0))
       return set_error(c, DI_EINVAL, "qk_norm_rope: needs 1 to 3 axes, their dims, position rows and theta > 0");
     int i = 0, sum = 0;
     for (int a = 0; a < n_axes; ++a) {
       if (axis_dims[a] < 2 || axis_dims[a] % 2 || axis_dims[a] > D - sum)
         return set_error(c, DI_EINVAL, "qk_norm_rope: axis dims must be even, positive and sum to the head dim");
-      sum += axis_dims[a];
-      for (int j = 0; j < axis_dims[a] / 2; ++j, ++i) {
-        p.freq[i] = std::pow(theta, -2.0 * j / axis_dims[a]) * 0.15915494309189533577;  // 1 / (2 pi)
+      sum += (int)axis_dims[a];
+      const long double ratio = std::pow((long double)theta, -2.0L / axis_dims[a]);
+      long double f = 0.159154943091895335768883763372514362L;  // 1 / (2 pi); 64-bit products stay exact to 53 bits
+      for (int j = 0; j < axis_dims[a] / 2; ++j, ++i, f *= ratio) {
+        p.freq[i] = (double)f;
         p.axis[i] = (unsigned char)a;
       }
     }
@@ -230,16 +283,10 @@ extern "C" int di_qk_norm_rope(di_ctx_t h, int dtype, const void* Q, long long l
   p.w[0] = q_weight; p.w[1] = k_weight;
   p.H[0] = Hq; p.H[1] = Hk;
   p.T = T;
-  p.P = positions ? pos_rows : 1;
-  p.axes = n_axes;
+  p.P = positions ? (int)pos_rows : 1;
+  p.axes = (int)n_axes;
   p.pos = positions;
   p.eps = eps;
-  // A warp keeps its pairs' frequencies over a few tokens when there are enough of them for 32 warps per SM;
-  // few tokens share out their heads over warps until the card has some 8 warps per SM.
-  p.tokens = (int)std::max<long long>(1, std::min<long long>(kQkTokens, T / (32LL * c->num_sms)));
-  const int steps = (Hq + Hk + 256 / D - 1) / (256 / D);
-  const long long groups = ((long long)T + p.tokens - 1) / p.tokens;
-  p.hsplit = (int)std::max<long long>(1, std::min<long long>(steps, 8LL * c->num_sms / groups));
-  if (dtype == DI_F16) return D == 64 ? launch_qk<__half, 64>(c, p, pairing) : launch_qk<__half, 128>(c, p, pairing);
-  return D == 64 ? launch_qk<__nv_bfloat16, 64>(c, p, pairing) : launch_qk<__nv_bfloat16, 128>(c, p, pairing);
+  if (dtype == DI_F16) return D == 64 ? launch_qk<__half, 64>(c, p, (int)pairing) : launch_qk<__half, 128>(c, p, (int)pairing);
+  return D == 64 ? launch_qk<__nv_bfloat16, 64>(c, p, (int)pairing) : launch_qk<__nv_bfloat16, 128>(c, p, (int)pairing);
 }

@@ -949,30 +949,33 @@ int launch_xattn(Ctx* c, XattnParams& p) {
 
 using namespace di;
 
-extern "C" size_t di_cross_attention_workspace(di_ctx_t h, int B, int H, int Hkv, int Sq, int Skv, int D) {
-  if (!h || B <= 0 || H <= 0 || Hkv <= 0 || Sq <= 0 || Skv <= 0 || D <= 0 || H % Hkv) return 0;
-  if (D != 64 && D != 128) return 0;
-  const XPlan x = xattn_plan(ctx_of(h), B, H, Hkv, Sq, Skv, D);
+extern "C" size_t di_cross_attention_workspace(di_ctx_t h, const long long cfg[18]) {
+  if (!h || !cfg) return 0;
+  for (int i = 0; i < 6; ++i)
+    if (cfg[i] <= 0 || cfg[i] > (1ll << 30)) return 0;
+  const int B = (int)cfg[0], H = (int)cfg[1], Hkv = (int)cfg[2], D = (int)cfg[5];
+  if (H % Hkv || (D != 64 && D != 128)) return 0;
+  const XPlan x = xattn_plan(ctx_of(h), B, H, Hkv, (int)cfg[3], (int)cfg[4], D);
   return (size_t)x.slots * 2 * 128 * (D + 2) * 4;
 }
 
-extern "C" int di_cross_attention(di_ctx_t h, int dtype, const void* Q, const long long q_strides[3], const void* K,
-                                  const long long k_strides[3], const void* V, const long long v_strides[3], void* O,
-                                  const long long o_strides[3], int B, int H, int Hkv, int Sq, int Skv, int D,
-                                  const int* q_len, const int* kv_len, const unsigned char* key_mask, float scale,
-                                  void* ws, size_t ws_bytes) {
+extern "C" int di_cross_attention(di_ctx_t h, int dtype, const long long cfg[18], float scale, const void* Q, const void* K,
+                                  const void* V, void* O, const int* q_len, const int* kv_len,
+                                  const unsigned char* key_mask, void* ws, size_t ws_bytes) {
   Ctx* c = ctx_of(h);
   if (!c || (dtype != DI_F16 && dtype != DI_BF16)) return DI_EINVAL;
   DeviceGuard guard(c->device);
-  if (B <= 0 || H <= 0 || Hkv <= 0 || Sq <= 0 || Skv <= 0 || !Q || !K || !V || !O || !q_strides || !k_strides ||
-      !v_strides || !o_strides)
-    return set_error(c, DI_EINVAL, "cross_attention: bad shape or missing tensor");
+  if (!cfg || !Q || !K || !V || !O) return set_error(c, DI_EINVAL, "cross_attention: bad shape or missing tensor");
+  for (int i = 0; i < 6; ++i)
+    if (cfg[i] <= 0 || cfg[i] > (1ll << 30)) return set_error(c, DI_EINVAL, "cross_attention: bad shape or missing tensor");
+  const int B = (int)cfg[0], H = (int)cfg[1], Hkv = (int)cfg[2], Sq = (int)cfg[3], Skv = (int)cfg[4], D = (int)cfg[5];
+  const long long *q_strides = cfg + 6, *k_strides = cfg + 9, *v_strides = cfg + 12, *o_strides = cfg + 15;
   if (H % Hkv) return set_error(c, DI_EINVAL, "cross_attention: H must be a multiple of Hkv");
   if (D != 64 && D != 128) return set_error(c, DI_EUNSUPPORTED, "cross_attention: head dim must be 64 or 128");
   if (!aligned16(Q) || !aligned16(K) || !aligned16(V) || !aligned16(O))
     return set_error(c, DI_EINVAL, "cross_attention: pointers must be 16-byte aligned");
   const XPlan x = xattn_plan(c, B, H, Hkv, Sq, Skv, D);
-  if ((long long)Sq * x.GP > (1 << 30) || Skv > (1 << 30) || (long long)B * x.HG * x.RT > 0x7fffffffll)
+  if ((long long)Sq * x.GP > (1 << 30) || (long long)B * x.HG * x.RT > 0x7fffffffll)
     return set_error(c, DI_EUNSUPPORTED, "cross_attention: too many tokens");
   // strides of axes of length one mean nothing: they are replaced by 8 elements (a valid tensor-map stride)
   long long qs[3], ks[3], vs[3], os[3];
@@ -989,7 +992,7 @@ extern "C" int di_cross_attention(di_ctx_t h, int dtype, const void* Q, const lo
   if (qs[1] == 0 || ks[1] == 0 || vs[1] == 0 || (qs[2] == 0 && x.GP > 1))
     return set_error(c, DI_EINVAL, "cross_attention: tokens and grouped query heads cannot be expanded");
   if (!(scale > 0.f) || !(scale < INFINITY)) return set_error(c, DI_EINVAL, "cross_attention: scale must be positive and finite");
-  const size_t need = di_cross_attention_workspace(h, B, H, Hkv, Sq, Skv, D);
+  const size_t need = di_cross_attention_workspace(h, cfg);
   if (need && (!ws || ws_bytes < need || !aligned16(ws)))
     return set_error(c, DI_EINVAL, "cross_attention: workspace missing, too small or not 16-byte aligned");
   XattnParams p;

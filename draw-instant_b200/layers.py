@@ -12,11 +12,13 @@ them, share none.  A result is the `out` that was passed, or a new tensor.  Bad 
     q = linear_lora(ctx, x, w_q, a_q, b_q, scale, rows).view(B * S, H, 64)
     qk_norm_rope(ctx, q, q_weight=g, positions=pos, axis_dims=(32, 32), q_out=q)
     o = cross_attention(ctx, q.view(B, S, H, 64), k, v, kv_len=prompt_lengths)
+
+A call's checks and its cfg block depend on shapes, strides, types and devices alone.  They are kept per such
+signature, so a repeated call costs one dictionary lookup before it launches.
 """
 from __future__ import annotations
 
 import ctypes
-import functools
 
 import torch
 
@@ -27,6 +29,21 @@ __all__ = ["linear_lora", "qk_norm_rope", "cross_attention"]
 _CODE = {torch.float16: DI_F16, torch.bfloat16: DI_BF16}
 _ACT = {"none": 0, "silu": 1, "gelu": 2}
 _PAIRING = {"interleaved": 0, "halves": 1}
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+# signature of a call -> (dtype code, cfg block, scratch bytes, shape of a new result, dtype)
+_plans: dict = {}
+
+
+def _keep(key, plan):
+    if len(_plans) >= 4096:
+        _plans.clear()
+    _plans[key] = plan
+    return plan
+
+
+def _cfg(*vals):
+    return (ctypes.c_longlong * len(vals))(*vals)
 
 
 def _code(t, what: str) -> int:
@@ -56,24 +73,16 @@ def _like(t, dtype, shape, what: str) -> None:
 
 def _new(ctx: Context, shape, dtype):
     """A tensor whose memory belongs to the context's stream."""
-    if torch.cuda.current_stream(ctx.device).cuda_stream == ctx.stream.cuda_stream:
-        return torch.empty(shape, dtype=dtype, device=ctx.stream.device)
-    with torch.cuda.stream(ctx.stream):
-        return torch.empty(shape, dtype=dtype, device=ctx.stream.device)
+    st = ctx.stream
+    now = _raw_stream(ctx.device) if _raw_stream else torch.cuda.current_stream(ctx.device).cuda_stream
+    if now == st.cuda_stream:
+        return torch.empty(shape, dtype=dtype, device=st.device)
+    with torch.cuda.stream(st):
+        return torch.empty(shape, dtype=dtype, device=st.device)
 
 
-def _p(t):
-    return None if t is None else t.data_ptr()
-
-
-@functools.lru_cache(maxsize=256)
-def _i64x3(a: int, b: int, c: int):
-    return (ctypes.c_longlong * 3)(a, b, c)
-
-
-@functools.lru_cache(maxsize=64)
-def _ints(vals):
-    return (ctypes.c_int * max(1, len(vals)))(*vals)
+def _sig(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
 
 
 def _rows(t, shape, dtype, what: str):
@@ -89,9 +98,28 @@ def linear_lora(ctx: Context, x, w, a, b, scale, row_adapter, bias=None, residua
 
     x [M, K], w [N, K], a [L, r, K], b [L, N, r] (fp16 or bf16), scale [L] fp32, row_adapter [M] int32 on the
     device (negative: no adapter), bias [N] fp32, residual and out [M, N].  K a multiple of 64, N of 16, r of 8 up
-    to 128: adapters of other ranks are padded with zeros.  x, residual and out may have a row stride.  Rows may
-    take the adapters in any order; equal neighbours are fastest.  act: none, silu or gelu, before the residual.
-    An index past the last adapter sets DEVERR_BOUNDS in the context's fault word and counts as none."""
+    to 128: adapters of other ranks are padded with zeros.  x, residual and out may have a row stride; out may be
+    the residual.  Rows may take the adapters in any order; from some hundred rows on, equal neighbours are fastest.
+    act: none, silu or gelu, before the residual.  An index past the last adapter sets flag 16 in the context's fault
+    word and counts as none.  In fp16, scale * (x a^T) has to stay inside the type's range."""
+    key = (ctx.device, act, _sig(x), _sig(w), _sig(a), _sig(b), _sig(scale), _sig(row_adapter), _sig(bias), _sig(residual), _sig(out))
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _keep(key, _plan_lora(ctx, x, w, a, b, scale, row_adapter, bias, residual, act, out))
+    code, cfg, n, shape, dt = plan
+    if out is None:
+        out = _new(ctx, shape, dt)
+    ws = _new(ctx, n, torch.uint8) if n else None
+    rc = lib().di_linear_lora(ctx.h, code, cfg, x.data_ptr(), w.data_ptr(), a.data_ptr(), b.data_ptr(), scale.data_ptr(),
+                              row_adapter.data_ptr(), None if bias is None else bias.data_ptr(),
+                              None if residual is None else residual.data_ptr(), out.data_ptr(),
+                              None if ws is None else ws.data_ptr(), n)
+    if rc:
+        ctx.check(rc, "linear_lora")
+    return out
+
+
+def _plan_lora(ctx, x, w, a, b, scale, row_adapter, bias, residual, act, out):
     what = "linear_lora"
     code, dt = _code(x, what), x.dtype
     _need(x.dim() == 2 and w.dim() == 2 and a.dim() == 3 and b.dim() == 3, f"{what}: x and w are matrices, a and b have three axes")
@@ -109,14 +137,8 @@ def linear_lora(ctx: Context, x, w, a, b, scale, row_adapter, bias=None, residua
     ldr = 0 if residual is None else _rows(residual, (M, N), dt, f"{what}: residual")
     ldy = N if out is None else _rows(out, (M, N), dt, f"{what}: out")
     _on(ctx, what, x, w, a, b, scale, row_adapter, bias, residual, out)
-    if out is None:
-        out = _new(ctx, (M, N), dt)
-    n = lib().di_linear_lora_workspace(ctx.h, M, N, K, r, L)
-    ws = _new(ctx, (n,), torch.uint8) if n else None
-    ctx.check(lib().di_linear_lora(ctx.h, code, x.data_ptr(), ldx, M, K, w.data_ptr(), N, a.data_ptr(), b.data_ptr(), r, L,
-                                   scale.data_ptr(), row_adapter.data_ptr(), _p(bias), _p(residual), ldr, _ACT[act],
-                                   out.data_ptr(), ldy, _p(ws), n), what)
-    return out
+    cfg = _cfg(M, N, K, r, L, ldx, ldr, ldy, _ACT[act])
+    return code, cfg, lib().di_linear_lora_workspace(ctx.h, cfg), (M, N), dt
 
 
 def _heads(t, dt, D, what: str):
@@ -139,6 +161,28 @@ def qk_norm_rope(ctx: Context, q, k=None, q_weight=None, k_weight=None, eps: flo
     on the device, token t takes row t % P, None: no rotation.  axis_dims: n = 1 to 3 even dims that sum to D, in
     the positions' order; pair j of axis a turns by positions[., a] * theta^(-2 j / axis_dims[a]).  pairing:
     "interleaved" (values 2i, 2i + 1) or "halves" (values i, i + D / 2)."""
+    if not theta > 0:
+        raise DIError("qk_norm_rope: theta must be positive")
+    key = (ctx.device, pairing, tuple(axis_dims), _sig(q), _sig(k), _sig(q_weight), _sig(k_weight), _sig(positions), _sig(q_out), _sig(k_out))
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _keep(key, _plan_qk(ctx, q, k, q_weight, k_weight, positions, axis_dims, pairing, q_out, k_out))
+    code, cfg = plan
+    if q_out is None:
+        q_out = _new(ctx, q.shape, q.dtype)
+    if k is not None and k_out is None:
+        k_out = _new(ctx, k.shape, q.dtype)
+    rc = lib().di_qk_norm_rope(ctx.h, code, cfg, eps, theta, q.data_ptr(), None if k is None else k.data_ptr(),
+                               None if q_weight is None else q_weight.data_ptr(),
+                               None if k_weight is None else k_weight.data_ptr(),
+                               None if positions is None else positions.data_ptr(), q_out.data_ptr(),
+                               None if k is None else k_out.data_ptr())
+    if rc:
+        ctx.check(rc, "qk_norm_rope")
+    return q_out if k is None else (q_out, k_out)
+
+
+def _plan_qk(ctx, q, k, q_weight, k_weight, positions, axis_dims, pairing, q_out, k_out):
     what = "qk_norm_rope"
     code, dt = _code(q, what), q.dtype
     _need(q.dim() == 3, f"{what}: q must have the axes [tokens, heads, head dim]")
@@ -155,45 +199,35 @@ def qk_norm_rope(ctx: Context, q, k=None, q_weight=None, k_weight=None, eps: flo
         _need(k_out is None, f"{what}: k_out without k")
     _like(q_weight, torch.float32, (D,), f"{what}: q_weight")
     _like(k_weight, torch.float32, (D,), f"{what}: k_weight")
-    axis_dims = tuple(axis_dims)
+    dims = tuple(axis_dims)
     P = 0
     if positions is not None:
-        _need(1 <= len(axis_dims) <= 3 and all(d > 0 and d % 2 == 0 for d in axis_dims) and sum(axis_dims) == D,
+        _need(1 <= len(dims) <= 3 and all(d > 0 and d % 2 == 0 for d in dims) and sum(dims) == D,
               f"{what}: axis_dims must be 1 to 3 even dims that sum to the head dim")
         _need(positions.dim() == 2 and positions.shape[0] > 0, f"{what}: positions must have the axes [rows, position axes]")
         P = positions.shape[0]
-        _like(positions, torch.int32, (P, len(axis_dims)), f"{what}: positions")
-        _need(theta > 0, f"{what}: theta must be positive")
+        _like(positions, torch.int32, (P, len(dims)), f"{what}: positions")
     else:
-        _need(not axis_dims, f"{what}: axis_dims without positions")
+        _need(not dims, f"{what}: axis_dims without positions")
+    ldqo = Hq * D
     if q_out is not None:
         _need(q_out.shape == q.shape, f"{what}: q_out must have the shape of q")
         ldqo = _heads(q_out, dt, D, f"{what}: q_out")[1]
-    else:
-        ldqo = Hq * D
     if k_out is not None:
         _need(k_out.shape == k.shape, f"{what}: k_out must have the shape of k")
         ldko = _heads(k_out, dt, D, f"{what}: k_out")[1]
     elif Hk:
         ldko = Hk * D
     _on(ctx, what, q, k, q_weight, k_weight, positions, q_out, k_out)
-    if q_out is None:
-        q_out = _new(ctx, (T, Hq, D), dt)
-    if k is not None and k_out is None:
-        k_out = _new(ctx, (T, Hk, D), dt)
-    ctx.check(lib().di_qk_norm_rope(ctx.h, code, q.data_ptr(), ldq, Hq, _p(k), ldk, Hk, T, D, _p(q_weight),
-                                    _p(k_weight), eps, _p(positions), P, len(axis_dims), _ints(axis_dims), theta,
-                                    _PAIRING[pairing], q_out.data_ptr(), ldqo, _p(k_out), ldko), what)
-    return q_out if k is None else (q_out, k_out)
+    return code, _cfg(T, Hq, Hk, D, ldq, ldk, ldqo, ldko, P, _PAIRING[pairing], len(dims), *(dims + (0, 0, 0))[:3])
 
 
 def _bshd(t, dt, what: str):
     """Batch, token and head strides of a [B, S, H, D] tensor whose last axis is contiguous."""
-    sb, ss, sh, sd = t.stride()
-    if t.dtype != dt or sd != 1:
+    if t.dtype != dt or t.stride(3) != 1:
         raise DIError(f"{what} must be a {dt} tensor [batch, tokens, heads, head dim] with a contiguous last axis, "
                       f"got {t.dtype} {tuple(t.shape)} with strides {t.stride()}")
-    return _i64x3(sb, ss, sh)
+    return t.stride()[:3]
 
 
 def cross_attention(ctx: Context, q, k, v, kv_len=None, q_len=None, key_mask=None, scale: float | None = None, out=None):
@@ -206,6 +240,27 @@ def cross_attention(ctx: Context, q, k, v, kv_len=None, q_len=None, key_mask=Non
     bool, both on the device, None: all); what masked keys and values hold, infinities and NaN included, has no effect.
     A request without a valid key gives zeros.  Query rows from q_len[b] on (int32) are not computed and
     their rows of out stay as they were.  scale: positive, 1 / sqrt(D) by default."""
+    if scale is not None and not 0 < scale < float("inf"):
+        raise DIError("cross_attention: scale must be positive and finite")
+    key = (ctx.device, _sig(q), _sig(k), _sig(v), _sig(kv_len), _sig(q_len), _sig(key_mask), _sig(out))
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _keep(key, _plan_cross(ctx, q, k, v, kv_len, q_len, key_mask, out))
+    code, cfg, n, default, _ = plan
+    if scale is None:
+        scale = default
+    if out is None:
+        out = _new(ctx, q.shape, q.dtype)
+    ws = _new(ctx, n, torch.uint8) if n else None
+    rc = lib().di_cross_attention(ctx.h, code, cfg, scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                                  None if q_len is None else q_len.data_ptr(), None if kv_len is None else kv_len.data_ptr(),
+                                  None if key_mask is None else key_mask.data_ptr(), None if ws is None else ws.data_ptr(), n)
+    if rc:
+        ctx.check(rc, "cross_attention")
+    return out
+
+
+def _plan_cross(ctx, q, k, v, kv_len, q_len, key_mask, out):
     what = "cross_attention"
     code, dt = _code(q, what), q.dtype
     _need(q.dim() == 4 and k.dim() == 4 and v.dim() == 4, f"{what}: q, k and v must have the axes [batch, tokens, heads, head dim]")
@@ -215,10 +270,7 @@ def cross_attention(ctx: Context, q, k, v, kv_len=None, q_len=None, key_mask=Non
     _need(D in (64, 128), f"{what}: head dim must be 64 or 128, got {D}")
     _need(k.shape == (B, Skv, Hkv, D) and v.shape == k.shape, f"{what}: k and v must be [{B}, tokens, heads, {D}], alike")
     _need(H % Hkv == 0, f"{what}: the query heads must be a multiple of the key heads")
-    if scale is None:
-        scale = D ** -0.5
-    _need(0 < scale < float("inf"), f"{what}: scale must be positive and finite")
-    qs, ks, vs = _bshd(q, dt, f"{what}: q"), _bshd(k, dt, f"{what}: k"), _bshd(v, dt, f"{what}: v")
+    strides = [_bshd(t, dt, f"{what}: {n}") for t, n in ((q, "q"), (k, "k"), (v, "v"))]
     _like(kv_len, torch.int32, (B,), f"{what}: kv_len")
     _like(q_len, torch.int32, (B,), f"{what}: q_len")
     if key_mask is not None and key_mask.dtype == torch.bool:
@@ -226,14 +278,9 @@ def cross_attention(ctx: Context, q, k, v, kv_len=None, q_len=None, key_mask=Non
     _like(key_mask, torch.uint8, (B, Skv), f"{what}: key_mask")
     if out is not None:
         _need(out.shape == q.shape, f"{what}: out must have the shape of q")
-        os_ = _bshd(out, dt, f"{what}: out")
+        strides.append(_bshd(out, dt, f"{what}: out"))
     else:
-        os_ = _i64x3(Sq * H * D, H * D, D)
+        strides.append((Sq * H * D, H * D, D))
     _on(ctx, what, q, k, v, kv_len, q_len, key_mask, out)
-    if out is None:
-        out = _new(ctx, (B, Sq, H, D), dt)
-    n = lib().di_cross_attention_workspace(ctx.h, B, H, Hkv, Sq, Skv, D)
-    ws = _new(ctx, (n,), torch.uint8) if n else None
-    ctx.check(lib().di_cross_attention(ctx.h, code, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(), os_,
-                                       B, H, Hkv, Sq, Skv, D, _p(q_len), _p(kv_len), _p(key_mask), scale, _p(ws), n), what)
-    return out
+    cfg = _cfg(B, H, Hkv, Sq, Skv, D, *(s for t in strides for s in t))
+    return code, cfg, lib().di_cross_attention_workspace(ctx.h, cfg), D ** -0.5, dt

@@ -218,36 +218,35 @@ DI_API int di_attention_causal(di_ctx_t ctx, int dtype, const void* Q, const voi
  * ------------------------------------------------------------------------------------------- */
 /* Linear layer with a low-rank adapter per row: Y[m] = act(X[m] . W^T + bias + scale[a] * (X[m] . A[a]^T) . B[a]^T)
  * + R[m] with a = row_adapter[m] in [0, n_adapters), none when negative; an index past the last adapter
- * counts as none and sets flag 16 in the device error word.  X [M,K] rows ldx, W [N,K], A [n_adapters,
- * rank,K], B [n_adapters,N,rank], scale [n_adapters] and bias [N] (may be NULL) fp32, R [M,N] rows ldr (may
- * be NULL, may be Y), Y rows ldy.  act as in di_linear_act.  K a multiple of 64, N of 16, rank of 8 up to
- * 128 (pad adapters of other ranks with zeros). */
-DI_API size_t di_linear_lora_workspace(di_ctx_t ctx, int M, int N, int K, int rank, int n_adapters);
-DI_API int di_linear_lora(di_ctx_t ctx, int dtype, const void* X, long long ldx, int M, int K, const void* W, int N,
-                          const void* A, const void* B, int rank, int n_adapters, const float* scale,
-                          const int* row_adapter, const float* bias, const void* R, long long ldr, int act, void* Y,
-                          long long ldy, void* ws, size_t ws_bytes);
+ * counts as none and sets flag 16 in the device error word.  cfg = {M, N, K, rank, n_adapters, ldx, ldr, ldy,
+ * act}: X [M,K] rows ldx, W [N,K], A [n_adapters,rank,K], B [n_adapters,N,rank], scale [n_adapters] and bias
+ * [N] (may be NULL) fp32, R [M,N] rows ldr (may be NULL, may be Y), Y rows ldy; act as in di_linear_act.
+ * K a multiple of 64, N of 16, rank of 8 up to 128 (pad adapters of other ranks with zeros).  In fp16,
+ * scale * (X . A^T) has to stay inside the type's range. */
+DI_API size_t di_linear_lora_workspace(di_ctx_t ctx, const long long cfg[9]);
+DI_API int di_linear_lora(di_ctx_t ctx, int dtype, const long long cfg[9], const void* X, const void* W, const void* A,
+                          const void* B, const float* scale, const int* row_adapter, const float* bias, const void* R,
+                          void* Y, void* ws, size_t ws_bytes);
 /* RMS norm of query and key heads and their rotation by position axes in one pass: per token t and head
- * y = rotate(x * rsqrt(mean(x^2) + eps) * weight, positions[t % pos_rows]).  Q [T,Hq,D] with token stride ldq, K
- * [T,Hk,D] with ldk (NULL with Hk = 0: queries only), heads contiguous, D 64 or 128; weights [D] fp32, NULL:
- * no norm.  positions [pos_rows, n_axes] int32, NULL: no rotation; axis a (1 to 3 of them) owns the next
+ * y = rotate(x * rsqrt(mean(x^2) + eps) * weight, positions[t % pos_rows]).  cfg = {T, Hq, Hk, D, ldq, ldk, ldqo,
+ * ldko, pos_rows, pairing, n_axes, axis_dims[3]}: Q [T,Hq,D] with token stride ldq, K [T,Hk,D] with ldk (NULL
+ * with Hk = 0: queries only), outputs with ldqo, ldko, heads contiguous, D 64 or 128; weights [D] fp32, NULL: no
+ * norm.  positions [pos_rows, n_axes] int32, NULL: no rotation; axis a (1 to 3 of them) owns the next
  * axis_dims[a] / 2 value pairs, even dims that sum to D, and pair j of axis a turns by position *
  * theta^(-2j / axis_dims[a]) radians.  pairing 0: values (2i, 2i + 1); 1: values (i, i + D/2).  The outputs may
  * be the inputs. */
-DI_API int di_qk_norm_rope(di_ctx_t ctx, int dtype, const void* Q, long long ldq, int Hq, const void* K,
-                           long long ldk, int Hk, int T, int D, const float* q_weight, const float* k_weight,
-                           float eps, const int* positions, int pos_rows, int n_axes, const int* axis_dims,
-                           double theta, int pairing, void* Qo, long long ldqo, void* Ko, long long ldko);
+DI_API int di_qk_norm_rope(di_ctx_t ctx, int dtype, const long long cfg[14], float eps, double theta, const void* Q,
+                           const void* K, const float* q_weight, const float* k_weight, const int* positions, void* Qo,
+                           void* Ko);
 /* Attention over an encoder's states: O = softmax(scale * Q K^T) V over each request's valid keys: j <
  * kv_len[b] (NULL: Skv; values outside [0, Skv] are clamped) and key_mask[b * Skv + j] != 0 (NULL: all).
  * Masked keys and values may hold anything, infinities and NaN included.  A request without valid keys
- * gives zeros; query rows from q_len[b] on (NULL: Sq) are not written.  Q, O [B,Sq,H,D], K, V [B,Skv,Hkv,D], H a
- * multiple of Hkv, D 64 or 128, strides {batch, token, head} (0 expands an input over an axis), scale > 0. */
-DI_API size_t di_cross_attention_workspace(di_ctx_t ctx, int B, int H, int Hkv, int Sq, int Skv, int D);
-DI_API int di_cross_attention(di_ctx_t ctx, int dtype, const void* Q, const long long q_strides[3], const void* K,
-                              const long long k_strides[3], const void* V, const long long v_strides[3], void* O,
-                              const long long o_strides[3], int B, int H, int Hkv, int Sq, int Skv, int D,
-                              const int* q_len, const int* kv_len, const unsigned char* key_mask, float scale,
+ * gives zeros; query rows from q_len[b] on (NULL: Sq) are not written.  cfg = {B, H, Hkv, Sq, Skv, D, Q strides
+ * {batch, token, head}, K strides, V strides, O strides}: Q, O [B,Sq,H,D], K, V [B,Skv,Hkv,D], H a multiple of Hkv,
+ * D 64 or 128 (a stride of 0 expands an input over its batch or heads); scale > 0. */
+DI_API size_t di_cross_attention_workspace(di_ctx_t ctx, const long long cfg[18]);
+DI_API int di_cross_attention(di_ctx_t ctx, int dtype, const long long cfg[18], float scale, const void* Q, const void* K,
+                              const void* V, void* O, const int* q_len, const int* kv_len, const unsigned char* key_mask,
                               void* ws, size_t ws_bytes);
 
 /* Timestep embedding, fused-tembed.js:73-130: y[b] = W2 . silu(W1 . [cos||sin](t_b f) + b1) + b2 with

@@ -212,27 +212,33 @@ def test_lora_back_to_back(ctx, layers, M, per, K, N, r, L):
 
 
 def test_lora_c_entry_refusals(ctx, dib):
+    import ctypes
     L, s = dib.lib(), lora_case(1, 4, 64, 32, 8, 2, torch.float16)
     y = torch.empty(4, 32, dtype=torch.float16, device="cuda")
     ws = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
 
     def call(**k):
-        v = dict(dtype=1, X=s["x"].data_ptr(), ldx=64, M=4, K=64, W=s["w"].data_ptr(), N=32, A=s["a"].data_ptr(),
-                 B=s["b"].data_ptr(), r=8, L=2, scale=s["scale"].data_ptr(), rows=s["row_adapter"].data_ptr(), bias=None, R=None,
-                 ldr=0, act=0, Y=y.data_ptr(), ldy=32, ws=ws.data_ptr(), n=ws.numel())
-        v.update(k)
+        c = dict(M=4, N=32, K=64, r=8, L=2, ldx=64, ldr=0, ldy=32, act=0)
+        v = dict(dtype=1, cfg=None, X=s["x"].data_ptr(), W=s["w"].data_ptr(), A=s["a"].data_ptr(), B=s["b"].data_ptr(),
+                 scale=s["scale"].data_ptr(), rows=s["row_adapter"].data_ptr(), bias=None, R=None, Y=y.data_ptr(), ws=ws.data_ptr(),
+                 n=ws.numel())
+        for key, val in k.items():
+            (c if key in c else v)[key] = val
+        v["cfg"] = (ctypes.c_longlong * 9)(*c.values())
         return L.di_linear_lora(ctx.h, *v.values())
 
     assert call() == 0
-    for bad in (dict(dtype=0), dict(M=0), dict(N=0), dict(L=0), dict(X=None), dict(A=None), dict(rows=None), dict(ldx=56), dict(ldx=68),
-                dict(ldy=24), dict(ldy=36), dict(X=s["x"].data_ptr() + 2), dict(Y=y.data_ptr() + 8), dict(act=3), dict(act=-1),
-                dict(R=y.data_ptr(), ldr=0)):
+    for bad in (dict(dtype=0), dict(M=0), dict(M=-1), dict(M=1 << 40), dict(N=0), dict(L=0), dict(X=None), dict(A=None), dict(rows=None),
+                dict(ldx=56), dict(ldx=68), dict(ldy=24), dict(ldy=36), dict(X=s["x"].data_ptr() + 2), dict(Y=y.data_ptr() + 8),
+                dict(act=3), dict(act=-1), dict(R=y.data_ptr(), ldr=0)):
         assert call(**bad) == dib.DI_EINVAL, bad
     for bad in (dict(K=32), dict(K=96), dict(N=24), dict(r=12), dict(r=0), dict(r=136)):
         assert call(**bad) == dib.DI_EUNSUPPORTED, bad
-    need = L.di_linear_lora_workspace(ctx.h, 4, 32, 64, 8, 2)
-    if need:
-        assert call(ws=None) == dib.DI_EINVAL and call(n=need - 1) == dib.DI_EINVAL
+    for M in (4, 64, 500):  # scratch that is missing, too small or misaligned (M rows need not exist: nothing is launched)
+        need = L.di_linear_lora_workspace(ctx.h, (ctypes.c_longlong * 9)(M, 32, 64, 8, 2, 64, 0, 32, 0))
+        if need:
+            for bad in (dict(ws=None), dict(n=need - 1), dict(ws=ws.data_ptr() + 8)):
+                assert call(M=M, **bad) == dib.DI_EINVAL, bad
 
 
 # ---- qk_norm_rope ---------------------------------------------------------------------------------------------
@@ -335,16 +341,19 @@ def test_qk_c_entry_refusals(ctx, dib):
     pos = torch.zeros(4, 2, dtype=torch.int32, device="cuda")
 
     def call(dims=(32, 32), **k):
-        v = dict(dtype=1, Q=q.data_ptr(), ldq=128, Hq=2, K=None, ldk=0, Hk=0, T=4, D=64, wq=None, wk=None, eps=1e-6,
-                 pos=pos.data_ptr(), P=4, n=len(dims), dims=(ctypes.c_int * 4)(*dims), theta=1e4, pairing=0, Qo=q.data_ptr(),
-                 ldqo=128, Ko=None, ldko=0)
-        v.update(k)
+        c = dict(T=4, Hq=2, Hk=0, D=64, ldq=128, ldk=0, ldqo=128, ldko=0, P=4, pairing=0, n=len(dims))
+        v = dict(dtype=1, cfg=None, eps=1e-6, theta=1e4, Q=q.data_ptr(), K=None, wq=None, wk=None, pos=pos.data_ptr(),
+                 Qo=q.data_ptr(), Ko=None)
+        for key, val in k.items():
+            (c if key in c else v)[key] = val
+        v["cfg"] = (ctypes.c_longlong * 16)(*c.values(), *dims)
         return L.di_qk_norm_rope(ctx.h, *v.values())
 
     assert call() == 0
-    for bad in (dict(dtype=0), dict(T=0), dict(Hq=0), dict(Q=None), dict(Hk=1), dict(K=q.data_ptr()), dict(ldq=64), dict(ldq=132),
-                dict(Q=q.data_ptr() + 2), dict(dims=(32, 16)), dict(dims=(33, 31)), dict(dims=(32, 32, -2)), dict(dims=()),
-                dict(dims=(16, 16, 16, 16)), dict(P=0), dict(theta=0.0), dict(pairing=2), dict(eps=-1.0), dict(eps=float("nan"))):
+    for bad in (dict(dtype=0), dict(T=0), dict(T=-4), dict(Hq=0), dict(Q=None), dict(Hk=1), dict(K=q.data_ptr()), dict(ldq=64),
+                dict(ldq=132), dict(Q=q.data_ptr() + 2), dict(dims=(32, 16)), dict(dims=(33, 31)), dict(dims=(32, 32, -2)),
+                dict(dims=()), dict(dims=(16, 16, 16, 16)), dict(P=0), dict(theta=0.0), dict(pairing=2), dict(eps=-1.0),
+                dict(eps=float("nan"))):
         assert call(**bad) == dib.DI_EINVAL, bad
     assert call(D=96) == dib.DI_EUNSUPPORTED
 
@@ -506,20 +515,22 @@ def test_cross_c_entry_refusals(ctx, dib):
     import ctypes
     L = dib.lib()
     q = torch.zeros(2, 3, 4, 64, dtype=torch.float16, device="cuda")
-    st = lambda *v: (ctypes.c_longlong * 3)(*v)  # noqa: E731
     ws = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
 
     def call(**k):
-        v = dict(dtype=1, Q=q.data_ptr(), qs=st(768, 256, 64), K=q.data_ptr(), ks=st(768, 256, 64), V=q.data_ptr(),
-                 vs=st(768, 256, 64), O=q.data_ptr(), os=st(768, 256, 64), B=2, H=4, Hkv=4, Sq=3, Skv=3, D=64, ql=None, kl=None,
-                 mask=None, scale=0.125, ws=ws.data_ptr(), n=ws.numel())
-        v.update(k)
+        c = dict(B=2, H=4, Hkv=4, Sq=3, Skv=3, D=64)
+        st = {n: (768, 256, 64) for n in ("qs", "ks", "vs", "os")}
+        v = dict(dtype=1, cfg=None, scale=0.125, Q=q.data_ptr(), K=q.data_ptr(), V=q.data_ptr(), O=q.data_ptr(), ql=None, kl=None,
+                 mask=None, ws=ws.data_ptr(), n=ws.numel())
+        for key, val in k.items():
+            (c if key in c else st if key in st else v)[key] = val
+        v["cfg"] = (ctypes.c_longlong * 18)(*c.values(), *(s for t in st.values() for s in t))
         return L.di_cross_attention(ctx.h, *v.values())
 
-    for bad in (dict(dtype=0), dict(B=0), dict(Sq=0), dict(Skv=0), dict(H=0), dict(Hkv=3), dict(Q=None), dict(ks=None),
-                dict(K=q.data_ptr() + 2), dict(ks=st(768, 252, 64)), dict(qs=st(-768, 256, 64)), dict(os=st(0, 256, 64)),
-                dict(os=st(768, 0, 64)), dict(os=st(768, 256, 0)), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
-                dict(scale=float("inf"))):
+    for bad in (dict(dtype=0), dict(B=0), dict(Sq=0), dict(Sq=-1), dict(Skv=0), dict(Skv=1 << 33), dict(H=0), dict(Hkv=3), dict(Q=None),
+                dict(K=q.data_ptr() + 2), dict(ks=(768, 252, 64)), dict(qs=(-768, 256, 64)), dict(os=(0, 256, 64)),
+                dict(os=(768, 0, 64)), dict(os=(768, 256, 0)), dict(ks=(768, 0, 64)), dict(scale=0.0), dict(scale=-1.0),
+                dict(scale=float("nan")), dict(scale=float("inf"))):
         assert call(**bad) == dib.DI_EINVAL, bad
     assert call(D=96) == dib.DI_EUNSUPPORTED
 

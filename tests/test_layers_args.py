@@ -107,10 +107,16 @@ def test_valid_arguments_end_at_the_device(layers, dib, op):
 
 
 def test_null_context_is_refused(dib):
-    L = dib.lib()
-    assert L.di_linear_lora(None, 1, *([None, 0] + [0, 0, None, 0, None, None, 8, 1] + [None] * 4 + [0, 0, None, 0, None, 0])) == dib.DI_EINVAL
-    assert L.di_qk_norm_rope(None, 1, None, 0, 0, None, 0, 0, 0, 64, None, None, 0.0, None, 0, 0, None, 0.0, 0, None, 0,
-                             None, 0) == dib.DI_EINVAL
-    assert L.di_cross_attention(None, 1, *([None] * 8), 1, 1, 1, 1, 1, 64, None, None, None, 1.0, None, 0) == dib.DI_EINVAL
-    assert L.di_linear_lora_workspace(None, 1, 16, 64, 8, 1) == 0
-    assert L.di_cross_attention_workspace(None, 1, 1, 1, 1, 1, 64) == 0
+    import ctypes
+    L, cfg = dib.lib(), (ctypes.c_longlong * 18)(*([1] * 18))
+    assert L.di_linear_lora(None, 1, cfg, *([None] * 10), 0) == dib.DI_EINVAL
+    assert L.di_qk_norm_rope(None, 1, cfg, 0.0, 1.0, *([None] * 7)) == dib.DI_EINVAL
+    assert L.di_cross_attention(None, 1, cfg, 1.0, *([None] * 8), 0) == dib.DI_EINVAL
+    assert L.di_linear_lora_workspace(None, cfg) == 0 and L.di_cross_attention_workspace(None, cfg) == 0
+
+
+def test_signatures_are_told_apart(layers):
+    """The kept checks of one call are not another's: shapes, strides and types are all in the signature."""
+    x = torch.zeros(4, 64, dtype=torch.float16)
+    sigs = [layers._sig(t) for t in (x, x[:2], torch.zeros(4, 128, dtype=torch.float16)[:, :64], x.bfloat16(), x.T, None)]
+    assert len(set(sigs)) == len(sigs)
