@@ -20,7 +20,7 @@
 //   warp 1       MMA issue (the pair's first CTA)
 //   warp 2       the tile's distinct adapters and the rows of each
 //   warp 3       zeroes other adapters' rows of a T block
-//   warps 4-15   epilogue: bias, activation, residual (fetched by TMA during the main loop), stores by TMA
+//   warps 4-15   epilogue: bias, activation, residual (fetched by TMA a chunk ahead), stores by TMA
 // The accumulator is double-buffered, so a tile's epilogue runs under the next one's main loop.
 //
 // Few rows (M <= kSkinnyRows): T in 32 bits (in shared memory, with no first launch, where that is less work); the second launch streams W once from memory into mma.sync fragments (16
@@ -58,6 +58,7 @@ namespace {
 
 constexpr int kSkinnyRows = 128;
 constexpr int kEpi = 12;           // epilogue warps: three share a quarter of the rows, 32-column chunks in turn
+constexpr int kEpiPer = kEpi / 4;
 constexpr int kLThreads = 128 + 32 * kEpi, kTThreads = 256;
 constexpr int kMaxStages = 12;
 constexpr int kSlots = 32;        // adapters per list entry
@@ -73,7 +74,7 @@ struct SlotList {
 constexpr uint32_t kListBytes = (kLists * sizeof(SlotList) + 15) / 16 * 16;
 constexpr uint32_t kBarBytes = 8 * (4 * kMaxStages + 2 * kLists + 4 + kEpi * kSlabs) + 16;
 constexpr uint32_t kTFixedSmem = 1024 + kListBytes + 8 * (2 * kMaxStages + 2 * kLists + 4) + 32;
-constexpr uint32_t kFixedSmem = 1024 + kEpi * kSlabs * kSlab + kEpi * 384 + kListBytes + (kBarBytes + 15) / 16 * 16;
+constexpr uint32_t kFixedSmem = 1024 + kEpi * kSlabs * kSlab + kEpi * 256 + kListBytes + (kBarBytes + 15) / 16 * 16;
 
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
@@ -119,17 +120,46 @@ template <bool BF16>
 __device__ __forceinline__ float2 unpack2(uint32_t w) {
   return BF16 ? __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&w)) : __half22float2(*reinterpret_cast<__half2*>(&w));
 }
-// SiLU and erf GELU (erf by Abramowitz & Stegun 7.1.26, as gelu_erf) with the approximate division: the exact one's
-// branches cost four times the rest of the epilogue.
+__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
+  return (uint64_t)__float_as_uint(a) | ((uint64_t)__float_as_uint(b) << 32);
+}
+__device__ __forceinline__ float lo_f(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float hi_f(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float ex2_approx(float x) {  // 2^x; -inf -> +0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float silu_fast(float v) { return __fdividef(v, 1.0f + __expf(-v)); }
+// erf GELU of two values: v Phi(v) = max(v, 0) - |v| Phi(-|v|), and log2 Phi(-a) is so smooth that a polynomial of degree
+// 6 (minimax fit on [0, 5.5] for the error of a Phi(-a)) gives the result within 1e-7: one exponential and no
+// division per value, half the special-function work of a rational approximation.  Past 5.5 the exponent falls
+// on at a slope of 8 (the product is below 1e-7 there and stays so).
+__device__ __forceinline__ uint64_t gelu2(uint64_t v) {
+  const float v0 = lo_f(v), v1 = hi_f(v), a0 = fabsf(v0), a1 = fabsf(v1), c0 = fminf(a0, 5.5f), c1 = fminf(a1, 5.5f);
+  const uint64_t c = f2_pack(c0, c1);
+  auto k = [](float x) { return f2_pack(x, x); };
+  uint64_t q = fma2(k(3.4440247e-05f), c, k(-0.000778908085f));
+  q = fma2(q, c, k(0.00810599886f));
+  q = fma2(q, c, k(-0.0534412861f));
+  q = fma2(q, c, k(-0.458756894f));
+  q = fma2(q, c, k(-1.15120339f));
+  q = fma2(q, c, k(-0.999993265f));
+  q = fma2(f2_pack(a0 - c0, a1 - c1), k(-8.0f), q);
+  return f2_pack(fmaf(-c0, ex2_approx(lo_f(q)), fmaxf(v0, 0.f)), fmaf(-c1, ex2_approx(hi_f(q)), fmaxf(v1, 0.f)));
+}
 __device__ __forceinline__ float act_of(float v, int act) {
-  if (act == 1) return __fdividef(v, 1.0f + __expf(-v));
-  if (act == 2) {
-    const float x = v * 0.70710678f, a = fabsf(x), t = __fdividef(1.0f, fmaf(0.3275911f, a, 1.0f));
-    const float y = (((1.061405429f * t - 1.453152027f) * t + 1.421413741f) * t - 0.284496736f) * t + 0.254829592f;
-    const float e = 1.0f - y * t * __expf(-a * a);
-    return 0.5f * v * (1.0f + copysignf(e, x));
-  }
-  return v;
+  return act == 1 ? silu_fast(v) : act == 2 ? lo_f(gelu2(f2_pack(v, 0.f))) : v;
 }
 template <bool BF16>
 __device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -400,32 +430,37 @@ __global__ void __launch_bounds__(kTThreads, 1) lora_t_kernel(const __grid_const
 
 // ---- tiles: Y ----
 
-// X[m] . W[n] + T[m] . B[a][n] of one row, from its own terms: lane l returns column n0 + l.
+// Out of the way of the epilogue's instructions: the rows of `bad` of a 32 x 32 chunk again, X[m] . W[n] + T[m] . B[a][n] from
+// each row's own terms (lane l computes column n0 + l); lane `row` holds row m0 + row as pairs of columns.
 template <bool BF16>
-__device__ __noinline__ float own_terms(const LoraParams& p, int m, int n0, int lane) {
-  const int n = n0 + lane, a = __ldg(p.rows + m);
-  if (n >= p.N) return 0.f;
-  const uint16_t* x = static_cast<const uint16_t*>(p.X) + m * p.ldx;
-  const uint16_t* w = static_cast<const uint16_t*>(p.W) + (long long)n * p.K;
-  float s = 0.f;
-  for (int k = 0; k < p.K; k += 2) {
-    const float2 f = unpack2<BF16>(*reinterpret_cast<const uint32_t*>(x + k));
-    const float2 g = unpack2<BF16>(*reinterpret_cast<const uint32_t*>(w + k));
-    s = fmaf(f.x, g.x, fmaf(f.y, g.y, s));
-  }
-  if (a >= 0 && a < p.L) {
-    const int half = p.r <= 32 ? 32 : 64;
-    const uint16_t* t = p.T16 + (long long)m * p.t_ld;
-    const uint16_t* b = static_cast<const uint16_t*>(p.B) + ((long long)a * p.N + n) * p.r;
-    for (int j = 0; j < p.r; ++j) {
-      const int at = j / half * (2 * half) + j % half;
-      const float tj = unpack2<BF16>(t[at]).x + unpack2<BF16>(t[at + half]).x;
-      s = fmaf(tj, unpack2<BF16>(b[j]).x, s);
+__device__ __noinline__ void own_rows(const LoraParams& p, unsigned bad, int m0, int n0, int lane, uint64_t* v) {
+  const int n = min(n0 + lane, p.N - 1);
+  while (bad) {
+    const int row = __ffs(bad) - 1, m = m0 + row, a = __ldg(p.rows + m);
+    bad &= bad - 1;
+    const uint16_t* x = static_cast<const uint16_t*>(p.X) + m * p.ldx;
+    const uint16_t* w = static_cast<const uint16_t*>(p.W) + (long long)n * p.K;
+    float s = 0.f;
+    for (int k = 0; k < p.K; k += 2) {
+      const float2 f = unpack2<BF16>(*reinterpret_cast<const uint32_t*>(x + k));
+      const float2 g = unpack2<BF16>(*reinterpret_cast<const uint32_t*>(w + k));
+      s = fmaf(f.x, g.x, fmaf(f.y, g.y, s));
+    }
+    if (a >= 0 && a < p.L) {
+      const int half = p.r <= 32 ? 32 : 64;
+      const uint16_t* t = p.T16 + (long long)m * p.t_ld;
+      const uint16_t* b = static_cast<const uint16_t*>(p.B) + ((long long)a * p.N + n) * p.r;
+      for (int j = 0; j < p.r; ++j) {
+        const int at = j / half * (2 * half) + j % half;
+        s = fmaf(unpack2<BF16>(t[at]).x + unpack2<BF16>(t[at + half]).x, unpack2<BF16>(b[j]).x, s);
+      }
+    }
+    for (int e = 0; e < 16; ++e) {
+      const float t0 = __shfl_sync(0xffffffffu, s, 2 * e), t1 = __shfl_sync(0xffffffffu, s, 2 * e + 1);
+      if (lane == row) v[e] = f2_pack(t0, t1);
     }
   }
-  return s;
 }
-
 
 template <bool BF16, bool PAIR>
 __global__ void __launch_bounds__(kLThreads, 1) lora_tile_kernel(const __grid_constant__ LoraParams p) {
@@ -433,8 +468,8 @@ __global__ void __launch_bounds__(kLThreads, 1) lora_tile_kernel(const __grid_co
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sStage = smem;                            // [stages]: 128 rows of X or T, then rows of W or B, 128 bytes each
   uint8_t* sSlab = smem + p.stages * p.stage_bytes;  // [kEpi][kSlabs]
-  float* sBias = reinterpret_cast<float*>(sSlab + kEpi * kSlabs * kSlab);  // [kEpi][3 chunks][32]
-  SlotList* lists = reinterpret_cast<SlotList*>(sBias + kEpi * 96);
+  float* sBias = reinterpret_cast<float*>(sSlab + kEpi * kSlabs * kSlab);  // [kEpi][2][32]
+  SlotList* lists = reinterpret_cast<SlotList*>(sBias + kEpi * 64);
   uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(lists) + kListBytes);  // [kMaxStages]
   uint64_t* empty = full + kMaxStages;         // [kMaxStages]
   uint64_t* t_full = empty + kMaxStages;       // [kMaxStages] this CTA's T rows landed
@@ -684,35 +719,70 @@ __global__ void __launch_bounds__(kLThreads, 1) lora_tile_kernel(const __grid_co
     }
     if (!ok) *abort_flag = 1;
   } else {
-    const int ew = warp - 4, q = warp & 3, third = ew / 4;
+    const int ew = warp - 4, q = warp & 3, part = ew / 4;
     uint8_t* slabs = sSlab + ew * kSlabs * kSlab;
     uint64_t* rb = r_full + ew * kSlabs;
-    float* bs = sBias + ew * 96;
+    float* bs = sBias + ew * 64;
+    // The warp's chunks (32 rows by 32 columns, columns part, part + kEpiPer, ... of each tile), as one sequence over its
+    // tiles: residual and bias are fetched one chunk ahead.
+    struct Chunk {
+      int u, i, mine, m0, n0;  // tile, chunk, chunks of the tile; first row of the warp, first column of the tile
+    };
+    const int dm = step / p.nt * TM, dn = step % p.nt * p.BN, n_end = p.nt * p.BN;
+    auto chunks_of = [&](Chunk& c) {
+      c.i = 0;
+      c.mine = c.m0 < p.M ? ((min(p.BN, p.N - c.n0) + 31) / 32 - part + kEpiPer - 1) / kEpiPer : 0;
+    };
+    auto next_tile = [&](Chunk& c) {
+      c.u += step;
+      c.m0 += dm;
+      c.n0 += dn;
+      if (c.n0 >= n_end) { c.n0 -= n_end; c.m0 += TM; }
+      chunks_of(c);
+    };
+    auto to_chunk = [&](Chunk& c) {  // on to the next tile while this one has no more chunks
+      while (c.u < units && c.i >= c.mine) next_tile(c);
+    };
+    auto column = [&](const Chunk& c) { return c.n0 + (part + kEpiPer * c.i) * 32; };
+    Chunk c, f, b;  // this chunk, next residual to fetch, next bias to load
+    c.u = first;
+    c.m0 = first / p.nt * TM + rank * 128 + q * 32;
+    c.n0 = first % p.nt * p.BN;
+    chunks_of(c);
+    f = c;
+    to_chunk(f);
+    b = f;
+    unsigned fetched = 0, k = 0;  // chunks so far
+    auto fetch = [&] {
+      if (f.u >= units) return;
+      const int sl = fetched % kSlabs;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&rb[sl], kSlab);
+        tma_load_2d(slabs + sl * kSlab, &p.tmR, &rb[sl], column(f), f.m0);
+      }
+      ++fetched;
+      ++f.i;
+      to_chunk(f);
+    };
+    auto bias_of = [&] {
+      float v = 0.f;
+      if (b.u < units) {
+        const int n = column(b) + lane;
+        if (n < p.N) v = __ldg(p.bias + n);
+        ++b.i;
+        to_chunk(b);
+      }
+      return v;
+    };
     Ring li;
     unsigned r_ph = 0;  // phases of this warp's residual barriers
     bool ok = true;
     int nu = 0;
+    if (p.R) fetch();
+    float bias = p.bias ? bias_of() : 0.f;
     pdl_wait();  // this grid is not over before lora_t_kernel is
-    for (int u = first; ok && u < units; u += step, ++nu) {
-      const int ab = nu & 1, m0 = u / p.nt * TM + rank * 128 + q * 32, n0 = u % p.nt * p.BN;
-      // 32-column chunks of this warp: third, third + 3, ...
-      const int all = (min(p.BN, p.N - n0) + 31) / 32, mine = m0 < p.M ? (all - third + 2) / 3 : 0;
-      auto fetch = [&](int i) {  // residual of chunk i into its slab (free: its last store has been read)
-        mbar_arrive_expect_tx(&rb[i % kSlabs], kSlab);
-        tma_load_2d(slabs + i % kSlabs * kSlab, &p.tmR, &rb[i % kSlabs], n0 + (third + 3 * i) * 32, m0);
-      };
-      if (p.R && lane == 0 && mine > 0) {
-        bulk_wait_read0();
-        for (int i = 0; i < min(mine, kSlabs); ++i) fetch(i);
-      }
-      if (p.bias) {
-#pragma unroll
-        for (int i = 0; i < 3; ++i) {
-          const int n = n0 + (third + 3 * i) * 32 + lane;
-          if (i < mine) bs[i * 32 + lane] = n < p.N ? __ldg(p.bias + n) : 0.f;
-        }
-        __syncwarp();
-      }
+    for (; ok && c.u < units; next_tile(c), ++nu) {
+      const int ab = nu & 1;
       bool mixed = false;  // some of the tile's rows do not take its first adapter
       for (bool more = true; ok && more;) {
         ok = __all_sync(0xffffffffu, wait_on<false>(&list_full[li.s], li.ph, abort_flag, p.err, DEVERR_WAIT_EPI));
@@ -728,78 +798,84 @@ __global__ void __launch_bounds__(kLThreads, 1) lora_tile_kernel(const __grid_co
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
-      const uint32_t d = tmem + ab * 256 + (static_cast<uint32_t>(q * 32) << 16);
+      const uint32_t d = tmem + ab * 256 + part * 32 + (static_cast<uint32_t>(q * 32) << 16);
       uint32_t r[32];
-      if (mine > 0) tmem_ld32(d + third * 32, r);
+      if (c.mine > 0) tmem_ld32(d, r);
 #pragma unroll 1
-      for (int i = 0; i < mine; ++i) {
-        const int c = (third + 3 * i) * 32, nb = n0 + c, sl = i % kSlabs;
+      for (; c.i < c.mine; ++c.i, ++k) {
+        const int nb = column(c), sl = k % kSlabs;
         uint8_t* slab = slabs + sl * kSlab;
         uint4* rp = reinterpret_cast<uint4*>(slab + lane * 64);  // 64-byte rows, 64-byte swizzle
+        float* bk = bs + (k & 1) * 32;
+        if (p.bias) {
+          bk[lane] = bias;
+          bias = bias_of();
+          __syncwarp();
+        }
         tmem_wait_ld();
-        float v[32];
+        uint64_t v[16];
 #pragma unroll
-        for (int k = 0; k < 32; ++k) v[k] = __uint_as_float(r[k]);
-        if (i + 1 < mine) tmem_ld32(d + c + 96, r);  // the next chunk arrives under this one's arithmetic
+        for (int e = 0; e < 16; ++e) v[e] = f2_pack(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]));
+        if (c.i + 1 < c.mine) tmem_ld32(d + (c.i + 1) * 32 * kEpiPer, r);  // the next chunk arrives under this one's arithmetic
         if (mixed) {
-          float z = 0.f;
+          uint64_t z = 0;
 #pragma unroll
-          for (int k = 0; k < 32; ++k) z = fmaf(v[k], 0.f, z);  // NaN if any value is not finite
-          unsigned bad = __ballot_sync(0xffffffffu, z != 0.f && m0 + lane < p.M);
-          while (bad) {
-            const int row = __ffs(bad) - 1;
-            bad &= bad - 1;
-            const float own = own_terms<BF16>(p, m0 + row, nb, lane);
+          for (int e = 0; e < 16; ++e) z = fma2(v[e], 0, z);  // NaN if any value is not finite
+          const unsigned bad = __ballot_sync(0xffffffffu, lo_f(z) + hi_f(z) != 0.f && c.m0 + lane < p.M);
+          if (bad) {
+            uint64_t t[16];
 #pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const float t = __shfl_sync(0xffffffffu, own, k);
-              if (lane == row) v[k] = t;
-            }
+            for (int e = 0; e < 16; ++e) t[e] = v[e];
+            own_rows<BF16>(p, bad, c.m0, nb, lane, t);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = t[e];
           }
         }
         if (p.bias) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const float4 b = reinterpret_cast<const float4*>(bs + i * 32)[k];
-            v[4 * k] += b.x; v[4 * k + 1] += b.y; v[4 * k + 2] += b.z; v[4 * k + 3] += b.w;
+          for (int e = 0; e < 8; ++e) {
+            const ulonglong2 t = reinterpret_cast<const ulonglong2*>(bk)[e];
+            v[2 * e] = add2(v[2 * e], t.x);
+            v[2 * e + 1] = add2(v[2 * e + 1], t.y);
           }
         }
-        if (p.act) {
+        if (p.act == 1) {
 #pragma unroll
-          for (int k = 0; k < 32; ++k) v[k] = act_of(v[k], p.act);
+          for (int e = 0; e < 16; ++e) v[e] = f2_pack(silu_fast(lo_f(v[e])), silu_fast(hi_f(v[e])));
+        } else if (p.act == 2) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) v[e] = gelu2(v[e]);
         }
         if (p.R) {
-          ok = mbar_wait(&rb[sl], (r_ph >> sl) & 1, p.err, DEVERR_WAIT_EPI) && ok;
+          ok = wait_on<false>(&rb[sl], (r_ph >> sl) & 1, abort_flag, p.err, DEVERR_WAIT_EPI) && ok;
           r_ph ^= 1u << sl;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint4 t = rp[k ^ ((lane >> 1) & 3)];
+          for (int e = 0; e < 4; ++e) {
+            const uint4 t = rp[e ^ ((lane >> 1) & 3)];
             const uint32_t w[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float2 f = unpack2<BF16>(w[e]);
-              v[8 * k + 2 * e] += f.x;
-              v[8 * k + 2 * e + 1] += f.y;
+            for (int x = 0; x < 4; ++x) {
+              const float2 g = unpack2<BF16>(w[x]);
+              v[4 * e + x] = add2(v[4 * e + x], f2_pack(g.x, g.y));
             }
           }
+          // the store of the chunk before this one has read its slab: the next residual goes there
+          if (lane == 0) bulk_wait_read0();
+          fetch();
         } else {
           if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kSlabs - 1) : "memory");
           __syncwarp();  // the store that last used this slab has read it
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          rp[k ^ ((lane >> 1) & 3)] = make_uint4(pack2<BF16>(v[8 * k], v[8 * k + 1]), pack2<BF16>(v[8 * k + 2], v[8 * k + 3]),
-                                                 pack2<BF16>(v[8 * k + 4], v[8 * k + 5]),
-                                                 pack2<BF16>(v[8 * k + 6], v[8 * k + 7]));
+        for (int e = 0; e < 4; ++e)
+          rp[e ^ ((lane >> 1) & 3)] =
+              make_uint4(pack2<BF16>(lo_f(v[4 * e]), hi_f(v[4 * e])), pack2<BF16>(lo_f(v[4 * e + 1]), hi_f(v[4 * e + 1])),
+                         pack2<BF16>(lo_f(v[4 * e + 2]), hi_f(v[4 * e + 2])), pack2<BF16>(lo_f(v[4 * e + 3]), hi_f(v[4 * e + 3])));
         fence_async_smem();
         __syncwarp();
         if (lane == 0) {
-          tma_store_2d(&p.tmY, slab, nb, m0);  // rows and columns outside Y are skipped
+          tma_store_2d(&p.tmY, slab, nb, c.m0);  // rows and columns outside Y are skipped
           bulk_commit();
-          if (p.R && i + kSlabs < mine) {
-            bulk_wait_read0();
-            fetch(i + kSlabs);
-          }
         }
       }
       tc_fence_before();
@@ -813,6 +889,10 @@ __global__ void __launch_bounds__(kLThreads, 1) lora_tile_kernel(const __grid_co
       }
     }
     if (!ok) *abort_flag = 1;
+    for (; p.R && k < fetched; ++k) {  // only after giving up: residuals still on their way
+      mbar_wait(&rb[k % kSlabs], (r_ph >> (k % kSlabs)) & 1, p.err, DEVERR_WAIT_EPI);
+      r_ph ^= 1u << (k % kSlabs);
+    }
     if (lane == 0) bulk_wait0();
   }
   tc_fence_before();
