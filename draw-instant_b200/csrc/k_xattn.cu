@@ -621,45 +621,42 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
       for (int t = ta; t < w.t1; t += tstep) {
         const int left = w.n - t * KT;  // > 0; keys of this tile inside the length
         const int nc = min(KT / 32, (left + 31) / 32);
-        const bool partial = left < KT || p.mask;
-        uint32_t bits[KT / 32];
-        if (partial) {
-#pragma unroll
-          for (int c = 0; c < KT / 32; ++c) {
-            const int j = c * 32 + lane;
-            bits[c] = __ballot_sync(0xffffffffu, j < left && (!p.mask || __ldg(p.mask + (long long)w.b * p.Skv + t * KT + j)));
-          }
-        }
         ok = wait_on(&s_full[i], ph_s, abort_flag, p.err, DEVERR_WAIT_SOFTMAX);
         ok = __all_sync(0xffffffffu, ok);
         ph_s ^= 1;
         if (!ok) break;
         tc_fence_after();
         if (warp_on) {
-          // two passes over the scores in TMEM, 32 at a time: the maximum, then the exponentials
+          // Two passes over the scores in TMEM, 32 at a time: the maximum, then the exponentials.  Loops, not unrolled: the
+          // code of a tile has to stay in the instruction caches that all roles share.
           float s[32];
-          auto load = [&](int c) {
+          float mx = -INFINITY;
+          bool rewritten = false;
+#pragma unroll 1
+          for (int c = 0; c < nc; ++c) {
             tmem_ld32(tS + c * 32, reinterpret_cast<uint32_t(&)[32]>(s));
+            uint32_t bits = left - c * 32 >= 32 ? 0xffffffffu : (1u << (left - c * 32)) - 1u;
+            if (p.mask) {
+              const int j = c * 32 + lane;
+              bits = __ballot_sync(0xffffffffu, j < left && __ldg(p.mask + (long long)w.b * p.Skv + t * KT + j));
+            }
             tmem_wait_ld();
-            if (partial && bits[c] != 0xffffffffu) {
+            if (bits != 0xffffffffu) {  // masked scores go back as -inf for the second pass
 #pragma unroll
               for (int k = 0; k < 32; ++k)
-                if (!((bits[c] >> k) & 1)) s[k] = -INFINITY;
+                if (!((bits >> k) & 1)) s[k] = -INFINITY;
+              tmem_st32(tS + c * 32, reinterpret_cast<uint32_t(&)[32]>(s));
+              rewritten = true;
             }
-          };
-          float mx = -INFINITY;
+            float a = mx, b = -INFINITY;
 #pragma unroll
-          for (int c = 0; c < KT / 32; ++c)
-            if (c < nc) {
-              load(c);
-              float a = mx, b = -INFINITY;
-#pragma unroll
-              for (int k = 0; k < 32; k += 4) {
-                a = max3f(a, s[k], s[k + 1]);
-                b = max3f(b, s[k + 2], s[k + 3]);
-              }
-              mx = fmaxf(a, b);
+            for (int k = 0; k < 32; k += 4) {
+              a = max3f(a, s[k], s[k + 1]);
+              b = max3f(b, s[k + 2], s[k + 3]);
             }
+            mx = fmaxf(a, b);
+          }
+          if (rewritten) tmem_wait_st();
           mx *= p.scale_log2;  // the scale is positive
           const bool move = mx > m_run + kRescale;
           const float m_new = move ? mx : m_run;
@@ -668,27 +665,27 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
           const uint64_t nm2 = f2_pack(-m_sub, -m_sub);
           uint64_t acc[4] = {0, 0, 0, 0};
           // P of chunk c lies over the scores of chunk c / 2, which have been read again by then
+#pragma unroll 1
+          for (int c = 0; c < nc; ++c) {
+            tmem_ld32(tS + c * 32, reinterpret_cast<uint32_t(&)[32]>(s));
+            tmem_wait_ld();
+            uint32_t* w32 = reinterpret_cast<uint32_t*>(s);  // 32 scores -> 16 words of probabilities, in place
 #pragma unroll
-          for (int c = 0; c < KT / 32; ++c)
-            if (c < nc) {
-              load(c);
-              uint32_t* w32 = reinterpret_cast<uint32_t*>(s);  // 32 scores -> 16 words of probabilities, in place
-#pragma unroll
-              for (int k = 0; k < 32; k += 2) {
-                const uint64_t x = fma2(f2_pack(s[k], s[k + 1]), sc2, nm2);
-                const float a = ex2_approx(lo_f(x)), b = ex2_approx(hi_f(x));
-                acc[k / 2 % 4] = add2(acc[k / 2 % 4], f2_pack(a, b));
-                w32[k / 2] = pack2<BF16>(a, b);
-              }
-              tmem_st16(tS + c * 16, w32);
+            for (int k = 0; k < 32; k += 2) {
+              const uint64_t x = fma2(f2_pack(s[k], s[k + 1]), sc2, nm2);
+              const float a = ex2_approx(lo_f(x)), b = ex2_approx(hi_f(x));
+              acc[k / 2 % 4] = add2(acc[k / 2 % 4], f2_pack(a, b));
+              w32[k / 2] = pack2<BF16>(a, b);
             }
+            tmem_st16(tS + c * 16, w32);
+          }
           const uint64_t sum = add2(add2(acc[0], acc[1]), add2(acc[2], acc[3]));
           l_run = l_run * alpha + (lo_f(sum) + hi_f(sum));
           m_run = m_new;
           if (t != ta && __any_sync(0xffffffffu, move)) {
             // this tile's scores follow the previous P V on the tensor pipe: O is complete
             const uint64_t al2 = f2_pack(alpha, alpha);
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
               uint32_t r[32];
               tmem_ld32(tO + c * 32, r);
@@ -724,7 +721,7 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
         staged = !p.by_keys && any && warp_row + 32 <= w.rows;
         uint16_t* o = static_cast<uint16_t*>(p.O) + w.b * p.osb + (tr >> p.gps) * p.oss +
                       ((w.hg << p.gps) + (tr & (p.GP - 1))) * p.osh;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           uint32_t r[32];
           if (any) {  // warp-uniform
