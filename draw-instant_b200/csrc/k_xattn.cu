@@ -72,6 +72,7 @@ constexpr int kMaxByKeys = 256;   // requests whose key tiles are laid end to en
 template <int D, bool SHORT>
 struct XCfg {
   static constexpr int NW = SHORT ? 3 : 2;                      // groups of 128 rows
+  static constexpr int NH = SHORT ? 1 : 2, KS = KT / NH;        // P of a tile is handed over in NH parts of KS keys
   static constexpr int SW = 4 * NW;                             // softmax warps
   static constexpr int THREADS = 32 * SW + 128;
   static constexpr int TCOLS = SHORT ? 128 : 256;                    // TMEM columns of a group: S (P over it), O
@@ -79,7 +80,7 @@ struct XCfg {
   static constexpr uint32_t TILE = 128 * D * 2, HALF = 128 * 128;  // Q, K or V tile; 64 columns of it (128-byte rows)
   static constexpr uint32_t DATA = D == 64 ? 13 * 16384 : 7 * 32768;
   static constexpr int MAXRING = 10;
-  static constexpr uint32_t BARS = 8 * (2 * kQBufs * NW + 3 * MAXRING + 4 * NW + 2 * kItems) + 16 + kItems * 64;
+  static constexpr uint32_t BARS = 8 * (2 * kQBufs * NW + 3 * MAXRING + NW * NH + 3 * NW + 2 * kItems) + 16 + kItems * 64;
   static constexpr uint32_t TOTAL = 1024 + DATA + (BARS + 15) / 16 * 16 + (kMaxByKeys + 4) * 4;
   static_assert(TOTAL <= 232448, "shared memory of one CTA");
 };
@@ -113,6 +114,22 @@ __device__ __forceinline__ float ex2_approx(float x) {  // 2^x; -inf -> +0
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// Waits for tcgen05.ld; the registers it fills pass through, so that nothing reads them before.
+__device__ __forceinline__ void wait_ld(float (&s)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(s[0]), "+f"(s[1]), "+f"(s[2]), "+f"(s[3]), "+f"(s[4]), "+f"(s[5]), "+f"(s[6]), "+f"(s[7]),
+                 "+f"(s[8]), "+f"(s[9]), "+f"(s[10]), "+f"(s[11]), "+f"(s[12]), "+f"(s[13]), "+f"(s[14]), "+f"(s[15]),
+                 "+f"(s[16]), "+f"(s[17]), "+f"(s[18]), "+f"(s[19]), "+f"(s[20]), "+f"(s[21]), "+f"(s[22]), "+f"(s[23]),
+                 "+f"(s[24]), "+f"(s[25]), "+f"(s[26]), "+f"(s[27]), "+f"(s[28]), "+f"(s[29]), "+f"(s[30]), "+f"(s[31])
+               ::"memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
 }
 __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* m, uint64_t* bar, int c0, int c1, int c2,
                                             int c3, int c4) {
@@ -252,7 +269,7 @@ struct Items {
 template <bool BF16, int D, bool SHORT>
 __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const __grid_constant__ XattnParams p) {
   using C = XCfg<D, SHORT>;
-  constexpr int NW = C::NW;
+  constexpr int NW = C::NW, NH = C::NH, KS = C::KS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int qtiles = p.by_keys ? 1 : p.tpi;        // Q tiles of an item
@@ -264,8 +281,8 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
   uint64_t* kv_empty = kv_full + C::MAXRING;       // [ring]
   uint64_t* v_clean = kv_empty + C::MAXRING;       // [ring] V rows of masked keys zeroed
   uint64_t* s_full = v_clean + C::MAXRING;         // [NW] scores ready
-  uint64_t* p_full = s_full + NW;                  // [NW] probabilities written
-  uint64_t* o_full = p_full + NW;                  // [NW] O complete
+  uint64_t* p_full = s_full + NW;                  // [NW][NH] probabilities written
+  uint64_t* o_full = p_full + NW * NH;             // [NW] O complete
   uint64_t* o_read = o_full + NW;                  // [NW] O read (SHORT: the next scores may overwrite it)
   uint64_t* item_full = o_read + NW;               // [kItems]
   uint64_t* item_empty = item_full + kItems;       // [kItems]
@@ -281,7 +298,7 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
     for (int i = 0; i < p.ring; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); mbar_init(&v_clean[i], 1); }
     for (int i = 0; i < NW; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
+      for (int h = 0; h < NH; ++h) mbar_init(&p_full[i * NH + h], 4);
       mbar_init(&o_full[i], 1);
       mbar_init(&o_read[i], 4);
     }
@@ -326,272 +343,279 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
     ip.advance(kItems);
   };
 
-  if (svc == 1) {
-    if (elect_one()) {
-      tma_prefetch_desc(&p.tmQ);
-      tma_prefetch_desc(&p.tmK);
-      tma_prefetch_desc(&p.tmV);
-      RingPos kv, q;
-      unsigned nkv = 0;                // copies issued
-      unsigned q_used = 0, q_any = 0;  // Q tiles loaded, modulo 2, and at all
-      bool ok = true;
-      for (const Item* item; ok && (item = next(DEVERR_WAIT_TMA)); done()) {
-        const Item w = *item;
-        if (w.t0 >= w.t1) continue;
-        for (int i = 0; ok && i * 128 < w.rows; ++i) {
-          // a group that earlier items left out is behind: its buffer's phase has a count of its own
-          const int qi = q.s * NW + i;
-          if (!(ok = wait_on(&q_empty[qi], ((q_used >> qi) & 1) ^ 1, abort_flag, p.err, DEVERR_WAIT_TMA))) break;
-          q_used ^= 1u << qi;
-          q_any |= 1u << qi;
-          mbar_arrive_expect_tx(&q_full[qi], C::TILE);
-          for (int c = 0; c < D / 64; ++c)
-            tma_load_5d(sQ + (q.s * qtiles + i) * C::TILE + c * C::HALF, &p.tmQ, &q_full[qi], c * 64, 0,
-                        (w.row0 + i * 128) >> p.gps, w.hg * p.qh_mul, w.b * p.qb_mul);
-        }
-        q.advance(p.nq);
-        const int hk = (w.hg << p.gps) / p.G;
-        for (int t = w.t0; ok && t < w.t1; ++t)
-          for (int v = 0; v < 2; ++v) {
-            if (!(ok = wait_on(&kv_empty[kv.s], kv.ph ^ 1, abort_flag, p.err, DEVERR_WAIT_TMA))) break;
-            mbar_arrive_expect_tx(&kv_full[kv.s], C::TILE);
+  if (svc >= 0) {
+    // 8 x 216 + 4 x 72 registers a lane are the launch's 12 x 168: the scores of a whole row need them
+    if constexpr (!SHORT) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (svc == 1) {
+      if (elect_one()) {
+        tma_prefetch_desc(&p.tmQ);
+        tma_prefetch_desc(&p.tmK);
+        tma_prefetch_desc(&p.tmV);
+        RingPos kv, q;
+        unsigned nkv = 0;                // copies issued
+        unsigned q_used = 0, q_any = 0;  // Q tiles loaded, modulo 2, and at all
+        bool ok = true;
+        for (const Item* item; ok && (item = next(DEVERR_WAIT_TMA)); done()) {
+          const Item w = *item;
+          if (w.t0 >= w.t1) continue;
+          for (int i = 0; ok && i * 128 < w.rows; ++i) {
+            // a group that earlier items left out is behind: its buffer's phase has a count of its own
+            const int qi = q.s * NW + i;
+            if (!(ok = wait_on(&q_empty[qi], ((q_used >> qi) & 1) ^ 1, abort_flag, p.err, DEVERR_WAIT_TMA))) break;
+            q_used ^= 1u << qi;
+            q_any |= 1u << qi;
+            mbar_arrive_expect_tx(&q_full[qi], C::TILE);
             for (int c = 0; c < D / 64; ++c)
-              tma_load_4d(sKV + kv.s * C::TILE + c * C::HALF, v ? &p.tmV : &p.tmK, &kv_full[kv.s], c * 64, t * KT,
-                          hk * (v ? p.vh_mul : p.kh_mul), w.b * (v ? p.vb_mul : p.kb_mul));
-            kv.advance(p.ring);
-            ++nkv;
+              tma_load_5d(sQ + (q.s * qtiles + i) * C::TILE + c * C::HALF, &p.tmQ, &q_full[qi], c * 64, 0,
+                          (w.row0 + i * 128) >> p.gps, w.hg * p.qh_mul, w.b * p.qb_mul);
           }
-      }
-      if (!ok || *abort_flag) {  // leave no copy in flight behind: the last ones issued into each buffer
-        *abort_flag = 1;
-        for (unsigned i = 0; i < min(nkv, (unsigned)p.ring); ++i) {
-          kv.back(p.ring);
-          mbar_wait(&kv_full[kv.s], kv.ph, p.err, DEVERR_WAIT_TMA);
+          q.advance(p.nq);
+          const int hk = (w.hg << p.gps) / p.G;
+          for (int t = w.t0; ok && t < w.t1; ++t)
+            for (int v = 0; v < 2; ++v) {
+              if (!(ok = wait_on(&kv_empty[kv.s], kv.ph ^ 1, abort_flag, p.err, DEVERR_WAIT_TMA))) break;
+              mbar_arrive_expect_tx(&kv_full[kv.s], C::TILE);
+              for (int c = 0; c < D / 64; ++c)
+                tma_load_4d(sKV + kv.s * C::TILE + c * C::HALF, v ? &p.tmV : &p.tmK, &kv_full[kv.s], c * 64, t * KT,
+                            hk * (v ? p.vh_mul : p.kh_mul), w.b * (v ? p.vb_mul : p.kb_mul));
+              kv.advance(p.ring);
+              ++nkv;
+            }
         }
-        for (int i = 0; i < kQBufs * NW; ++i)
-          if ((q_any >> i) & 1) mbar_wait(&q_full[i], ((q_used >> i) & 1) ^ 1, p.err, DEVERR_WAIT_TMA);
+        if (!ok || *abort_flag) {  // leave no copy in flight behind: the last ones issued into each buffer
+          *abort_flag = 1;
+          for (unsigned i = 0; i < min(nkv, (unsigned)p.ring); ++i) {
+            kv.back(p.ring);
+            mbar_wait(&kv_full[kv.s], kv.ph, p.err, DEVERR_WAIT_TMA);
+          }
+          for (int i = 0; i < kQBufs * NW; ++i)
+            if ((q_any >> i) & 1) mbar_wait(&q_full[i], ((q_used >> i) & 1) ^ 1, p.err, DEVERR_WAIT_TMA);
+        }
       }
-    }
-  } else if (svc == 0) {
-    if (elect_one()) {
-      RingPos kv, q;
-      bool ok = true;
-      unsigned ph_p = 0, ph_c = 0, ph_r = 0;  // phases of p_full, v_clean, o_read, one bit each
-      unsigned used = 0;                      // groups whose O has to be read before new scores (SHORT)
-      unsigned ph_q = 0;                      // phases of q_full
-      auto wait = [&](uint64_t* b, int ph) { return wait_on(b, ph, abort_flag, p.err, DEVERR_WAIT_MMA); };
-      {
-        auto issue_s = [&](const Item& w, int i, int qt, int t, int slot) {  // qt: Q tile
-
-          if (SHORT) {
-            if ((used >> i) & 1) {
-              ok = wait(&o_read[i], (ph_r >> i) & 1);
-              ph_r ^= 1u << i;
-              tc_fence_after();
-            }
-            used |= 1u << i;
-          }
-          const uint64_t dq = kdesc(smem_u32(sQ + qt * C::TILE)), dk = kdesc(smem_u32(sKV + slot * C::TILE));
-          // the score tile is as wide as the softmax reads it: 32-key chunks
-          const int n = min((w.n - t * KT + 31) / 32, KT / 32) * 32;
-          const uint32_t id = idesc_f16(128, 0, BF16) | ((uint32_t)(n >> 3) << 17);
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk)
-            umma_f16(tmem + i * C::TCOLS, dq + ((kk / 4) * C::HALF + (kk % 4) * 32) / 16,
-                     dk + ((kk / 4) * C::HALF + (kk % 4) * 32) / 16, id, kk != 0);
-          umma_commit(&s_full[i]);
-        };
-        auto issue_pv = [&](const Item& w, int i, int t, int slot, bool first) {
-          const uint64_t dv = sdesc_sw128(0, C::HALF, 1024) | (smem_u32(sKV + slot * C::TILE) >> 4);
-          constexpr uint32_t id = idesc_f16(128, D, BF16, false, true);  // V is MN-major (d contiguous)
-          const int steps = min((w.n - t * KT + 15) / 16, KT / 16);
-#pragma unroll
-          for (int kk = 0; kk < KT / 16; ++kk)
-            if (kk < steps)
-              umma_f16_ta(tmem + i * C::TCOLS + C::TO, tmem + i * C::TCOLS + kk * 8, dv + kk * 2048 / 16, id,
-                          !first || kk != 0);
-        };
-        auto v_wait = [&](const Item& w, const RingPos& v, int t) {
-          if (!wait(&kv_full[v.s], v.ph)) return false;
-          if (cleaned(w, t)) {
-            if (!wait(&v_clean[v.s], (ph_c >> v.s) & 1)) return false;
-            ph_c ^= 1u << v.s;
-          }
-          return true;
-        };
-        auto p_wait = [&](int i) {
-          const bool r = wait(&p_full[i], (ph_p >> i) & 1);
-          ph_p ^= 1u << i;
-          tc_fence_after();
-          return r;
-        };
-        auto q_wait = [&](int i) {  // Q tile of group i of the item at q
-          const int qi = q.s * NW + i;
-          const bool r = wait(&q_full[qi], (ph_q >> qi) & 1);
-          ph_q ^= 1u << qi;
-          tc_fence_after();
-          return r;
-        };
-        auto take = [&](Item& w) {  // the next item that has keys
-          const Item* item;
-          while ((item = next(DEVERR_WAIT_MMA)) != nullptr) {
-            w = *item;
-            done();
-            if (w.t0 < w.t1) return true;
-          }
-          return false;
-        };
-        Item w, w2;
-        if (SHORT) {
-          // kv: the K tile of w, then its V tile, then the K tile of w2
-          bool have = take(w), loaded = false;
-          auto start = [&](const Item& x, int i, const RingPos& k) {  // S of group i of an item
-            if (i * 128 >= x.rows) return;
-            if (!loaded) ok = wait(&kv_full[k.s], k.ph);
-            loaded = true;
-            ok = ok && q_wait(i);
-            if (ok) issue_s(x, i, q.s * qtiles + i, 0, k.s);
-          };
-          if (have) {
-            for (int i = 0; ok && i < NW; ++i) start(w, i, kv);
-            umma_commit(&kv_empty[kv.s]);
-            q.advance(p.nq);
-          }
-          while (ok && have) {
-            const bool more = take(w2);
-            const RingPos v = kv.next(p.ring), k2 = v.next(p.ring);
-            loaded = false;
-            ok = v_wait(w, v, 0);
-            for (int i = 0; ok && i < NW; ++i) {
-              if (i * 128 < w.rows) {
-                if (!(ok = p_wait(i))) break;
-                issue_pv(w, i, 0, v.s, true);
-                umma_commit(&o_full[i]);
+    } else if (svc == 0) {
+      if (elect_one()) {
+        RingPos kv, q;
+        bool ok = true;
+        unsigned ph_p = 0, ph_c = 0, ph_r = 0;  // phases of p_full, v_clean, o_read, one bit each
+        unsigned used = 0;                      // groups whose O has to be read before new scores (SHORT)
+        unsigned ph_q = 0;                      // phases of q_full
+        auto wait = [&](uint64_t* b, int ph) { return wait_on(b, ph, abort_flag, p.err, DEVERR_WAIT_MMA); };
+        {
+          auto issue_s = [&](const Item& w, int i, int qt, int t, int slot) {  // qt: Q tile
+            if (SHORT) {
+              if ((used >> i) & 1) {
+                ok = wait(&o_read[i], (ph_r >> i) & 1);
+                ph_r ^= 1u << i;
+                tc_fence_after();
               }
-              if (more && i > 0) start(w2, i - 1, k2);
+              used |= 1u << i;
             }
-            if (!ok) break;
-            umma_commit(&kv_empty[v.s]);
-            if (more) {
-              start(w2, NW - 1, k2);
-              umma_commit(&kv_empty[k2.s]);
+            const uint64_t dq = kdesc(smem_u32(sQ + qt * C::TILE)), dk = kdesc(smem_u32(sKV + slot * C::TILE));
+            // the score tile is as wide as the softmax reads it: 32-key chunks
+            const int n = min((w.n - t * KT + 31) / 32, KT / 32) * 32;
+            const uint32_t id = idesc_f16(128, 0, BF16) | ((uint32_t)(n >> 3) << 17);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk)
+              umma_f16(tmem + i * C::TCOLS, dq + ((kk / 4) * C::HALF + (kk % 4) * 32) / 16,
+                       dk + ((kk / 4) * C::HALF + (kk % 4) * 32) / 16, id, kk != 0);
+            umma_commit(&s_full[i]);
+          };
+          auto issue_pv = [&](const Item& w, int i, int t, int h, int slot, bool first) {  // first: of the item's tiles
+            const uint64_t dv = sdesc_sw128(0, C::HALF, 1024) | (smem_u32(sKV + slot * C::TILE + h * KS * 128) >> 4);
+            constexpr uint32_t id = idesc_f16(128, D, BF16, false, true);  // V is MN-major (d contiguous)
+            const int steps = min((w.n - t * KT - h * KS + 15) / 16, KS / 16);
+#pragma unroll
+            for (int kk = 0; kk < KS / 16; ++kk)
+              if (kk < steps)
+                umma_f16_ta(tmem + i * C::TCOLS + C::TO, tmem + i * C::TCOLS + h * (KS / 2) + kk * 8, dv + kk * 2048 / 16, id,
+                            !first || h != 0 || kk != 0);
+          };
+          auto v_wait = [&](const Item& w, const RingPos& v, int t) {
+            if (!wait(&kv_full[v.s], v.ph)) return false;
+            if (cleaned(w, t)) {
+              if (!wait(&v_clean[v.s], (ph_c >> v.s) & 1)) return false;
+              ph_c ^= 1u << v.s;
+            }
+            return true;
+          };
+          auto p_wait = [&](int i, int h) {
+            const bool r = wait(&p_full[i * NH + h], (ph_p >> (i * NH + h)) & 1);
+            ph_p ^= 1u << (i * NH + h);
+            tc_fence_after();
+            return r;
+          };
+          auto q_wait = [&](int i) {  // Q tile of group i of the item at q
+            const int qi = q.s * NW + i;
+            const bool r = wait(&q_full[qi], (ph_q >> qi) & 1);
+            ph_q ^= 1u << qi;
+            tc_fence_after();
+            return r;
+          };
+          auto take = [&](Item& w) {  // the next item that has keys
+            const Item* item;
+            while ((item = next(DEVERR_WAIT_MMA)) != nullptr) {
+              w = *item;
+              done();
+              if (w.t0 < w.t1) return true;
+            }
+            return false;
+          };
+          Item w, w2;
+          if (SHORT) {
+            // kv: the K tile of w, then its V tile, then the K tile of w2
+            bool have = take(w), loaded = false;
+            auto start = [&](const Item& x, int i, const RingPos& k) {  // S of group i of an item
+              if (i * 128 >= x.rows) return;
+              if (!loaded) ok = wait(&kv_full[k.s], k.ph);
+              loaded = true;
+              ok = ok && q_wait(i);
+              if (ok) issue_s(x, i, q.s * qtiles + i, 0, k.s);
+            };
+            if (have) {
+              for (int i = 0; ok && i < NW; ++i) start(w, i, kv);
+              umma_commit(&kv_empty[kv.s]);
               q.advance(p.nq);
             }
-            kv = k2;
-            w = w2;
-            have = more;
-          }
-        } else {
-          while (ok && take(w)) {
-            const int nw = (w.rows + 127) / 128, qb = q.s * qtiles;
-            if (!p.by_keys) {
-              if ((ok = wait(&kv_full[kv.s], kv.ph))) {
-                for (int i = 0; ok && i < nw; ++i)
-                  if ((ok = q_wait(i))) issue_s(w, i, qb + i, w.t0, kv.s);
-                umma_commit(&kv_empty[kv.s]);
-              }
-              for (int t = w.t0; ok && t < w.t1; ++t) {  // kv: the K tile of t, then its V tile, then the next K tile
-                const bool more = t + 1 < w.t1;
-                const RingPos v = kv.next(p.ring), k2 = v.next(p.ring);
-                ok = v_wait(w, v, t) && (!more || wait(&kv_full[k2.s], k2.ph));
-                for (int i = 0; ok && i < nw; ++i) {
-                  if (!(ok = p_wait(i))) break;
-                  issue_pv(w, i, t, v.s, t == w.t0);
-                  if (more) issue_s(w, i, qb + i, t + 1, k2.s);
-                  else umma_commit(&o_full[i]);
+            while (ok && have) {
+              const bool more = take(w2);
+              const RingPos v = kv.next(p.ring), k2 = v.next(p.ring);
+              loaded = false;
+              ok = v_wait(w, v, 0);
+              for (int i = 0; ok && i < NW; ++i) {
+                if (i * 128 < w.rows) {
+                  if (!(ok = p_wait(i, 0))) break;
+                  issue_pv(w, i, 0, 0, v.s, true);
+                  umma_commit(&o_full[i]);
                 }
-                if (!ok) break;
-                umma_commit(&kv_empty[v.s]);
-                if (more) umma_commit(&kv_empty[k2.s]);
-                kv = k2;
+                if (more && i > 0) start(w2, i - 1, k2);
               }
-            } else {
-              // group i takes tiles t0 + i, t0 + i + NW, ...: P V of a tile, then S of the group's next one
-              ok = q_wait(0);
-              RingPos v = kv.next(p.ring);  // V tile of `t`; kv: K tile of `t + NW`
-              for (int t = w.t0 - NW; ok && t < w.t1; ++t) {
-                if (t >= w.t0) {
-                  const int i = (t - w.t0) % NW;
-                  if (!(ok = v_wait(w, v, t) && p_wait(i))) break;
-                  issue_pv(w, i, t, v.s, t - w.t0 < NW);
-                  if (t + NW >= w.t1) umma_commit(&o_full[i]);
-                  umma_commit(&kv_empty[v.s]);
-                  v = v.next(p.ring).next(p.ring);
-                }
-                if (t + NW < w.t1) {
-                  if (!(ok = wait(&kv_full[kv.s], kv.ph))) break;
-                  tc_fence_after();
-                  issue_s(w, (t + NW - w.t0) % NW, qb, t + NW, kv.s);
-                  umma_commit(&kv_empty[kv.s]);
-                  kv = kv.next(p.ring).next(p.ring);
-                }
+              if (!ok) break;
+              umma_commit(&kv_empty[v.s]);
+              if (more) {
+                start(w2, NW - 1, k2);
+                umma_commit(&kv_empty[k2.s]);
+                q.advance(p.nq);
               }
+              kv = k2;
+              w = w2;
+              have = more;
             }
-            q.advance(p.nq);
+          } else {
+            while (ok && take(w)) {
+              const int nw = (w.rows + 127) / 128, qb = q.s * qtiles;
+              if (!p.by_keys) {
+                if ((ok = wait(&kv_full[kv.s], kv.ph))) {
+                  for (int i = 0; ok && i < nw; ++i)
+                    if ((ok = q_wait(i))) issue_s(w, i, qb + i, w.t0, kv.s);
+                  umma_commit(&kv_empty[kv.s]);
+                }
+                for (int t = w.t0; ok && t < w.t1; ++t) {  // kv: the K tile of t, then its V tile, then the next K tile
+                  const bool more = t + 1 < w.t1;
+                  const RingPos v = kv.next(p.ring), k2 = v.next(p.ring);
+                  ok = v_wait(w, v, t) && (!more || wait(&kv_full[k2.s], k2.ph));
+                  for (int i = 0; ok && i < nw; ++i) {
+                    for (int h = 0; ok && h < NH; ++h)
+                      if ((ok = p_wait(i, h))) issue_pv(w, i, t, h, v.s, t == w.t0);
+                    if (!ok) break;
+                    if (more) issue_s(w, i, qb + i, t + 1, k2.s);
+                    else umma_commit(&o_full[i]);
+                  }
+                  if (!ok) break;
+                  umma_commit(&kv_empty[v.s]);
+                  if (more) umma_commit(&kv_empty[k2.s]);
+                  kv = k2;
+                }
+              } else {
+                // group i takes tiles t0 + i, t0 + i + NW, ...: P V of a tile, then S of the group's next one
+                ok = q_wait(0);
+                RingPos v = kv.next(p.ring);  // V tile of `t`; kv: K tile of `t + NW`
+                for (int t = w.t0 - NW; ok && t < w.t1; ++t) {
+                  if (t >= w.t0) {
+                    const int i = (t - w.t0) % NW;
+                    if (!(ok = v_wait(w, v, t))) break;
+                    for (int h = 0; ok && h < NH; ++h)
+                      if ((ok = p_wait(i, h))) issue_pv(w, i, t, h, v.s, t - w.t0 < NW);
+                    if (!ok) break;
+                    if (t + NW >= w.t1) umma_commit(&o_full[i]);
+                    umma_commit(&kv_empty[v.s]);
+                    v = v.next(p.ring).next(p.ring);
+                  }
+                  if (t + NW < w.t1) {
+                    if (!(ok = wait(&kv_full[kv.s], kv.ph))) break;
+                    tc_fence_after();
+                    issue_s(w, (t + NW - w.t0) % NW, qb, t + NW, kv.s);
+                    umma_commit(&kv_empty[kv.s]);
+                    kv = kv.next(p.ring).next(p.ring);
+                  }
+                }
+              }
+              q.advance(p.nq);
+            }
           }
+        }
+        if (!ok) *abort_flag = 1;
+      }
+    } else if (svc == 2) {
+      RingPos kv;
+      bool ok = true;
+      for (const Item* item; ok && (item = next(DEVERR_WAIT_SOFTMAX));) {
+        const Item w = *item;
+        __syncwarp();
+        if (lane == 0) mbar_arrive_relaxed(&item_empty[ip.s]);
+        ip.advance(kItems);
+        for (int t = w.t0; ok && t < w.t1; ++t) {
+          // every tile is waited for, cleaned or not: a wait that runs a whole ring ahead would find the phase before it
+          const RingPos k = kv, v = kv.next(p.ring);
+          kv = v.next(p.ring);
+          ok = wait_on(&kv_full[k.s], k.ph, abort_flag, p.err, DEVERR_WAIT_SOFTMAX);
+          if (!cleaned(w, t)) {
+            ok = __all_sync(0xffffffffu, ok && wait_on(&kv_full[v.s], v.ph, abort_flag, p.err, DEVERR_WAIT_SOFTMAX));
+            continue;
+          }
+          const int left = min(w.n - t * KT, KT), reach = (left + 15) / 16 * 16;  // rows that P V reads
+          uint32_t off[KT / 32];
+#pragma unroll
+          for (int c = 0; c < KT / 32; ++c) {
+            const int j = c * 32 + lane;
+            off[c] = __ballot_sync(0xffffffffu, j < reach && (j >= left || (p.mask && !__ldg(p.mask + (long long)w.b * p.Skv + t * KT + j))));
+          }
+          ok = __all_sync(0xffffffffu, ok && wait_on(&kv_full[v.s], v.ph, abort_flag, p.err, DEVERR_WAIT_SOFTMAX));
+          if (!ok) break;
+          uint4* vt = reinterpret_cast<uint4*>(sKV + v.s * C::TILE);
+#pragma unroll
+          for (int c = 0; c < KT / 32; ++c)
+            if (off[c]) {
+#pragma unroll
+              for (int k = 0; k < 8; ++k)  // four rows at a time: lane / 8 the row, lane % 8 its 16-byte piece
+                if ((off[c] >> (k * 4 + lane / 8)) & 1) {
+#pragma unroll
+                  for (int h = 0; h < D / 64; ++h) vt[h * (C::HALF / 16) + (c * 32 + k * 4) * 8 + lane] = make_uint4(0, 0, 0, 0);
+                }
+            }
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&v_clean[v.s]);
         }
       }
       if (!ok) *abort_flag = 1;
-    }
-  } else if (svc == 2) {
-    RingPos kv;
-    bool ok = true;
-    for (const Item* item; ok && (item = next(DEVERR_WAIT_SOFTMAX));) {
-      const Item w = *item;
-      __syncwarp();
-      if (lane == 0) mbar_arrive_relaxed(&item_empty[ip.s]);
-      ip.advance(kItems);
-      for (int t = w.t0; ok && t < w.t1; ++t) {
-        // every tile is waited for, cleaned or not: a wait that runs a whole ring ahead would find the phase before it
-        const RingPos k = kv, v = kv.next(p.ring);
-        kv = v.next(p.ring);
-        ok = wait_on(&kv_full[k.s], k.ph, abort_flag, p.err, DEVERR_WAIT_SOFTMAX);
-        if (!cleaned(w, t)) {
-          ok = __all_sync(0xffffffffu, ok && wait_on(&kv_full[v.s], v.ph, abort_flag, p.err, DEVERR_WAIT_SOFTMAX));
-          continue;
-        }
-        const int left = min(w.n - t * KT, KT), reach = (left + 15) / 16 * 16;  // rows that P V reads
-        uint32_t off[KT / 32];
-#pragma unroll
-        for (int c = 0; c < KT / 32; ++c) {
-          const int j = c * 32 + lane;
-          off[c] = __ballot_sync(0xffffffffu, j < reach && (j >= left || (p.mask && !__ldg(p.mask + (long long)w.b * p.Skv + t * KT + j))));
-        }
-        ok = __all_sync(0xffffffffu, ok && wait_on(&kv_full[v.s], v.ph, abort_flag, p.err, DEVERR_WAIT_SOFTMAX));
-        if (!ok) break;
-        uint4* vt = reinterpret_cast<uint4*>(sKV + v.s * C::TILE);
-#pragma unroll
-        for (int c = 0; c < KT / 32; ++c)
-          if (off[c]) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k)  // four rows at a time: lane / 8 the row, lane % 8 its 16-byte piece
-              if ((off[c] >> (k * 4 + lane / 8)) & 1) {
-#pragma unroll
-                for (int h = 0; h < D / 64; ++h) vt[h * (C::HALF / 16) + (c * 32 + k * 4) * 8 + lane] = make_uint4(0, 0, 0, 0);
-              }
+    } else if (svc == 3) {
+      if (elect_one()) {
+        Items it(p, ends);
+        for (Item w = {}; w.rows >= 0; ip.advance(kItems)) {
+          const bool more = it.next(w);
+          if (!wait_on(&item_empty[ip.s], ip.ph ^ 1, abort_flag, p.err, DEVERR_WAIT_EPI)) {
+            *abort_flag = 1;
+            break;
           }
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&v_clean[v.s]);
-      }
-    }
-    if (!ok) *abort_flag = 1;
-  } else if (svc == 3) {
-    if (elect_one()) {
-      Items it(p, ends);
-      for (Item w = {}; w.rows >= 0; ip.advance(kItems)) {
-        const bool more = it.next(w);
-        if (!wait_on(&item_empty[ip.s], ip.ph ^ 1, abort_flag, p.err, DEVERR_WAIT_EPI)) {
-          *abort_flag = 1;
-          break;
+          if (!more) w.rows = 0;
+          items[ip.s] = w;
+          mbar_arrive(&item_full[ip.s]);
+          if (!more) break;
         }
-        if (!more) w.rows = 0;
-        items[ip.s] = w;
-        mbar_arrive(&item_full[ip.s]);
-        if (!more) break;
       }
     }
   } else {
+    if constexpr (!SHORT) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // ---------------- softmax warps: one packed row per lane ----------------
     const int i = warp / 4, wq = warp & 3;
     const int lrow = wq * 32 + lane;  // row of the tile = TMEM lane
@@ -600,7 +624,7 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
     const int warp_row = p.by_keys ? wq * 32 : i * 128 + wq * 32;
     const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2);
     RingPos q;
-    int ph_s = 0, ph_o = 0;
+    unsigned ph_s = 0, ph_o = 0;
     bool ok = true;
     for (const Item* item; ok && (item = next(DEVERR_WAIT_SOFTMAX)) != nullptr;) {
       const Item& w = *item;  // read again where it is used: registers are short here
@@ -617,94 +641,142 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
       const bool mine = row < w.rows, warp_on = warp_row < w.rows;
       const int ta = p.by_keys ? w.t0 + i : w.t0, tstep = p.by_keys ? NW : 1;  // this group's key tiles
       const bool any = ta < w.t1;
-      float m_run = -INFINITY, l_run = 0.f;
-      for (int t = ta; t < w.t1; t += tstep) {
-        const int left = w.n - t * KT;  // > 0; keys of this tile inside the length
-        const int nc = min(KT / 32, (left + 31) / 32);
-        ok = wait_on(&s_full[i], ph_s, abort_flag, p.err, DEVERR_WAIT_SOFTMAX);
-        ok = __all_sync(0xffffffffu, ok);
-        ph_s ^= 1;
-        if (!ok) break;
-        tc_fence_after();
-        if (warp_on) {
-          // Two passes over the scores in TMEM, 32 at a time: the maximum, then the exponentials.  Loops, not unrolled: the
-          // code of a tile has to stay in the instruction caches that all roles share.
-          float s[32];
-          float mx = -INFINITY;
-          bool rewritten = false;
-#pragma unroll 1
-          for (int c = 0; c < nc; ++c) {
-            tmem_ld32(tS + c * 32, reinterpret_cast<uint32_t(&)[32]>(s));
-            uint32_t bits = left - c * 32 >= 32 ? 0xffffffffu : (1u << (left - c * 32)) - 1u;
-            if (p.mask) {
-              const int j = c * 32 + lane;
-              bits = __ballot_sync(0xffffffffu, j < left && __ldg(p.mask + (long long)w.b * p.Skv + t * KT + j));
-            }
-            tmem_wait_ld();
-            if (bits != 0xffffffffu) {  // masked scores go back as -inf for the second pass
-#pragma unroll
-              for (int k = 0; k < 32; ++k)
-                if (!((bits >> k) & 1)) s[k] = -INFINITY;
-              tmem_st32(tS + c * 32, reinterpret_cast<uint32_t(&)[32]>(s));
-              rewritten = true;
-            }
-            float a = mx, b = -INFINITY;
-#pragma unroll
-            for (int k = 0; k < 32; k += 4) {
-              a = max3f(a, s[k], s[k + 1]);
-              b = max3f(b, s[k + 2], s[k + 3]);
-            }
-            mx = fmaxf(a, b);
-          }
-          if (rewritten) tmem_wait_st();
-          mx *= p.scale_log2;  // the scale is positive
-          const bool move = mx > m_run + kRescale;
-          const float m_new = move ? mx : m_run;
-          const float alpha = move ? ex2_approx(m_run - m_new) : 1.0f;
-          const float m_sub = m_new == -INFINITY ? 0.f : m_new;  // no valid key yet: every p is 2^-inf = 0
-          const uint64_t nm2 = f2_pack(-m_sub, -m_sub);
-          uint64_t acc[4] = {0, 0, 0, 0};
-          // P of chunk c lies over the scores of chunk c / 2, which have been read again by then
-#pragma unroll 1
-          for (int c = 0; c < nc; ++c) {
-            tmem_ld32(tS + c * 32, reinterpret_cast<uint32_t(&)[32]>(s));
-            tmem_wait_ld();
-            uint32_t* w32 = reinterpret_cast<uint32_t*>(s);  // 32 scores -> 16 words of probabilities, in place
-#pragma unroll
-            for (int k = 0; k < 32; k += 2) {
-              const uint64_t x = fma2(f2_pack(s[k], s[k + 1]), sc2, nm2);
-              const float a = ex2_approx(lo_f(x)), b = ex2_approx(hi_f(x));
-              acc[k / 2 % 4] = add2(acc[k / 2 % 4], f2_pack(a, b));
-              w32[k / 2] = pack2<BF16>(a, b);
-            }
-            tmem_st16(tS + c * 16, w32);
-          }
-          const uint64_t sum = add2(add2(acc[0], acc[1]), add2(acc[2], acc[3]));
-          l_run = l_run * alpha + (lo_f(sum) + hi_f(sum));
-          m_run = m_new;
-          if (t != ta && __any_sync(0xffffffffu, move)) {
-            // this tile's scores follow the previous P V on the tensor pipe: O is complete
-            const uint64_t al2 = f2_pack(alpha, alpha);
-#pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t r[32];
-              tmem_ld32(tO + c * 32, r);
-              tmem_wait_ld();
-#pragma unroll
-              for (int k = 0; k < 32; k += 2) {
-                const uint64_t x = mul2(f2_pack(__uint_as_float(r[k]), __uint_as_float(r[k + 1])), al2);
-                r[k] = (uint32_t)x;
-                r[k + 1] = (uint32_t)(x >> 32);
-              }
-              tmem_st32(tO + c * 32, r);
-            }
-          }
-          tmem_wait_st();
-        }
+      float m_run = -INFINITY;
+      uint64_t acc[2] = {0, 0};  // sums of the probabilities under m_run
+      auto s_wait = [&] {
+        const bool r = wait_on(&s_full[i], ph_s, abort_flag, p.err, DEVERR_WAIT_SOFTMAX);
+        return __all_sync(0xffffffffu, r);
+      };
+      auto p_done = [&](int h) {
+        tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[i]);
+        if (lane == 0) mbar_arrive(&p_full[i * NH + h]);
+      };
+      auto mask = [&](float(&s)[32], int t, int c) {  // -inf for the keys that are masked or past the length
+        const int left = w.n - t * KT - c * 32;
+        if (__builtin_expect(left >= 32 && !p.mask, 1)) return;
+        uint32_t bits = left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1u : 0;
+        if (p.mask)
+          bits = __ballot_sync(0xffffffffu, lane < left && __ldg(p.mask + (long long)w.b * p.Skv + t * KT + c * 32 + lane));
+#pragma unroll
+        for (int k = 0; k < 32; ++k)
+          if (!((bits >> k) & 1)) s[k] = -INFINITY;
+      };
+      auto top_of = [&](float (&mx)[4], const float(&s)[32]) {
+#pragma unroll
+        for (int k = 0; k < 32; k += 2) mx[k / 2 % 4] = max3f(mx[k / 2 % 4], s[k], s[k + 1]);
+      };
+      // the tile's maximum is at hand: where it passes the one that the exponentials were taken under by more than
+      // kRescale, what was made under that one is scaled down (past an item's first tile this is rare)
+      auto rescale = [&](const float (&mx)[4], bool first) {
+        const float top = fmaxf(max3f(mx[0], mx[1], mx[2]), mx[3]) * p.scale_log2;  // the scale is positive
+        const bool move = top > m_run + kRescale;
+        if (__builtin_expect(!__any_sync(0xffffffffu, move), 1)) return;
+        const float m_new = move ? top : m_run, alpha = move ? ex2_approx(m_run - m_new) : 1.0f;
+        const uint64_t al2 = f2_pack(alpha, alpha);
+        m_run = m_new;
+        acc[0] = mul2(acc[0], al2);
+        acc[1] = mul2(acc[1], al2);
+        if (first) return;
+        // this tile's scores follow the last P V on the tensor pipe: O is complete
+#pragma unroll 1
+        for (int j = 0; j < D / 16; ++j) {
+          uint32_t r[16];
+          tmem_ld16(tO + j * 16, r);
+          tmem_wait_ld();
+#pragma unroll
+          for (int k = 0; k < 16; k += 2) {
+            const uint64_t x = mul2(f2_pack(__uint_as_float(r[k]), __uint_as_float(r[k + 1])), al2);
+            r[k] = (uint32_t)x;
+            r[k + 1] = (uint32_t)(x >> 32);
+          }
+          tmem_st16(tO + j * 16, r);
+        }
+      };
+      auto exps = [&](float(&s)[32], uint32_t tP) {  // probabilities, in place (32 scores -> 16 words) and into TMEM
+        const float m_sub = m_run == -INFINITY ? 0.f : m_run;  // no valid key yet: every p is 2^-inf = 0
+        const uint64_t nm2 = f2_pack(-m_sub, -m_sub);
+        uint32_t* w32 = reinterpret_cast<uint32_t*>(s);
+#pragma unroll
+        for (int k = 0; k < 32; k += 2) {
+          const uint64_t x = fma2(f2_pack(s[k], s[k + 1]), sc2, nm2);
+          const float a = ex2_approx(lo_f(x)), b = ex2_approx(hi_f(x));
+          acc[k / 2 % 2] = add2(acc[k / 2 % 2], f2_pack(a, b));
+          w32[k / 2] = pack2<BF16>(a, b);
+        }
+        tmem_st16(tP, w32);
+      };
+      auto load = [&](float(&s)[32], int c) { tmem_ld32(tS + c * 32, reinterpret_cast<uint32_t(&)[32]>(s)); };
+#pragma unroll 1
+      for (int t = ta; t < w.t1; t += tstep) {
+        ok = s_wait();
+        if (!ok) break;
+        tc_fence_after();
+        if constexpr (SHORT) {
+          // Two passes over the scores in TMEM, 32 at a time: the maximum, then the exponentials.  Loops, not unrolled: with
+          // three groups the code of a tile has to stay in the instruction caches that all roles share.
+          if (warp_on) {
+            const int nc = (w.n + 31) / 32;
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+            for (int c = 0; c < nc; ++c) {
+              float s[32];
+              load(s, c);
+              wait_ld(s);
+              mask(s, t, c);
+              top_of(mx, s);
+            }
+            rescale(mx, true);
+#pragma unroll 1
+            for (int c = 0; c < nc; ++c) {
+              float s[32];
+              load(s, c);
+              wait_ld(s);
+              mask(s, t, c);
+              exps(s, tS + c * 16);  // over the scores of chunk c / 2
+            }
+          }
+          p_done(0);
+        } else if (!warp_on) {
+          p_done(0);
+          p_done(1);
+        } else {
+          // The tile's scores are read once and stay in registers: every trip to TMEM costs 150 cycles, a second pass
+          // over the scores made this 4300 cycles a tile and group pair instead of 3600.  P of the tile's first half is
+          // handed over while the exponentials of the second run.
+          float s0[32], s1[32], s2[32], s3[32];
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          load(s0, 0);
+          load(s1, 1);
+          load(s2, 2);
+          load(s3, 3);
+          wait_ld(s0);
+          wait_ld(s1);
+          wait_ld(s2);
+          wait_ld(s3);
+          if (__builtin_expect(p.mask || w.n - t * KT < KT, 0)) {
+            mask(s0, t, 0);
+            mask(s1, t, 1);
+            mask(s2, t, 2);
+            mask(s3, t, 3);
+          }
+          top_of(mx, s0);
+          top_of(mx, s1);
+          top_of(mx, s2);
+          top_of(mx, s3);
+          rescale(mx, t == ta);
+          exps(s0, tS);
+          exps(s1, tS + 16);
+          p_done(0);
+          exps(s2, tS + 32);
+          exps(s3, tS + 48);
+          p_done(1);
+        }
+        ph_s ^= 1;
       }
+      const uint64_t sum = add2(acc[0], acc[1]);
+      const float l_run = lo_f(sum) + hi_f(sum);
       if (ok && any) {
         ok = wait_on(&o_full[i], ph_o, abort_flag, p.err, DEVERR_WAIT_SOFTMAX);
         ok = __all_sync(0xffffffffu, ok);
