@@ -907,23 +907,32 @@ __global__ void __launch_bounds__(kLThreads, 1) lora_tile_kernel(const __grid_co
 
 // ---- few rows ----
 
-// x . w over K values by one warp; every lane returns it.
-template <bool BF16>
-__device__ __forceinline__ float dot_k(const uint16_t* x, const uint16_t* w, int K, int lane) {
-  float s = 0.f;
-#pragma unroll 4
-  for (int k = lane * 8; k < K; k += 256) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(x + k)), v = __ldg(reinterpret_cast<const uint4*>(w + k));
-    const uint32_t uu[4] = {u.x, u.y, u.z, u.w}, vv[4] = {v.x, v.y, v.z, v.w};
+// s[j] = x . w[j] over K values by one warp, for J rows of w that lie K apart; every lane gets them.
+template <bool BF16, int J>
+__device__ __forceinline__ void dot_k(const uint16_t* x, const uint16_t* w, int K, int lane, float (&s)[J]) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 f = unpack2<BF16>(uu[e]), g = unpack2<BF16>(vv[e]);
-      s = fmaf(f.x, g.x, fmaf(f.y, g.y, s));
+  for (int j = 0; j < J; ++j) s[j] = 0.f;
+#pragma unroll(4 / J)
+  for (int k = lane * 8; k < K; k += 256) {
+    const uint4 u = __ldg(reinterpret_cast<const uint4*>(x + k));
+    uint4 v[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) v[j] = __ldg(reinterpret_cast<const uint4*>(w + (long long)j * K + k));
+    const uint32_t uu[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const uint32_t vv[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = unpack2<BF16>(uu[e]), g = unpack2<BF16>(vv[e]);
+        s[j] = fmaf(f.x, g.x, fmaf(f.y, g.y, s[j]));
+      }
     }
   }
 #pragma unroll
-  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  return s;
+  for (int o = 16; o; o >>= 1)
+#pragma unroll
+    for (int j = 0; j < J; ++j) s[j] += __shfl_xor_sync(0xffffffffu, s[j], o);
 }
 
 // T[m][j] = scale[a] * X[m] . A[a][j]: one warp per value, eight of one row to a block.
@@ -937,22 +946,22 @@ __global__ void __launch_bounds__(256) lora_shrink_kernel(const __grid_constant_
     a = -1;
   }
   if (a < 0) return;  // nothing reads this row of T
-  const float s = dot_k<BF16>(static_cast<const uint16_t*>(p.X) + m * p.ldx,
-                              static_cast<const uint16_t*>(p.A) + ((long long)a * p.r + j) * p.K, p.K, lane);
-  if (lane == 0) p.T[m * p.r + j] = __ldg(p.scale + a) * s;
+  float s[1];
+  dot_k<BF16>(static_cast<const uint16_t*>(p.X) + m * p.ldx, static_cast<const uint16_t*>(p.A) + ((long long)a * p.r + j) * p.K,
+              p.K, lane, s);
+  if (lane == 0) p.T[m * p.r + j] = __ldg(p.scale + a) * s[0];
 }
 
-// 16 columns of Y for 8 MT rows per block.  The 8 warps are KW shares of K (32-wide blocks in turn) by 8 / KW groups of
-// rows, summed in shared memory.  A lane's 16-byte loads of 8 consecutive k stand for two 16-wide MMA steps: both
+// 16 columns of Y for 8 MT rows per block.  The 8 warps take shares of K (32-wide blocks in turn), summed in shared
+// memory.  A lane's 16-byte loads of 8 consecutive k stand for two 16-wide MMA steps: both
 // operands use the same order of k.  Bound: the bytes of W and B, and from L2 those of X, which every block reads whole.
 // CLUSTER: no first launch; the eight blocks of a cluster share out the values of T, which eight more warps of each compute
 // and hand to all through distributed shared memory while the MMAs run.
 template <bool BF16, int MT, bool CLUSTER>
 __global__ void __launch_bounds__(CLUSTER ? 512 : 256) lora_skinny_kernel(const __grid_constant__ LoraParams p) {
-  constexpr int KW = MT == 8 ? 4 : 8, RT = MT * KW / 8;  // row tiles per warp
-  constexpr int ROWS = 8 * MT, COLS = 16, AHEAD = 4;
+  constexpr int KW = 8, ROWS = 8 * MT, COLS = 16, AHEAD = 8;
   __shared__ float red[KW][ROWS][COLS + 1];
-  __shared__ __align__(16) float ts[ROWS * (MT == 8 ? 40 : 128)];  // T of the rows, up to that rank
+  __shared__ __align__(16) float ts[ROWS * 128];  // T of the rows
   __shared__ int as[ROWS];                                         // their adapters
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   const int n0 = blockIdx.x * COLS, m0 = blockIdx.y * ROWS;
@@ -975,45 +984,52 @@ __global__ void __launch_bounds__(CLUSTER ? 512 : 256) lora_skinny_kernel(const 
   if (CLUSTER && warp >= 8) {
     const int n = min(ROWS, p.M - m0) * p.r;
     bool waited = false;
-    for (int v = (int)cluster_ctarank() + 8 * (warp - 8); v < n; v += 64) {
+    constexpr int J = 2;  // values of a row at a time
+    for (int v = ((int)cluster_ctarank() + 8 * (warp - 8)) * J; v < n; v += 64 * J) {
       const int m = v / p.r, a = __ldg(p.rows + m0 + m);
-      float s = 0.f;
-      if (a >= 0 && a < p.L)
-        s = __ldg(p.scale + a) * dot_k<BF16>(static_cast<const uint16_t*>(p.X) + (m0 + m) * p.ldx,
-                                             static_cast<const uint16_t*>(p.A) + ((long long)a * p.r + v % p.r) * p.K, p.K, lane);
+      float s[J] = {};
+      if (a >= 0 && a < p.L) {
+        dot_k<BF16>(static_cast<const uint16_t*>(p.X) + (m0 + m) * p.ldx,
+                    static_cast<const uint16_t*>(p.A) + ((long long)a * p.r + v % p.r) * p.K, p.K, lane, s);
+#pragma unroll
+        for (int j = 0; j < J; ++j) s[j] *= __ldg(p.scale + a);
+      }
       if (!waited) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // 1: all eight have started
       waited = true;
-      if (lane < 8)
-        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(smem_u32(ts + v), lane)), "f"(s) : "memory");
+      if (lane < 8) {
+        const uint32_t d = mapa_shared(smem_u32(ts + v), lane);
+#pragma unroll
+        for (int j = 0; j < J; ++j) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(d + 4 * j), "f"(s[j]) : "memory");
+      }
     }
     if (!waited) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   } else {
-  const int kw = warp % KW, rw = warp / KW * RT * 8;
-  float acc[RT][4] = {};
+  const int kw = warp;
+  float acc[MT][4] = {};
   const uint16_t* wp[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i)
     wp[i] = static_cast<const uint16_t*>(p.W) + (long long)min(n0 + i * 8 + lane / 4, p.N - 1) * p.K + (lane & 3) * 8;
-  const uint16_t* xp[RT];
+  const uint16_t* xp[MT];
 #pragma unroll
-  for (int t = 0; t < RT; ++t)  // rows and columns past the last are computed and not stored
-    xp[t] = static_cast<const uint16_t*>(p.X) + min(m0 + rw + t * 8 + lane / 4, p.M - 1) * p.ldx + (lane & 3) * 8;
+  for (int t = 0; t < MT; ++t)  // rows and columns past the last are computed and not stored
+    xp[t] = static_cast<const uint16_t*>(p.X) + min(m0 + t * 8 + lane / 4, p.M - 1) * p.ldx + (lane & 3) * 8;
 #pragma unroll 4
   for (int k = kw * 32; k < p.K; k += KW * 32) {
     const uint4 a0 = __ldg(reinterpret_cast<const uint4*>(wp[0] + k)), a1 = __ldg(reinterpret_cast<const uint4*>(wp[1] + k));
-    uint4 b[RT];
+    uint4 b[MT];
 #pragma unroll
-    for (int t = 0; t < RT; ++t) b[t] = __ldg(reinterpret_cast<const uint4*>(xp[t] + k));
+    for (int t = 0; t < MT; ++t) b[t] = __ldg(reinterpret_cast<const uint4*>(xp[t] + k));
     const uint32_t f0[4] = {a0.x, a1.x, a0.y, a1.y}, f1[4] = {a0.z, a1.z, a0.w, a1.w};
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
+    for (int t = 0; t < MT; ++t) {
       mma_16x8x16<BF16>(acc[t], f0, b[t].x, b[t].y);
       mma_16x8x16<BF16>(acc[t], f1, b[t].z, b[t].w);
     }
   }
 #pragma unroll
-  for (int t = 0; t < RT; ++t) {  // d[0..1]: column lane / 4, rows 2 (lane & 3) + {0, 1}; d[2..3]: column + 8
-    const int m = rw + t * 8 + (lane & 3) * 2, n = lane / 4;
+  for (int t = 0; t < MT; ++t) {  // d[0..1]: column lane / 4, rows 2 (lane & 3) + {0, 1}; d[2..3]: column + 8
+    const int m = t * 8 + (lane & 3) * 2, n = lane / 4;
     red[kw][m][n] = acc[t][0];
     red[kw][m + 1][n] = acc[t][1];
     red[kw][m][n + 8] = acc[t][2];
@@ -1023,8 +1039,8 @@ __global__ void __launch_bounds__(CLUSTER ? 512 : 256) lora_skinny_kernel(const 
   }
   if (CLUSTER) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // 2: this warp's values of T are written
   __syncthreads();
-  // One output per thread at a time, neighbours in a row: its B row in 16-byte pieces, the first AHEAD of the next output's
-  // already on their way.
+  // One output per thread at a time, neighbours in a row: its B row in pieces of AHEAD x 16 bytes, the next piece (of this
+  // output or of the thread's next one) already on its way.
   constexpr int total = ROWS * COLS;
   uint4 u[AHEAD];
   auto b_row = [&](int o) -> const uint4* {  // null: no adapter, or outside Y
@@ -1032,25 +1048,25 @@ __global__ void __launch_bounds__(CLUSTER ? 512 : 256) lora_skinny_kernel(const 
     return a >= 0 && n < p.N ? reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.B) + ((long long)a * p.N + n) * p.r)
                              : nullptr;
   };
-  auto fetch = [&](const uint4* row) {
+  const int pieces = p.r / 8;
+  auto fetch = [&](const uint4* row, int c) {
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) u[i] = row && i * 8 < p.r ? __ldg(row + i) : make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < AHEAD; ++i) u[i] = row && c + i < pieces ? __ldg(row + c + i) : make_uint4(0, 0, 0, 0);
   };
   const uint4* row = b_row(threadIdx.x);
-  fetch(row);
-  const bool shared_t = CLUSTER || ROWS * p.r <= (int)(sizeof ts / 4);
+  fetch(row, 0);
   if (CLUSTER) {
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   } else {
     pdl_wait();  // T is complete
   }
-  if (!CLUSTER && shared_t) {
+  if (!CLUSTER) {
     for (int i = threadIdx.x; i < ROWS * p.r; i += THREADS) ts[i] = m0 * p.r + i < p.M * p.r ? p.T[(long long)m0 * p.r + i] : 0.f;
     __syncthreads();
   }
   for (int o = threadIdx.x; o < total; o += THREADS) {
     const int ml = o / COLS, n = n0 + o % COLS, m = m0 + ml;
-    const float4* t = reinterpret_cast<const float4*>(shared_t ? ts + ml * p.r : p.T + (long long)m * p.r);
+    const float4* t = reinterpret_cast<const float4*>(ts + ml * p.r);
     float s = 0.f, s2 = 0.f;
     auto dot = [&](const uint4& v, const float4* t) {
       const float4 ta = t[0], tb = t[1];
@@ -1058,18 +1074,21 @@ __global__ void __launch_bounds__(CLUSTER ? 512 : 256) lora_skinny_kernel(const 
       s = fmaf(ta.x, f0.x, fmaf(ta.y, f0.y, fmaf(ta.z, f1.x, fmaf(ta.w, f1.y, s))));
       s2 = fmaf(tb.x, f2.x, fmaf(tb.y, f2.y, fmaf(tb.z, f3.x, fmaf(tb.w, f3.y, s2))));
     };
-    uint4 now[AHEAD];
+    const uint4* next = b_row(o + THREADS);
+#pragma unroll 1
+    for (int c = 0; c < pieces; c += AHEAD) {
+      uint4 now[AHEAD];
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) now[i] = u[i];
-    const uint4* mine = row;
-    row = b_row(o + THREADS);
-    fetch(row);
-    if (mine) {
+      for (int i = 0; i < AHEAD; ++i) now[i] = u[i];
+      if (c + AHEAD < pieces) fetch(row, c + AHEAD);
+      else fetch(next, 0);
+      if (row) {
 #pragma unroll
-      for (int i = 0; i < AHEAD; ++i)
-        if (i * 8 < p.r) dot(now[i], t + 2 * i);
-      for (int i = AHEAD; i * 8 < p.r; ++i) dot(__ldg(mine + i), t + 2 * i);
+        for (int i = 0; i < AHEAD; ++i)
+          if (c + i < pieces) dot(now[i], t + 2 * (c + i));
+      }
     }
+    row = next;
     if (m < p.M && n < p.N) {
 #pragma unroll
       for (int x = 0; x < KW; ++x) s += red[x][ml][o % COLS];
@@ -1082,29 +1101,37 @@ __global__ void __launch_bounds__(CLUSTER ? 512 : 256) lora_skinny_kernel(const 
   }
 }
 
-// Whether few rows run in one launch: each cluster of eight blocks (128 columns) reads the rows' adapters itself, which
-// has to stay small next to a launch (2 us against the L2 traffic of 16 MB).
-bool one_launch(long long M, long long N, long long K, long long r) {
-  return M <= 32 && M * r * K * 2 * ((N + 127) / 128) <= (16 << 20);
+// Few rows in one launch: row tiles of 8 per block, or 0 for two launches.  Each cluster of eight blocks (128 columns)
+// works out T of its rows itself; up to 12 clusters find room at once (16 took twice the time of 10).  It saves a launch,
+// 5 us of a caller's time, and costs the GPU 1 us up to 256 values of T (8 x 1280 x 1280, rank 16: 5.5 us against 4.5;
+// with 1024 values 10 against 7).
+int one_launch(long long M, long long N, long long K, long long r) {
+  const long long tiles = (M + 7) / 8, columns = (N + 127) / 128;
+  for (int mt = 1; mt <= 4; mt *= 2)
+    if (columns * ((tiles + mt - 1) / mt) <= 12) return std::min<long long>(M, 8 * mt) * r <= 256 ? mt : 0;
+  return 0;
 }
 
 template <bool BF16>
 int launch_skinny(Ctx* c, const LoraParams& p) {
   const int tiles = (p.M + 7) / 8;
-  if (one_launch(p.M, p.N, p.K, p.r)) {
-    const dim3 grid((p.N + 127) / 128 * 8);
-    auto kern = tiles == 1 ? lora_skinny_kernel<BF16, 1, true> : tiles == 2 ? lora_skinny_kernel<BF16, 2, true> : lora_skinny_kernel<BF16, 4, true>;
+  if (const int mt = one_launch(p.M, p.N, p.K, p.r)) {
+    const dim3 grid((p.N + 127) / 128 * 8, (tiles + mt - 1) / mt);
+    auto kern = mt == 1 ? lora_skinny_kernel<BF16, 1, true> : mt == 2 ? lora_skinny_kernel<BF16, 2, true> : lora_skinny_kernel<BF16, 4, true>;
     launch_k_cluster(kern, grid, 512, 0, c->stream, 8, p);
     return check_launch(c, "linear_lora");
   }
   launch_k(lora_shrink_kernel<BF16>, dim3(p.r / 8, p.M), 256, 0, c->stream, p);
   const int rc = check_launch(c, "linear_lora");
   if (rc != DI_OK) return rc;
-  auto go = [&](auto kern, int mt) { launch_k(kern, dim3(p.N / 16, (tiles + mt - 1) / mt), 256, 0, c->stream, p); };
-  if (tiles == 1) go(lora_skinny_kernel<BF16, 1, false>, 1);
-  else if (tiles == 2) go(lora_skinny_kernel<BF16, 2, false>, 2);
-  else if (tiles <= 4) go(lora_skinny_kernel<BF16, 4, false>, 4);
-  else go(lora_skinny_kernel<BF16, 8, false>, 8);
+  // Row tiles per block: up to four (eight: 128 x 4096 x 4096 60 us instead of 48), fewer while the blocks are fewer than
+  // the SMs.
+  int mt = tiles == 1 ? 1 : tiles == 2 ? 2 : 4;
+  while (mt > 1 && p.N / 16 * ((tiles + mt - 1) / mt) < c->num_sms) mt /= 2;
+  auto go = [&](auto kern) { launch_k(kern, dim3(p.N / 16, (tiles + mt - 1) / mt), 256, 0, c->stream, p); };
+  if (mt == 1) go(lora_skinny_kernel<BF16, 1, false>);
+  else if (mt == 2) go(lora_skinny_kernel<BF16, 2, false>);
+  else go(lora_skinny_kernel<BF16, 4, false>);
   return check_launch(c, "linear_lora");
 }
 
