@@ -908,7 +908,14 @@ __global__ void __launch_bounds__(128) xattn_join_kernel(const __grid_constant__
   float acc[W] = {};
   if (nt) {
     // CTA c has tiles [all c / grid, all (c + 1) / grid): the first and last that meet [g0, g1)
-    const int c0 = (int)(((g0 + 1) * p.grid - 1) / all), c1 = (int)((g1 * p.grid - 1) / all);
+    int c0, c1;
+    if (all * p.grid < 1ll << 31) {  // 32-bit divisions take a tenth of the time
+      c0 = ((int)(g0 + 1) * p.grid - 1) / (int)all;
+      c1 = ((int)g1 * p.grid - 1) / (int)all;
+    } else {
+      c0 = (int)(((g0 + 1) * p.grid - 1) / all);
+      c1 = (int)((g1 * p.grid - 1) / all);
+    }
     const float2* ml = reinterpret_cast<const float2*>(p.part + (long long)p.slots * NW * 128 * D);
     const int n = (c1 - c0 + 1) * NW;
     const long long base = ((long long)(c0 + pair) * NW) * 128 + lrow;
@@ -918,24 +925,33 @@ __global__ void __launch_bounds__(128) xattn_join_kernel(const __grid_constant__
       if (all < p.grid && all * c / p.grid == all * (c + 1) / p.grid) return make_float2(-INFINITY, 0.f);
       return ml[base + s * 128];
     };
-    for (int s = lane; s < n; s += 32) {
+    const float2 first = part_of(lane);
+    if (first.y != 0.f) m = first.x;
+    for (int s = lane + 32; s < n; s += 32) {
       const float2 v = part_of(s);
       if (v.y != 0.f) m = fmaxf(m, v.x);
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     for (int s0 = 0; s0 < n; s0 += 32) {
-      const float2 v = part_of(s0 + lane);
+      const float2 v = s0 ? part_of(s0 + lane) : first;
       const float mine = v.y != 0.f ? ex2_approx(v.x - m) : 0.f;  // NaN passes
       if (v.y != 0.f) l = fmaf(v.y, mine, l);
-      unsigned with = __ballot_sync(0xffffffffu, v.y != 0.f);
-      while (with) {
-        const int j = __ffs(with) - 1;
-        with &= with - 1;
-        const float f = __shfl_sync(0xffffffffu, mine, j);
-        const float* o = p.part + (base + (s0 + j) * 128) * D + lane * W;
+      const unsigned with = __ballot_sync(0xffffffffu, v.y != 0.f);
+      for (int j0 = 0; j0 < min(n - s0, 32); j0 += 8) {  // eight parts' loads in flight
+        uint32_t o[8][W];
 #pragma unroll
-        for (int k = 0; k < W; ++k) acc[k] = fmaf(o[k], f, acc[k]);
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t* src = reinterpret_cast<const uint32_t*>(p.part + (base + (s0 + j0 + j) * 128) * D + lane * W);
+#pragma unroll
+          for (int k = 0; k < W; ++k) o[j][k] = (with >> (j0 + j)) & 1 ? src[k] : 0u;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float f = __shfl_sync(0xffffffffu, mine, j0 + j);
+#pragma unroll
+          for (int k = 0; k < W; ++k) acc[k] = fmaf(__uint_as_float(o[j][k]), f, acc[k]);
+        }
       }
     }
 #pragma unroll
@@ -958,16 +974,6 @@ XPlan xattn_plan(const Ctx* c, int B, int H, int Hkv, int Sq, int Skv, int D) {
   if (x.GP > 128) x.GP = 128;
   x.HG = H / x.GP;
   const long long rows = (long long)Sq * x.GP, tiles = (rows + 127) / 128, nt = ((long long)Skv + KT - 1) / KT;
-  // By keys: when the row tiles leave most SMs idle and there are key tiles to share out.
-  if ((long long)B * x.HG * tiles * 2 <= c->num_sms && nt >= 4 && B <= kMaxByKeys &&
-      nt * B * x.HG * tiles < (1ll << 30)) {
-    x.by_keys = 1;
-    x.tpi = 1;
-    x.RT = (int)tiles;
-    x.grid = (int)std::min<long long>(c->num_sms, std::max<long long>(1, B * x.HG * tiles * nt / 2));
-    x.slots = x.grid + B * x.HG * x.RT;
-    return x;
-  }
   // By rows: as many row tiles per item as fill the SMs in the fewest rounds (an item costs a share of its
   // latency however many tiles it has).
   double best = 1e30;
@@ -977,6 +983,24 @@ XPlan xattn_plan(const Ctx* c, int B, int H, int Hkv, int Sq, int Skv, int D) {
     if (cost <= best) {
       best = cost;
       x.tpi = n;
+    }
+  }
+  // By keys where that is estimated to be sooner, in microseconds as measured: 5 to start and end and 1.5 for a key tile of
+  // one group, 1.9 for one of each of two that take turns; 6 more and the parts' bytes, out and in, to join them.  (112
+  // blocks of 2 rows, 4185 keys, head dim 64: 28 by keys, 56 by rows; 72 blocks of 77 rows, 513 keys: 16 and 13.)
+  const long long blocks = (long long)B * x.HG * tiles;
+  if (blocks <= c->num_sms && nt >= 4 && B <= kMaxByKeys && nt * blocks < (1ll << 30)) {
+    const int grid = (int)std::min<long long>(c->num_sms, blocks * nt / 2);
+    const double parts = (double)(grid + blocks) * 2 * std::min<long long>(rows, 128) * (D + 2) * 4;
+    const double by_rows = 5 + nt * (x.tpi == 1 ? 1.5 : 1.9) * (D == 128 ? 1.15 : 1.0);
+    const double by_keys = 11 + (double)((blocks * nt + grid - 1) / grid) * 0.95 + 2 * parts / 6.5e6;
+    if (by_keys < by_rows) {
+      x.by_keys = 1;
+      x.tpi = 1;
+      x.RT = (int)tiles;
+      x.grid = grid;
+      x.slots = grid + (int)blocks;
+      return x;
     }
   }
   x.RT = (int)((tiles + x.tpi - 1) / x.tpi);
