@@ -20,12 +20,12 @@
 //   warp 1       MMA issue (the pair's first CTA)
 //   warp 2       the tile's distinct adapters and the rows of each
 //   warp 3       zeroes other adapters' rows of a T block
-//   warps 4-15   epilogue: bias, activation, residual (fetched by TMA a chunk ahead), stores by TMA
+//   warps 4-15   epilogue: bias, activation, residual (fetched by TMA a chunk ahead), stores from registers
 // The accumulator is double-buffered, so a tile's epilogue runs under the next one's main loop.
 //
-// Few rows (M <= kSkinnyRows): T in 32 bits (in shared memory, with no first launch, where that is less work); the second launch streams W once from memory into mma.sync fragments (16
-// weight rows by 8 rows of X) and adds the rows' own B products with plain FMAs: every byte of W, A and B is
-// read about once, whoever owns it.
+// Few rows (M <= kSkinnyRows): T in 32 bits (in shared memory, with no first launch, where that is less work); the second
+// launch streams W into mma.sync fragments (16 weight rows by 8 rows of X) and adds the rows' own B products with plain
+// FMAs: every byte of W, A and B comes from memory once, whoever owns it.
 #include <algorithm>
 #include <cstring>
 
@@ -34,7 +34,7 @@
 namespace di {
 
 struct LoraParams {
-  CUtensorMap tmX, tmW, tmA, tmT, tmB, tmR, tmY;
+  CUtensorMap tmX, tmW, tmA, tmT, tmB, tmR;
   const void *X, *W, *A, *B, *R;
   void* Y;
   long long ldx, ldr, ldy;
@@ -45,6 +45,7 @@ struct LoraParams {
   int* err;
   // tiles
   int BN, stages, mt, nt;
+  int wide;             // rows of Y take 32-byte stores
   uint32_t stage_bytes;
   int tslots, tstages;  // first kernel: adapters per pass
   uint32_t tstage_bytes;
@@ -63,7 +64,7 @@ constexpr int kLThreads = 128 + 32 * kEpi, kTThreads = 256;
 constexpr int kMaxStages = 12;
 constexpr int kSlots = 32;        // adapters per list entry
 constexpr int kLists = 3;
-constexpr int kSlabs = 2;         // residual / output slabs per epilogue warp
+constexpr int kSlabs = 2;         // residual slabs per epilogue warp
 constexpr uint32_t kSlab = 2048;  // 32 x 32 16-bit values
 
 struct SlotList {
@@ -74,7 +75,7 @@ struct SlotList {
 constexpr uint32_t kListBytes = (kLists * sizeof(SlotList) + 15) / 16 * 16;
 constexpr uint32_t kBarBytes = 8 * (4 * kMaxStages + 2 * kLists + 4 + kEpi * kSlabs) + 16;
 constexpr uint32_t kTFixedSmem = 1024 + kListBytes + 8 * (2 * kMaxStages + 2 * kLists + 4) + 32;
-constexpr uint32_t kFixedSmem = 1024 + kEpi * kSlabs * kSlab + kEpi * 256 + kListBytes + (kBarBytes + 15) / 16 * 16;
+constexpr uint32_t kFixedSmem = 1024 + kEpi * 256 + kListBytes + (kBarBytes + 15) / 16 * 16;
 
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
@@ -467,8 +468,8 @@ __global__ void __launch_bounds__(kLThreads, 1) lora_tile_kernel(const __grid_co
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sStage = smem;                            // [stages]: 128 rows of X or T, then rows of W or B, 128 bytes each
-  uint8_t* sSlab = smem + p.stages * p.stage_bytes;  // [kEpi][kSlabs]
-  float* sBias = reinterpret_cast<float*>(sSlab + kEpi * kSlabs * kSlab);  // [kEpi][2][32]
+  uint8_t* sSlab = smem + p.stages * p.stage_bytes;  // [kEpi][kSlabs], with a residual
+  float* sBias = reinterpret_cast<float*>(sSlab + (p.R ? kEpi * kSlabs * kSlab : 0));  // [kEpi][2][32]
   SlotList* lists = reinterpret_cast<SlotList*>(sBias + kEpi * 64);
   uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(lists) + kListBytes);  // [kMaxStages]
   uint64_t* empty = full + kMaxStages;         // [kMaxStages]
@@ -744,42 +745,33 @@ __global__ void __launch_bounds__(kLThreads, 1) lora_tile_kernel(const __grid_co
       while (c.u < units && c.i >= c.mine) next_tile(c);
     };
     auto column = [&](const Chunk& c) { return c.n0 + (part + kEpiPer * c.i) * 32; };
-    Chunk c, f, b;  // this chunk, next residual to fetch, next bias to load
+    Chunk c, f;  // this chunk, the next one
     c.u = first;
     c.m0 = first / p.nt * TM + rank * 128 + q * 32;
     c.n0 = first % p.nt * p.BN;
     chunks_of(c);
     f = c;
     to_chunk(f);
-    b = f;
-    unsigned fetched = 0, k = 0;  // chunks so far
+    unsigned k = 0, fetched = 0, r_ph = 0;  // chunks so far, residuals fetched, phases of their barriers
+    float bias = 0.f;                       // of the next chunk
     auto fetch = [&] {
       if (f.u >= units) return;
-      const int sl = fetched % kSlabs;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&rb[sl], kSlab);
-        tma_load_2d(slabs + sl * kSlab, &p.tmR, &rb[sl], column(f), f.m0);
+      const int n = column(f);
+      if (p.bias) bias = n + lane < p.N ? __ldg(p.bias + n + lane) : 0.f;
+      if (p.R) {
+        const int sl = fetched++ % kSlabs;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&rb[sl], kSlab);
+          tma_load_2d(slabs + sl * kSlab, &p.tmR, &rb[sl], n, f.m0);
+        }
       }
-      ++fetched;
       ++f.i;
       to_chunk(f);
     };
-    auto bias_of = [&] {
-      float v = 0.f;
-      if (b.u < units) {
-        const int n = column(b) + lane;
-        if (n < p.N) v = __ldg(p.bias + n);
-        ++b.i;
-        to_chunk(b);
-      }
-      return v;
-    };
     Ring li;
-    unsigned r_ph = 0;  // phases of this warp's residual barriers
     bool ok = true;
     int nu = 0;
-    if (p.R) fetch();
-    float bias = p.bias ? bias_of() : 0.f;
+    fetch();
     pdl_wait();  // this grid is not over before lora_t_kernel is
     for (; ok && c.u < units; next_tile(c), ++nu) {
       const int ab = nu & 1;
@@ -799,24 +791,19 @@ __global__ void __launch_bounds__(kLThreads, 1) lora_tile_kernel(const __grid_co
       if (!ok) break;
       tc_fence_after();
       const uint32_t d = tmem + ab * 256 + part * 32 + (static_cast<uint32_t>(q * 32) << 16);
-      uint32_t r[32];
-      if (c.mine > 0) tmem_ld32(d, r);
 #pragma unroll 1
       for (; c.i < c.mine; ++c.i, ++k) {
-        const int nb = column(c), sl = k % kSlabs;
-        uint8_t* slab = slabs + sl * kSlab;
-        uint4* rp = reinterpret_cast<uint4*>(slab + lane * 64);  // 64-byte rows, 64-byte swizzle
+        const int nb = column(c), m = c.m0 + lane;
         float* bk = bs + (k & 1) * 32;
-        if (p.bias) {
-          bk[lane] = bias;
-          bias = bias_of();
-          __syncwarp();
-        }
+        uint32_t r[32];
+        tmem_ld32(d + c.i * 32 * kEpiPer, r);
+        if (p.bias) bk[lane] = bias;
+        fetch();  // into the slab that the chunk before this one has read
+        __syncwarp();
         tmem_wait_ld();
         uint64_t v[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) v[e] = f2_pack(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]));
-        if (c.i + 1 < c.mine) tmem_ld32(d + (c.i + 1) * 32 * kEpiPer, r);  // the next chunk arrives under this one's arithmetic
         if (mixed) {
           uint64_t z = 0;
 #pragma unroll
@@ -847,8 +834,10 @@ __global__ void __launch_bounds__(kLThreads, 1) lora_tile_kernel(const __grid_co
           for (int e = 0; e < 16; ++e) v[e] = gelu2(v[e]);
         }
         if (p.R) {
+          const int sl = k % kSlabs;
           ok = wait_on<false>(&rb[sl], (r_ph >> sl) & 1, abort_flag, p.err, DEVERR_WAIT_EPI) && ok;
           r_ph ^= 1u << sl;
+          const uint4* rp = reinterpret_cast<const uint4*>(slabs + sl * kSlab + lane * 64);  // 64-byte rows, 64-byte swizzle
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const uint4 t = rp[e ^ ((lane >> 1) & 3)];
@@ -859,23 +848,24 @@ __global__ void __launch_bounds__(kLThreads, 1) lora_tile_kernel(const __grid_co
               v[4 * e + x] = add2(v[4 * e + x], f2_pack(g.x, g.y));
             }
           }
-          // the store of the chunk before this one has read its slab: the next residual goes there
-          if (lane == 0) bulk_wait_read0();
-          fetch();
-        } else {
-          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kSlabs - 1) : "memory");
-          __syncwarp();  // the store that last used this slab has read it
         }
+        if (m < p.M) {
+          uint16_t* dst = static_cast<uint16_t*>(p.Y) + m * p.ldy + nb;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          rp[e ^ ((lane >> 1) & 3)] =
-              make_uint4(pack2<BF16>(lo_f(v[4 * e]), hi_f(v[4 * e])), pack2<BF16>(lo_f(v[4 * e + 1]), hi_f(v[4 * e + 1])),
-                         pack2<BF16>(lo_f(v[4 * e + 2]), hi_f(v[4 * e + 2])), pack2<BF16>(lo_f(v[4 * e + 3]), hi_f(v[4 * e + 3])));
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          tma_store_2d(&p.tmY, slab, nb, c.m0);  // rows and columns outside Y are skipped
-          bulk_commit();
+          for (int h = 0; h < 2; ++h)
+            if (nb + 16 * h < p.N) {
+              uint32_t t[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) t[e] = pack2<BF16>(lo_f(v[8 * h + e]), hi_f(v[8 * h + e]));
+              if (p.wide)
+                asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + 16 * h), "r"(t[0]), "r"(t[1]),
+                             "r"(t[2]), "r"(t[3]), "r"(t[4]), "r"(t[5]), "r"(t[6]), "r"(t[7])
+                             : "memory");
+              else
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                  reinterpret_cast<uint4*>(dst)[2 * h + e] = make_uint4(t[4 * e], t[4 * e + 1], t[4 * e + 2], t[4 * e + 3]);
+            }
         }
       }
       tc_fence_before();
@@ -893,7 +883,6 @@ __global__ void __launch_bounds__(kLThreads, 1) lora_tile_kernel(const __grid_co
       mbar_wait(&rb[k % kSlabs], (r_ph >> (k % kSlabs)) & 1, p.err, DEVERR_WAIT_EPI);
       r_ph ^= 1u << (k % kSlabs);
     }
-    if (lane == 0) bulk_wait0();
   }
   tc_fence_before();
   if (PAIR) cluster_sync();
@@ -1193,22 +1182,24 @@ int launch_tiles(Ctx* c, LoraParams& p) {
   }
   const int b_rows = pair ? p.BN / 2 : p.BN;
   p.stage_bytes = (16384 + b_rows * 128 + 1023) / 1024 * 1024;
-  p.stages = (int)std::min<uint32_t>(kMaxStages, (232448 - kFixedSmem) / p.stage_bytes);
-  const uint32_t smem = kFixedSmem + p.stages * p.stage_bytes;
+  const uint32_t fixed = kFixedSmem + (p.R ? kEpi * kSlabs * kSlab : 0);
+  p.stages = (int)std::min<uint32_t>(kMaxStages, (232448 - fixed) / p.stage_bytes);
+  const uint32_t smem = fixed + p.stages * p.stage_bytes;
+  p.wide = (reinterpret_cast<uintptr_t>(p.Y) & 31) == 0 && p.ldy % 16 == 0;
   p.t_ld = p.r <= 32 ? 64 : (p.r + 63) / 64 * 128;
   const CUtensorMapDataType dt = BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const uint64_t M = p.M, N = p.N, K = p.K, r = p.r, tl = p.t_ld;
-  const uint64_t xd[2] = {K, M}, wd[2] = {K, N}, td[2] = {tl, M}, bd[3] = {r, N, (uint64_t)p.L}, yd[2] = {N, M};
+  const uint64_t xd[2] = {K, M}, wd[2] = {K, N}, td[2] = {tl, M}, bd[3] = {r, N, (uint64_t)p.L};
   const uint64_t xs[1] = {(uint64_t)p.ldx * 2}, ws[1] = {K * 2}, ts[1] = {tl * 2}, bs[2] = {r * 2, N * r * 2};
-  const uint64_t rs[1] = {(uint64_t)p.ldr * 2}, ys[1] = {(uint64_t)p.ldy * 2};
-  const uint32_t xb[2] = {64, 128}, wb[2] = {64, (uint32_t)b_rows}, bb[3] = {64, (uint32_t)b_rows, 1}, yb[2] = {32, 32};
+  const uint32_t xb[2] = {64, 128}, wb[2] = {64, (uint32_t)b_rows}, bb[3] = {64, (uint32_t)b_rows, 1};
+  const uint64_t rd[2] = {N, M}, rs[1] = {(uint64_t)p.ldr * 2};
+  const uint32_t rb[2] = {32, 32};
   std::string err;
   if (!make_tmap(&p.tmX, dt, 2, p.X, xd, xs, xb, CU_TENSOR_MAP_SWIZZLE_128B, &err) ||
       !make_tmap(&p.tmW, dt, 2, p.W, wd, ws, wb, CU_TENSOR_MAP_SWIZZLE_128B, &err) ||
       !make_tmap(&p.tmT, dt, 2, p.T16, td, ts, xb, CU_TENSOR_MAP_SWIZZLE_128B, &err) ||
       !make_tmap(&p.tmB, dt, 3, p.B, bd, bs, bb, CU_TENSOR_MAP_SWIZZLE_128B, &err) ||
-      (p.R && !make_tmap(&p.tmR, dt, 2, p.R, yd, rs, yb, CU_TENSOR_MAP_SWIZZLE_64B, &err)) ||
-      !make_tmap(&p.tmY, dt, 2, p.Y, yd, ys, yb, CU_TENSOR_MAP_SWIZZLE_64B, &err))
+      (p.R && !make_tmap(&p.tmR, dt, 2, p.R, rd, rs, rb, CU_TENSOR_MAP_SWIZZLE_64B, &err)))
     return set_error(c, DI_EINVAL, "linear_lora: " + err);
   const int rp = (p.r + 15) / 16 * 16;
   p.tslots = std::max(1, std::min({p.L, kSlots, 256 / rp}));
