@@ -10,7 +10,9 @@
 // 1 KB that a warp reads and writes per step, so the arithmetic is packed (two values per instruction) and the
 // angles are taken once per token for all its heads.  A warp takes four tokens (two at D = 128) side by side and walks their
 // heads, queries then keys: a lane owns the same 8-value chunk of every head of one token, with the weights times the
-// sines and cosines of its pairs in registers, and all traffic is whole 128-byte lines.  Loads run four steps ahead.
+// sines and cosines of its pairs in registers, and all traffic is whole 128-byte lines.  Loads run four steps ahead, and
+// two steps go side by side: their shuffles and roots hide one another (65536 tokens of 5 + 5 heads of 64, fp16: 33.8 us,
+// 5.0 TB/s; one at a time 38.7.  21600 tokens of 16 + 4 heads of 128, bf16: 41.6 us, 5.3 TB/s; 45.8).
 // The angle is the product of an integer position and a 64-bit frequency in turns, reduced to half a turn in 64 bits
 // before the 32-bit sine (absolute error 2^-20.9): positions of any size keep the accuracy of position zero.
 // Sums and products are 32-bit; the result is rounded once.
@@ -75,7 +77,7 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 }
 
 template <typename T, int D, bool HALVES>
-__global__ void __launch_bounds__(32 * kQkWarps, 5) qk_norm_rope_kernel(const __grid_constant__ QkParams p) {
+__global__ void __launch_bounds__(32 * kQkWarps, HALVES ? 5 : 6) qk_norm_rope_kernel(const __grid_constant__ QkParams p) {
   constexpr int LPH = D / 8;   // lanes per head
   constexpr int TPW = 32 / LPH;  // tokens per warp
   const int lane = threadIdx.x & 31, chunk = lane % LPH;
@@ -94,15 +96,14 @@ __global__ void __launch_bounds__(32 * kQkWarps, 5) qk_norm_rope_kernel(const __
   // (halves); it takes the angles of 4 pairs, in the halves' case 4 of the 8 and the other lane the rest.
   const int pair0 = HALVES ? chunk % (LPH / 2) * 8 + chunk / (LPH / 2) * 4 : chunk * 4;
   pdl_begin();
-  // This warp's query heads and key heads, each list padded to whole blocks of kQkAhead steps: step v of the two lists
-  // laid end to end uses buffer v % kQkAhead.
+  // This warp's query heads and key heads, the queries padded to whole pairs of steps: step v of the two lists laid end to
+  // end uses buffer v % kQkAhead.
   const int q0 = min(h0, p.H[0]), nq = min(h1, p.H[0]) - q0, k0 = max(h0 - p.H[0], 0), nk = max(h1 - p.H[0], 0) - k0;
-  const int qpad = (nq + kQkAhead - 1) / kQkAhead * kQkAhead, steps = qpad + nk;
+  const int qpad = (nq + 1) / 2 * 2, steps = qpad + nk;
   const long long tt = on ? t : 0;
   const T* xq = static_cast<const T*>(p.x[0]) + tt * p.ldx[0] + (long long)q0 * D + chunk * 8;
   const T* xk = static_cast<const T*>(p.x[1]) + tt * p.ldx[1] + (long long)(k0 - qpad) * D + chunk * 8;
-  T* yq = static_cast<T*>(p.y[0]) + tt * p.ldy[0] + (long long)q0 * D + chunk * 8;
-  T* yk = static_cast<T*>(p.y[1]) + tt * p.ldy[1] + (long long)(k0 - qpad) * D + chunk * 8;
+  T* y = nullptr;  // step v of the list at hand at y + v D
   uint4 raw[kQkAhead];
   auto fetch = [&](uint4& r, int v) {
     if (on && (v < nq || (v >= qpad && v < steps))) r = *reinterpret_cast<const uint4*>((v < qpad ? xq : xk) + (long long)v * D);
@@ -141,83 +142,108 @@ __global__ void __launch_bounds__(32 * kQkWarps, 5) qk_norm_rope_kernel(const __
   // and other value times m1 and m2).
   uint64_t m1[HALVES ? 4 : 2], m2[HALVES ? 4 : 2], m3[2], m4[2];
   bool norm = false;
-  for (int v = 0; v < steps; v += kQkAhead) {
-    if (v == 0 || v == qpad) {  // on to the queries, or the keys
-      const float* wp = v < qpad ? p.w[0] : p.w[1];
-      norm = wp != nullptr;
-      float w[8];
+  auto list = [&](int l) {  // on to the queries, or the keys
+    y = static_cast<T*>(p.y[l]) + (on ? t : 0) * p.ldy[l] + (long long)(l ? k0 - qpad : q0) * D + chunk * 8;
+    const float* wp = p.w[l];
+    norm = wp != nullptr;
+    float w[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = wp ? __ldg(wp + chunk * 8 + e) : 1.f;
+    for (int e = 0; e < 8; ++e) w[e] = wp ? __ldg(wp + chunk * 8 + e) : 1.f;
 #pragma unroll
-      for (int j = 0; j < (HALVES ? 4 : 2); ++j) {
-        if (HALVES) {
-          const float sign = chunk < LPH / 2 ? -1.f : 1.f;
-          const float o0 = __shfl_xor_sync(0xffffffffu, w[2 * j], LPH / 2), o1 = __shfl_xor_sync(0xffffffffu, w[2 * j + 1], LPH / 2);
-          m1[j] = f2_pack(w[2 * j] * co[2 * j], w[2 * j + 1] * co[2 * j + 1]);
-          m2[j] = f2_pack(sign * o0 * si[2 * j], sign * o1 * si[2 * j + 1]);
-        } else {
-          const float c0 = co[2 * j], c1 = co[2 * j + 1], s0 = si[2 * j], s1 = si[2 * j + 1];
-          m1[j] = f2_pack(w[4 * j] * c0, w[4 * j + 2] * c1);
-          m2[j] = f2_pack(-w[4 * j + 1] * s0, -w[4 * j + 3] * s1);
-          m3[j] = f2_pack(w[4 * j] * s0, w[4 * j + 2] * s1);
-          m4[j] = f2_pack(w[4 * j + 1] * c0, w[4 * j + 3] * c1);
-        }
+    for (int j = 0; j < (HALVES ? 4 : 2); ++j) {
+      if (HALVES) {
+        const float sign = chunk < LPH / 2 ? -1.f : 1.f;
+        const float o0 = __shfl_xor_sync(0xffffffffu, w[2 * j], LPH / 2), o1 = __shfl_xor_sync(0xffffffffu, w[2 * j + 1], LPH / 2);
+        m1[j] = f2_pack(w[2 * j] * co[2 * j], w[2 * j + 1] * co[2 * j + 1]);
+        m2[j] = f2_pack(sign * o0 * si[2 * j], sign * o1 * si[2 * j + 1]);
+      } else {
+        const float c0 = co[2 * j], c1 = co[2 * j + 1], s0 = si[2 * j], s1 = si[2 * j + 1];
+        m1[j] = f2_pack(w[4 * j] * c0, w[4 * j + 2] * c1);
+        m2[j] = f2_pack(-w[4 * j + 1] * s0, -w[4 * j + 3] * s1);
+        m3[j] = f2_pack(w[4 * j] * s0, w[4 * j + 2] * s1);
+        m4[j] = f2_pack(w[4 * j + 1] * c0, w[4 * j + 3] * c1);
       }
     }
-    T* y = v < qpad ? yq : yk;
-    const int left = (v < qpad ? nq : steps) - v;
+  };
+  // N steps side by side: their chains of shuffles hide one another.
+  auto work = [&](auto count, uint4* r, int v) {
+    constexpr int N = decltype(count)::value;
+    uint64_t x[N][4], r2[N];
 #pragma unroll
-    for (int u = 0; u < kQkAhead; ++u) {
-      const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-      fetch(raw[u], v + u + kQkAhead);
-      if (u >= left) continue;  // warp-uniform
-      uint64_t x[4];
+    for (int n = 0; n < N; ++n) {
+      const uint32_t w[4] = {r[n].x, r[n].y, r[n].z, r[n].w};
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const float2 f = unpack2<T>(w[2 * j]), g = unpack2<T>(w[2 * j + 1]);
-        x[2 * j] = HALVES ? f2_pack(f.x, f.y) : f2_pack(f.x, g.x);
-        x[2 * j + 1] = HALVES ? f2_pack(g.x, g.y) : f2_pack(f.y, g.y);
+        x[n][2 * j] = HALVES ? f2_pack(f.x, f.y) : f2_pack(f.x, g.x);
+        x[n][2 * j + 1] = HALVES ? f2_pack(g.x, g.y) : f2_pack(f.y, g.y);
       }
-      uint64_t r2 = f2_pack(1.f, 1.f);
-      if (norm) {
-        const uint64_t q = fma2(x[0], x[0], fma2(x[1], x[1], fma2(x[2], x[2], mul2(x[3], x[3]))));
-        float ss = lo_f(q) + hi_f(q);
+    }
+    fetch(r[0], v + kQkAhead);
+    fetch(r[1], v + kQkAhead + 1);
+    if (norm) {
+      float ss[N];
 #pragma unroll
-        for (int o = LPH / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float r = rsqrtf(fmaf(ss, 1.0f / D, p.eps));
-        r2 = f2_pack(r, r);
+      for (int n = 0; n < N; ++n) {
+        const uint64_t q = fma2(x[n][0], x[n][0], fma2(x[n][1], x[n][1], fma2(x[n][2], x[n][2], mul2(x[n][3], x[n][3]))));
+        ss[n] = lo_f(q) + hi_f(q);
       }
+#pragma unroll
+      for (int o = LPH / 2; o; o >>= 1)
+#pragma unroll
+        for (int n = 0; n < N; ++n) ss[n] += __shfl_xor_sync(0xffffffffu, ss[n], o);
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const float s = rsqrtf(fmaf(ss[n], 1.0f / D, p.eps));
+        r2[n] = f2_pack(s, s);
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < N; ++n) r2[n] = f2_pack(1.f, 1.f);
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
       uint32_t out[4];
       if (HALVES) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          uint64_t z = mul2(x[j], m1[j]);
+          uint64_t z = mul2(x[n][j], m1[j]);
           if (p.pos) {
-            const uint64_t o = f2_pack(__shfl_xor_sync(0xffffffffu, lo_f(x[j]), LPH / 2),
-                                       __shfl_xor_sync(0xffffffffu, hi_f(x[j]), LPH / 2));
+            const uint64_t o = f2_pack(__shfl_xor_sync(0xffffffffu, lo_f(x[n][j]), LPH / 2),
+                                       __shfl_xor_sync(0xffffffffu, hi_f(x[n][j]), LPH / 2));
             z = fma2(o, m2[j], z);
           }
-          z = mul2(z, r2);
+          z = mul2(z, r2[n]);
           out[j] = pack2<T>(lo_f(z), hi_f(z));
         }
       } else {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const uint64_t f = x[2 * j], g = x[2 * j + 1];
+          const uint64_t f = x[n][2 * j], g = x[n][2 * j + 1];
           uint64_t f1 = mul2(f, m1[j]), g1 = mul2(g, m4[j]);
           if (p.pos) {
             f1 = fma2(g, m2[j], f1);
             g1 = fma2(f, m3[j], g1);
           }
-          f1 = mul2(f1, r2);
-          g1 = mul2(g1, r2);
+          f1 = mul2(f1, r2[n]);
+          g1 = mul2(g1, r2[n]);
           out[2 * j] = pack2<T>(lo_f(f1), lo_f(g1));
           out[2 * j + 1] = pack2<T>(hi_f(f1), hi_f(g1));
         }
       }
-      if (on) *reinterpret_cast<uint4*>(y + (long long)(v + u) * D) = make_uint4(out[0], out[1], out[2], out[3]);
+      if (on) *reinterpret_cast<uint4*>(y + (long long)(v + n) * D) = make_uint4(out[0], out[1], out[2], out[3]);
     }
-  }
+  };
+#pragma unroll 1
+  for (int v0 = 0; v0 < steps; v0 += kQkAhead)
+#pragma unroll
+    for (int u = 0; u < kQkAhead; u += 2) {
+      const int v = v0 + u, left = (v < qpad ? nq : steps) - v;
+      if (left <= 0) break;  // past the keys
+      if (v == 0 || v == qpad) list(v >= qpad);
+      if (left >= 2) work(std::integral_constant<int, 2>(), raw + u, v);
+      else work(std::integral_constant<int, 1>(), raw + u, v);
+    }
 }
 
 template <typename T, int D>
