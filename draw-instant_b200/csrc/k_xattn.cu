@@ -83,6 +83,8 @@ struct XCfg {
   static constexpr uint32_t BARS = 8 * (2 * kQBufs * NW + 3 * MAXRING + NW * NH + 3 * NW + 2 * kItems) + 16 + kItems * 64;
   static constexpr uint32_t TOTAL = 1024 + DATA + (BARS + 15) / 16 * 16 + (kMaxByKeys + 4) * 4;
   static_assert(TOTAL <= 232448, "shared memory of one CTA");
+  // Registers a lane once the roles have shared them out (two groups): the scores of a whole row stay in them.
+  static constexpr int SOFT_REGS = 216, SERVICE_REGS = 72;
 };
 
 __device__ __forceinline__ uint64_t f2_pack(float a, float b) {
@@ -344,8 +346,7 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
   };
 
   if (svc >= 0) {
-    // 8 x 216 + 4 x 72 registers a lane are the launch's 12 x 168: the scores of a whole row need them
-    if constexpr (!SHORT) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if constexpr (!SHORT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::SERVICE_REGS));
     if (svc == 1) {
       if (elect_one()) {
         tma_prefetch_desc(&p.tmQ);
@@ -615,7 +616,7 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
       }
     }
   } else {
-    if constexpr (!SHORT) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    if constexpr (!SHORT) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::SOFT_REGS));
     // ---------------- softmax warps: one packed row per lane ----------------
     const int i = warp / 4, wq = warp & 3;
     const int lrow = wq * 32 + lane;  // row of the tile = TMEM lane
@@ -632,6 +633,7 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
       ip.advance(kItems);
       const bool keys = w.t0 < w.t1;  // the item has a Q tile
       uint8_t* stage = sQ + (q.s * qtiles + (p.by_keys ? 0 : i)) * C::TILE + wq * 4096;
+      const RingPos at = q;
       uint64_t* q_done = &q_empty[q.s * NW + (p.by_keys ? 0 : i)];
       if (keys) q.advance(p.nq);
       if (!p.by_keys && i * 128 >= w.rows) {
@@ -858,6 +860,12 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
       } else if (SHORT && any && lane == 0) {
         mbar_arrive_relaxed(&o_read[i]);
       }
+      // By keys all groups release the one Q tile.  A group without a key tile waits until it has landed: running ahead, it
+      // would release the buffer's next tile in another group's place.
+      if (p.by_keys && keys && !any) {
+        ok = __all_sync(0xffffffffu, wait_on(&q_full[at.s * NW], at.ph, abort_flag, p.err, DEVERR_WAIT_SOFTMAX));
+        if (!ok) break;
+      }
       tc_fence_before();  // O is read before the next item's first P V, which waits for this warp's p_full
       __syncwarp();
       if (lane == 0) {
@@ -1015,6 +1023,11 @@ int launch_xattn(Ctx* c, XattnParams& p) {
   if (!(attr_done & (1u << (c->device & 31)))) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::TOTAL) != cudaSuccess)
       return cudaGetLastError(), set_error(c, DI_ECUDA, "cross_attention: shared memory attribute");
+    // the softmax warps' registers come out of the launch's: too few would leave them waiting for more
+    cudaFuncAttributes a = {};
+    if (!SHORT && (cudaFuncGetAttributes(&a, kern) != cudaSuccess ||
+                   a.numRegs * C::THREADS < 32 * (C::SW * C::SOFT_REGS + 4 * C::SERVICE_REGS)))
+      return cudaGetLastError(), set_error(c, DI_ECUDA, "cross_attention: built with too few registers");
     attr_done |= 1u << (c->device & 31);
   }
   const int qtiles = p.by_keys ? 1 : p.tpi;

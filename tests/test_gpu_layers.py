@@ -100,6 +100,8 @@ LORA = [  # M, K, N, r, L
     (1, 64, 16, 8, 1), (1, 1280, 1280, 16, 4), (2, 320, 48, 24, 3), (7, 1024, 4096, 64, 9), (8, 1280, 320, 16, 8),
     (16, 640, 640, 128, 5), (33, 192, 176, 40, 33), (64, 1024, 1024, 32, 64), (65, 640, 208, 16, 3),
     (127, 320, 320, 8, 20), (128, 320, 320, 64, 2), (129, 1280, 336, 128, 40), (300, 704, 960, 48, 7),
+    (9, 64, 16, 128, 2), (12, 640, 1536, 16, 4), (13, 640, 1552, 16, 4), (25, 320, 1568, 64, 1), (32, 128, 384, 8, 5),
+    (44, 1408, 192, 128, 3), (106, 64, 256, 64, 2), (128, 64, 4096, 128, 7),
     (1001, 1024, 4096, 64, 6), (2048, 320, 640, 104, 16), (4097, 128, 32, 16, 2), (20000, 320, 320, 32, 8)]
 
 
@@ -191,6 +193,19 @@ def test_lora_strided_rows_in_place_residual_and_surroundings(ctx, layers, M):
     around = hold.clone()
     around[1:-1, 32:368] = 5.0
     assert (around == 5.0).all()
+
+
+@pytest.mark.parametrize("M", [40, 300])
+@pytest.mark.parametrize("ld,at", [(344, 0), (352, 8), (352, 16)])
+def test_lora_rows_on_16_bytes(ctx, layers, M, ld, at):
+    """Output and residual rows that start on 16 bytes, but not on 32."""
+    s = lora_case(10, M, 320, 336, 16, 3, torch.bfloat16, res=True)
+    hold, held = torch.zeros(M, ld, dtype=torch.bfloat16, device="cuda"), torch.zeros(M, ld, dtype=torch.bfloat16, device="cuda")
+    at = min(at, ld - 336)
+    held[:, at:at + 336] = s["residual"]
+    ref = lora_ref(s, "silu")
+    check(layers.linear_lora(ctx, **{**s, "residual": held[:, at:at + 336]}, act="silu", out=hold[:, at:at + 336]), *ref)
+    assert (hold[:, :at] == 0).all() and (hold[:, at + 336:] == 0).all()
 
 
 @pytest.mark.parametrize("M", [12, 1000])
@@ -395,7 +410,8 @@ CROSS = [  # B, Sq, Skv, H, Hkv, D
     (1, 1, 1, 1, 1, 64), (1, 1, 1, 1, 1, 128), (2, 1, 77, 5, 5, 64), (3, 1, 1000, 8, 1, 128), (2, 3, 4097, 6, 2, 64),
     (2, 64, 64, 2, 2, 64), (2, 65, 63, 3, 3, 128), (2, 127, 128, 4, 4, 64), (1, 129, 129, 4, 2, 128), (2, 333, 231, 10, 10, 64),
     (16, 128, 77, 5, 5, 64), (2, 1024, 77, 10, 10, 64), (1, 4096, 20, 5, 5, 64), (1, 500, 2000, 6, 2, 128), (1, 1000, 1, 4, 4, 64),
-    (4, 17, 515, 24, 8, 64), (5, 2, 300, 7, 7, 64), (1, 100, 192, 9, 3, 64), (2, 640, 256, 2, 2, 128)]
+    (4, 17, 515, 24, 8, 64), (5, 2, 300, 7, 7, 64), (1, 100, 192, 9, 3, 64), (2, 640, 256, 2, 2, 128),
+    (16, 2, 1500, 7, 7, 64), (3, 400, 1700, 8, 1, 64), (7, 77, 1600, 3, 3, 128), (74, 1, 600, 2, 1, 64), (1, 2000, 700, 8, 2, 128)]
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
@@ -476,6 +492,24 @@ def test_cross_large_scores(ctx, layers, Sq, Skv):
     check(layers.cross_attention(ctx, q, k, v), *cross_ref(q, k, v))
 
 
+@pytest.mark.parametrize("Sq,Skv", [(1, 3000), (3, 200), (300, 700), (260, 1290), (130, 128)])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("order", ["rising", "falling", "saw"])
+def test_cross_maximum_moves_in_every_tile(ctx, layers, Sq, Skv, D, order):
+    """Scores that rise by some 12 per 128 keys: what was summed before is scaled down again and again."""
+    g = gen(16)
+    q, k, v = normal(g, 2, Sq, 2, D, scale=0.5), normal(g, 2, Skv, 2, D), normal(g, 2, Skv, 2, D)
+    at = torch.arange(Skv, device="cuda").float()
+    ramp = {"rising": at, "falling": Skv - at, "saw": at + (at % 128 < 40) * 300}[order] * 0.1
+    q[..., 0] = 16.0
+    k[..., 0] = (ramp * D ** 0.5 / 16)[None, :, None].half()
+    check(layers.cross_attention(ctx, q, k, v), *cross_ref(q, k, v))
+    lens = torch.tensor([Skv, max(1, Skv - 70)], dtype=torch.int32, device="cuda")
+    mask = torch.rand(2, Skv, generator=g, device="cuda") < 0.5
+    check(layers.cross_attention(ctx, q, k, v, kv_len=lens, key_mask=mask), *cross_ref(q, k, v, lens, None, mask))
+    assert ctx.fault() == 0
+
+
 @pytest.mark.parametrize("Sq,Skv", [(1, 3000), (40, 77), (300, 600)])
 def test_cross_repeats_bit_for_bit(ctx, layers, Sq, Skv):
     g = gen(12)
@@ -496,6 +530,20 @@ def test_cross_back_to_back(ctx, layers, B, Sq, Skv, G, Hkv, D):
     check(outs[0], *cross_ref(q, k, v, lens))
     for o in outs[1:]:
         assert torch.equal(o, outs[0])
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens", [[1500, 100] * 8, [100] * 15 + [1500], [1500, 1, 0, 128, 1500, 130, 64, 1500] * 2])
+def test_cross_keys_of_one_tile_in_a_row(ctx, layers, lens, D):
+    """Keys shared out over the card, some requests with a single tile for each of their heads: only one of a block's groups
+    of warps has work, many times in a row."""
+    g = gen(17)
+    q, k, v = normal(g, 16, 2, 7, D), normal(g, 16, 1500, 7, D), normal(g, 16, 1500, 7, D)
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    outs = [layers.cross_attention(ctx, q, k, v, kv_len=n) for _ in range(5)]
+    for o in outs:
+        check(o, *cross_ref(q, k, v, n))
+    assert ctx.fault() == 0
 
 
 @pytest.mark.parametrize("Sq", [1, 140])
