@@ -32,8 +32,8 @@
 // 24.2 us.  Neither memory nor the tensor pipe is full: a tile's k blocks, T blocks, zeroing and epilogue hand over to one
 // another some ten times, 150 to 300 ns each (without the epilogue the first takes 29.6 us, with a quarter of the MMAs
 // 40.8).  T as a second kernel's work costs 2.5 to 9 us.
-// Few rows: 8 x 1280 x 1280, rank 16: 4.6 us; 64 x 1024 x 4096, rank 32, 64 adapters: 14.1 us, 1.9 TB/s; bound by the
-// latency of one pass (two launches, one batch of loads each) and, towards 128 rows, by X from L2 for every 16 columns.
+// Few rows: 8 x 1280 x 1280, rank 16: 4.6 us; 64 x 1024 x 4096, rank 32, 64 adapters: 12.6 us, 2.1 TB/s; bound by the
+// latency of one pass (two launches, one batch of loads each) and, towards 128 rows, by X from L2 for every 32 columns.
 #include <algorithm>
 #include <cstring>
 
@@ -806,8 +806,8 @@ __global__ void __launch_bounds__(kLThreads, 1) lora_tile_kernel(const __grid_co
         uint32_t r[32];
         tmem_ld32(d + c.i * 32 * kEpiPer, r);
         if (p.bias) bk[lane] = bias;
-        fetch();  // into the slab that the chunk before this one has read
         __syncwarp();
+        fetch();  // into the slab that the chunk before this one has read
         tmem_wait_ld();
         uint64_t v[16];
 #pragma unroll
@@ -949,16 +949,16 @@ __global__ void __launch_bounds__(256) lora_shrink_kernel(const __grid_constant_
   if (lane == 0) p.T[m * p.r + j] = __ldg(p.scale + a) * s[0];
 }
 
-// 16 columns of Y for 8 MT rows per block.  The 8 warps take shares of K (32-wide blocks in turn), summed in shared
+// 16 NT columns of Y for 8 MT rows per block.  The 8 warps take shares of K (32-wide blocks in turn), summed in shared
 // memory.  A lane's 16-byte loads of 8 consecutive k stand for two 16-wide MMA steps: both
 // operands use the same order of k.  Bound: the bytes of W and B, and from L2 those of X, which every block reads whole.
 // CLUSTER: no first launch; the eight blocks of a cluster share out the values of T, which eight more warps of each compute
 // and hand to all through distributed shared memory while the MMAs run.
-template <bool BF16, int MT, bool CLUSTER>
+template <bool BF16, int MT, bool CLUSTER, int NT = 1>
 __global__ void __launch_bounds__(CLUSTER ? 512 : 256) lora_skinny_kernel(const __grid_constant__ LoraParams p) {
-  constexpr int KW = 8, ROWS = 8 * MT, COLS = 16, AHEAD = 8;
+  constexpr int KW = 8, ROWS = 8 * MT, COLS = 16 * NT, AHEAD = 8, RANK = NT > 1 ? 64 : 128;
   __shared__ float red[KW][ROWS][COLS + 1];
-  __shared__ __align__(16) float ts[ROWS * 128];  // T of the rows
+  __shared__ __align__(16) float ts[ROWS * RANK];  // T of the rows
   __shared__ int as[ROWS];                                         // their adapters
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   const int n0 = blockIdx.x * COLS, m0 = blockIdx.y * ROWS;
@@ -1002,36 +1002,43 @@ __global__ void __launch_bounds__(CLUSTER ? 512 : 256) lora_skinny_kernel(const 
     if (!waited) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   } else {
   const int kw = warp;
-  float acc[MT][4] = {};
-  const uint16_t* wp[2];
+  float acc[NT][MT][4] = {};
+  const uint16_t* wp[2 * NT];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < 2 * NT; ++i)
     wp[i] = static_cast<const uint16_t*>(p.W) + (long long)min(n0 + i * 8 + lane / 4, p.N - 1) * p.K + (lane & 3) * 8;
   const uint16_t* xp[MT];
 #pragma unroll
   for (int t = 0; t < MT; ++t)  // rows and columns past the last are computed and not stored
     xp[t] = static_cast<const uint16_t*>(p.X) + min(m0 + t * 8 + lane / 4, p.M - 1) * p.ldx + (lane & 3) * 8;
-#pragma unroll 4
+#pragma unroll (NT > 1 ? 2 : 4)
   for (int k = kw * 32; k < p.K; k += KW * 32) {
-    const uint4 a0 = __ldg(reinterpret_cast<const uint4*>(wp[0] + k)), a1 = __ldg(reinterpret_cast<const uint4*>(wp[1] + k));
-    uint4 b[MT];
+    uint4 a[2 * NT], b[MT];
+#pragma unroll
+    for (int i = 0; i < 2 * NT; ++i) a[i] = __ldg(reinterpret_cast<const uint4*>(wp[i] + k));
 #pragma unroll
     for (int t = 0; t < MT; ++t) b[t] = __ldg(reinterpret_cast<const uint4*>(xp[t] + k));
-    const uint32_t f0[4] = {a0.x, a1.x, a0.y, a1.y}, f1[4] = {a0.z, a1.z, a0.w, a1.w};
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      mma_16x8x16<BF16>(acc[t], f0, b[t].x, b[t].y);
-      mma_16x8x16<BF16>(acc[t], f1, b[t].z, b[t].w);
+    for (int c = 0; c < NT; ++c) {
+      const uint4 a0 = a[2 * c], a1 = a[2 * c + 1];
+      const uint32_t f0[4] = {a0.x, a1.x, a0.y, a1.y}, f1[4] = {a0.z, a1.z, a0.w, a1.w};
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        mma_16x8x16<BF16>(acc[c][t], f0, b[t].x, b[t].y);
+        mma_16x8x16<BF16>(acc[c][t], f1, b[t].z, b[t].w);
+      }
     }
   }
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {  // d[0..1]: column lane / 4, rows 2 (lane & 3) + {0, 1}; d[2..3]: column + 8
-    const int m = t * 8 + (lane & 3) * 2, n = lane / 4;
-    red[kw][m][n] = acc[t][0];
-    red[kw][m + 1][n] = acc[t][1];
-    red[kw][m][n + 8] = acc[t][2];
-    red[kw][m + 1][n + 8] = acc[t][3];
-  }
+  for (int c = 0; c < NT; ++c)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {  // d[0..1]: column lane / 4, rows 2 (lane & 3) + {0, 1}; d[2..3]: column + 8
+      const int m = t * 8 + (lane & 3) * 2, n = c * 16 + lane / 4;
+      red[kw][m][n] = acc[c][t][0];
+      red[kw][m + 1][n] = acc[c][t][1];
+      red[kw][m][n + 8] = acc[c][t][2];
+      red[kw][m + 1][n + 8] = acc[c][t][3];
+    }
   if (CLUSTER) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // 1
   }
   if (CLUSTER) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // 2: this warp's values of T are written
@@ -1125,9 +1132,15 @@ int launch_skinny(Ctx* c, const LoraParams& p) {
   // the SMs.
   int mt = tiles == 1 ? 1 : tiles == 2 ? 2 : 4;
   while (mt > 1 && p.N / 16 * ((tiles + mt - 1) / mt) < c->num_sms) mt /= 2;
-  auto go = [&](auto kern) { launch_k(kern, dim3(p.N / 16, (tiles + mt - 1) / mt), 256, 0, c->stream, p); };
+  auto go = [&](auto kern, int cols = 16) {
+    launch_k(kern, dim3((p.N + cols - 1) / cols, (tiles + mt - 1) / mt), 256, 0, c->stream, p);
+  };
+  // 32 columns per block where enough blocks remain (and T and the sums fit shared memory): X comes from L2 half as often
+  // (64 x 1024 x 4096: 12.7 us, with 16 columns 14.8; 128 x 4096 x 4096: 38.6 and 47.7)
+  const bool wide = mt == 4 && p.r <= 64 && (p.N + 31) / 32 * ((tiles + 3) / 4) >= c->num_sms;
   if (mt == 1) go(lora_skinny_kernel<BF16, 1, false>);
   else if (mt == 2) go(lora_skinny_kernel<BF16, 2, false>);
+  else if (wide) go(lora_skinny_kernel<BF16, 4, false, 2>, 32);
   else go(lora_skinny_kernel<BF16, 4, false>);
   return check_launch(c, "linear_lora");
 }

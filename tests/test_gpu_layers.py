@@ -101,7 +101,7 @@ LORA = [  # M, K, N, r, L
     (16, 640, 640, 128, 5), (33, 192, 176, 40, 33), (64, 1024, 1024, 32, 64), (65, 640, 208, 16, 3),
     (127, 320, 320, 8, 20), (128, 320, 320, 64, 2), (129, 1280, 336, 128, 40), (300, 704, 960, 48, 7),
     (9, 64, 16, 128, 2), (12, 640, 1536, 16, 4), (13, 640, 1552, 16, 4), (25, 320, 1568, 64, 1), (32, 128, 384, 8, 5),
-    (44, 1408, 192, 128, 3), (106, 64, 256, 64, 2), (128, 64, 4096, 128, 7),
+    (44, 1408, 192, 128, 3), (106, 64, 256, 64, 2), (128, 64, 4096, 128, 7), (64, 320, 4784, 64, 5), (33, 128, 2400, 24, 33),
     (1001, 1024, 4096, 64, 6), (2048, 320, 640, 104, 16), (4097, 128, 32, 16, 2), (20000, 320, 320, 32, 8)]
 
 
