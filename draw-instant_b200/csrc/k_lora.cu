@@ -32,7 +32,7 @@
 // 24.2 us.  Neither memory nor the tensor pipe is full: a tile's k blocks, T blocks, zeroing and epilogue hand over to one
 // another some ten times, 150 to 300 ns each (without the epilogue the first takes 29.6 us, with a quarter of the MMAs
 // 40.8).  T as a second kernel's work costs 2.5 to 9 us.
-// Few rows: 8 x 1280 x 1280, rank 16: 4.6 us; 64 x 1024 x 4096, rank 32, 64 adapters: 12.6 us, 2.1 TB/s; bound by the
+// Few rows: 8 x 1280 x 1280, rank 16: 4.6 us; 64 x 1024 x 4096, rank 32, 64 adapters: 12.0 us, 2.3 TB/s; bound by the
 // latency of one pass (two launches, one batch of loads each) and, towards 128 rows, by X from L2 for every 32 columns.
 #include <algorithm>
 #include <cstring>

@@ -411,7 +411,8 @@ CROSS = [  # B, Sq, Skv, H, Hkv, D
     (2, 64, 64, 2, 2, 64), (2, 65, 63, 3, 3, 128), (2, 127, 128, 4, 4, 64), (1, 129, 129, 4, 2, 128), (2, 333, 231, 10, 10, 64),
     (16, 128, 77, 5, 5, 64), (2, 1024, 77, 10, 10, 64), (1, 4096, 20, 5, 5, 64), (1, 500, 2000, 6, 2, 128), (1, 1000, 1, 4, 4, 64),
     (4, 17, 515, 24, 8, 64), (5, 2, 300, 7, 7, 64), (1, 100, 192, 9, 3, 64), (2, 640, 256, 2, 2, 128),
-    (16, 2, 1500, 7, 7, 64), (3, 400, 1700, 8, 1, 64), (7, 77, 1600, 3, 3, 128), (74, 1, 600, 2, 1, 64), (1, 2000, 700, 8, 2, 128)]
+    (16, 2, 1500, 7, 7, 64), (3, 400, 1700, 8, 1, 64), (7, 77, 1600, 3, 3, 128), (74, 1, 600, 2, 1, 64), (1, 2000, 700, 8, 2, 128),
+    (1, 3, 200, 64, 1, 64), (2, 5, 300, 128, 1, 128), (1, 9, 100, 256, 1, 64), (2, 1, 2100, 96, 1, 128), (1, 40, 130, 40, 1, 64)]
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
