@@ -337,14 +337,19 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
   const uint32_t tmem = *tmem_slot;
   // a tile needs its V rows cleaned when it has masked keys inside the tensor (rows past Skv are zero already)
   auto cleaned = [&](const Item& w, int t) { return p.mask || (w.n < p.Skv && w.n - t * KT < KT); };
-  // The next item, or nothing: one thread (or one per warp, the rest following) takes it, done() gives its place back.
+  // The next item, or nothing, for a single thread; done() gives its place back.
   RingPos ip;
-  auto next = [&](int code) -> const Item* {
-    if (!wait_on(&item_full[ip.s], ip.ph, abort_flag, p.err, code)) {
+  auto taken = [&](bool ok) -> const Item* {
+    if (!ok) {
       *abort_flag = 1;
       return nullptr;
     }
     return items[ip.s].rows ? &items[ip.s] : nullptr;
+  };
+  auto next = [&](int code) { return taken(wait_on(&item_full[ip.s], ip.ph, abort_flag, p.err, code)); };
+  // The same for a whole warp: its lanes agree on the wait, as one that left alone would be missing from what follows.
+  auto next_all = [&](int code) {
+    return taken(__all_sync(0xffffffffu, wait_on(&item_full[ip.s], ip.ph, abort_flag, p.err, code)));
   };
   auto done = [&] {
     mbar_arrive_relaxed(&item_empty[ip.s]);
@@ -565,7 +570,7 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
     } else if (svc == 2) {
       RingPos kv;
       bool ok = true;
-      for (const Item* item; ok && (item = next(DEVERR_WAIT_SOFTMAX));) {
+      for (const Item* item; ok && (item = next_all(DEVERR_WAIT_SOFTMAX));) {
         const Item w = *item;
         __syncwarp();
         if (lane == 0) mbar_arrive_relaxed(&item_empty[ip.s]);
@@ -574,9 +579,10 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
           // every tile is waited for, cleaned or not: a wait that runs a whole ring ahead would find the phase before it
           const RingPos k = kv, v = kv.next(p.ring);
           kv = v.next(p.ring);
-          ok = wait_on(&kv_full[k.s], k.ph, abort_flag, p.err, DEVERR_WAIT_SOFTMAX);
+          ok = __all_sync(0xffffffffu, wait_on(&kv_full[k.s], k.ph, abort_flag, p.err, DEVERR_WAIT_SOFTMAX));
+          if (!ok) break;
           if (!cleaned(w, t)) {
-            ok = __all_sync(0xffffffffu, ok && wait_on(&kv_full[v.s], v.ph, abort_flag, p.err, DEVERR_WAIT_SOFTMAX));
+            ok = __all_sync(0xffffffffu, wait_on(&kv_full[v.s], v.ph, abort_flag, p.err, DEVERR_WAIT_SOFTMAX));
             continue;
           }
           const int left = min(w.n - t * KT, KT), reach = (left + 15) / 16 * 16;  // rows that P V reads
@@ -586,7 +592,7 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
             const int j = c * 32 + lane;
             off[c] = __ballot_sync(0xffffffffu, j < reach && (j >= left || (p.mask && !__ldg(p.mask + (long long)w.b * p.Skv + t * KT + j))));
           }
-          ok = __all_sync(0xffffffffu, ok && wait_on(&kv_full[v.s], v.ph, abort_flag, p.err, DEVERR_WAIT_SOFTMAX));
+          ok = __all_sync(0xffffffffu, wait_on(&kv_full[v.s], v.ph, abort_flag, p.err, DEVERR_WAIT_SOFTMAX));
           if (!ok) break;
           uint4* vt = reinterpret_cast<uint4*>(sKV + v.s * C::TILE);
 #pragma unroll
@@ -633,7 +639,7 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
     RingPos q;
     unsigned ph_s = 0, ph_o = 0;
     bool ok = true;
-    for (const Item* item; ok && (item = next(DEVERR_WAIT_SOFTMAX)) != nullptr;) {
+    for (const Item* item; ok && (item = next_all(DEVERR_WAIT_SOFTMAX)) != nullptr;) {
       const Item& w = *item;  // read again where it is used: registers are short here
       const int slot = ip.s;
       ip.advance(kItems);

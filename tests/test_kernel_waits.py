@@ -1,0 +1,80 @@
+"""Rules of the barrier waits in the pipelined layer kernels, read from their source (a wait that goes wrong shows on a
+device only as a hang, so it is looked for here).
+
+A bounded wait may give up in one lane and succeed in its neighbour.  Where a whole warp waits, the lanes therefore agree
+on the result before they act on it: those that left alone would stay away from the warp-wide instructions that follow."""
+from __future__ import annotations
+
+import re
+from pathlib import Path
+
+import pytest
+
+CSRC = Path(__file__).resolve().parents[1] / "draw-instant_b200" / "csrc"
+KERNELS = [("k_xattn.cu", "xattn_kernel")]
+WAIT = re.compile(r"\b(?:wait_on|mbar_wait)(?:<\w+>)?\(")
+
+
+def closing(text, at):
+    """Index of the brace that closes the one at `at`."""
+    depth = 0
+    for i in range(at, len(text)):
+        depth += (text[i] == "{") - (text[i] == "}")
+        if depth == 0:
+            return i
+    raise AssertionError("unbalanced braces")
+
+
+def body(file, name):
+    """A function's text, without comments."""
+    text = re.sub(r"/\*.*?\*/|//[^\n]*", "", (CSRC / file).read_text(), flags=re.S)
+    m = re.search(r"__(?:launch_bounds__\([^{;]*\)|forceinline__)[^{;]*\b%s\([^{;]*\) \{" % name, text)
+    assert m, f"{file}: no {name}"
+    return text[m.end() - 1:closing(text, m.end() - 1) + 1]
+
+
+def one_thread(text):
+    """Spans that a single thread of a warp runs."""
+    heads = re.finditer(r"if \((?:[^;{}]*\belect_one\(\)|lane == 0|threadIdx\.x == 0)\) \{", text)
+    return [(m.start(), closing(text, m.end() - 1)) for m in heads]
+
+
+def inside(spans, at):
+    return any(a <= at <= b for a, b in spans)
+
+
+def statement(text, at):
+    """The statement around `at`, and the one behind it."""
+    start = max(text.rfind(c, 0, at) for c in ";{}") + 1
+    end = text.index(";", at)
+    return text[start:end].strip(), text[end + 1:text.index(";", end + 1)].strip()
+
+
+def unagreed(text):
+    """Waits of a whole warp whose lanes may go on with different results."""
+    alone = one_thread(text)
+    lambdas = [(m.group(1), m.start(), closing(text, m.end() - 1))
+               for m in re.finditer(r"auto (\w+) = \[&\](?:\([^{;]*?\))?(?: -> [\w ]+\*)? \{", text)]
+    bad = []
+    for m in WAIT.finditer(text):
+        if inside(alone, m.start()):
+            continue
+        now, then = statement(text, m.start())
+        if "__all_sync(" in now or WAIT.match(now):  # agreed on at once, or a wait whose result is dropped
+            continue
+        var = re.match(r"(?:const )?(?:bool )?(\w+) = ", now)
+        if var and re.search(r"__all_sync\(0xffffffffu, %s\)" % var.group(1), then):
+            continue
+        around = [n for n, a, b in lambdas if a <= m.start() <= b]
+        calls = [c.start() for n in around for c in re.finditer(r"(?<![.\w])%s\(" % n, text)]
+        if calls and all(inside(alone, c) for c in calls):  # a helper of single threads
+            continue
+        bad.append(now)
+    return bad
+
+
+@pytest.mark.parametrize("file,name", KERNELS)
+def test_a_warps_lanes_agree_on_a_wait(file, name):
+    text = body(file, name)
+    assert len(WAIT.findall(text)) > 0 and len(one_thread(text)) > 0
+    assert unagreed(text) == []
