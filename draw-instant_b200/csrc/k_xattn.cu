@@ -649,6 +649,7 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
       uint64_t* q_done = &q_empty[q.s * NW + (p.by_keys ? 0 : i)];
       if (keys) q.advance(p.nq);
       if (!p.by_keys && i * 128 >= w.rows) {
+        __syncwarp();  // every lane has read the item
         if (lane == 0) mbar_arrive_relaxed(&item_empty[slot]);
         continue;
       }

@@ -78,3 +78,29 @@ def test_a_warps_lanes_agree_on_a_wait(file, name):
     text = body(file, name)
     assert len(WAIT.findall(text)) > 0 and len(one_thread(text)) > 0
     assert unagreed(text) == []
+
+
+# barriers on which a warp gives back the entry of a list or of the items that it has read
+PLACES = re.compile(r"if \((?:any && )?lane == 0\) mbar_arrive(?:_relaxed)?\(&(?:item_empty|list_empty|o_read|d_empty|list_full)\[[^]]*\]\)")
+
+
+def early_releases(text):
+    """Places where lane 0 gives an entry back before the other lanes' reads of it are over."""
+    alone = [s for s in one_thread(text) if not text.startswith("if (lane == 0)", s[0])]
+    bad = []
+    for m in PLACES.finditer(text):
+        if not inside(alone, m.start()) and not re.search(r"__syncwarp\(\);\s*$", text[:m.start()]):
+            bad.append(m.group(0))
+    for m in re.finditer(r"if \(lane == 0\) \{", text):
+        block = text[m.end():closing(text, m.end() - 1)]
+        if re.search(r"_empty\[", block) and not re.search(r"__syncwarp\(\);\s*$", text[:m.start()]):
+            bad.append(block.strip())
+    return bad
+
+
+@pytest.mark.parametrize("file,name", KERNELS)
+def test_a_warp_has_read_what_its_first_lane_gives_back(file, name):
+    """What follows a release may overwrite the entry at once; only a warp barrier orders the other lanes' reads before it."""
+    text = body(file, name)
+    assert PLACES.search(text)
+    assert early_releases(text) == []
