@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + C::DATA);  // [nq][NW] Q tile of group i
   uint64_t* q_empty = q_full + kQBufs * NW;        // [nq][NW]
   uint64_t* kv_full = q_empty + kQBufs * NW;       // [ring]
-  uint64_t* kv_empty = kv_full + C::MAXRING;       // [ring]
+  uint64_t* kv_empty = kv_full + C::MAXRING;       // [ring] products over, and seen by the clean warp
   uint64_t* v_clean = kv_empty + C::MAXRING;       // [ring] V rows of masked keys zeroed
   uint64_t* s_full = v_clean + C::MAXRING;         // [NW] scores ready
   uint64_t* p_full = s_full + NW;                  // [NW][NH] probabilities written
@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
   const int svc = warp - C::SW;  // service warps: 0 MMA, 1 TMA, 2 clean, 3 items
   if (threadIdx.x == 0) {
     for (int i = 0; i < kQBufs * NW; ++i) { mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], p.by_keys ? C::SW : 4); }
-    for (int i = 0; i < p.ring; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); mbar_init(&v_clean[i], 1); }
+    for (int i = 0; i < p.ring; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 2); mbar_init(&v_clean[i], 1); }
     for (int i = 0; i < NW; ++i) {
       mbar_init(&s_full[i], 1);
       for (int h = 0; h < NH; ++h) mbar_init(&p_full[i * NH + h], 4);
@@ -576,13 +576,16 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
         if (lane == 0) mbar_arrive_relaxed(&item_empty[ip.s]);
         ip.advance(kItems);
         for (int t = w.t0; ok && t < w.t1; ++t) {
-          // every tile is waited for, cleaned or not: a wait that runs a whole ring ahead would find the phase before it
+          // Every tile is waited for and given back, cleaned or not: nothing refills it before this warp has seen it, so its
+          // phase here is never more than one behind.
           const RingPos k = kv, v = kv.next(p.ring);
           kv = v.next(p.ring);
           ok = __all_sync(0xffffffffu, wait_on(&kv_full[k.s], k.ph, abort_flag, p.err, DEVERR_WAIT_SOFTMAX));
           if (!ok) break;
+          if (lane == 0) mbar_arrive_relaxed(&kv_empty[k.s]);
           if (!cleaned(w, t)) {
             ok = __all_sync(0xffffffffu, wait_on(&kv_full[v.s], v.ph, abort_flag, p.err, DEVERR_WAIT_SOFTMAX));
+            if (ok && lane == 0) mbar_arrive_relaxed(&kv_empty[v.s]);
             continue;
           }
           const int left = min(w.n - t * KT, KT), reach = (left + 15) / 16 * 16;  // rows that P V reads
@@ -607,7 +610,10 @@ __global__ void __launch_bounds__(XCfg<D, SHORT>::THREADS, 1) xattn_kernel(const
             }
           fence_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&v_clean[v.s]);
+          if (lane == 0) {
+            mbar_arrive(&v_clean[v.s]);
+            mbar_arrive_relaxed(&kv_empty[v.s]);
+          }
         }
       }
       if (!ok) *abort_flag = 1;

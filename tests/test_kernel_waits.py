@@ -5,6 +5,7 @@ A bounded wait may give up in one lane and succeed in its neighbour.  Where a wh
 on the result before they act on it: those that left alone would stay away from the warp-wide instructions that follow."""
 from __future__ import annotations
 
+import random
 import re
 from pathlib import Path
 
@@ -104,3 +105,90 @@ def test_a_warp_has_read_what_its_first_lane_gives_back(file, name):
     text = body(file, name)
     assert PLACES.search(text)
     assert early_releases(text) == []
+
+
+# ---- the ring of key and value tiles --------------------------------------------------------------------------
+
+class Barrier:
+    def __init__(self, count):
+        self.count, self.left, self.done = count, count, 0  # done: phases completed
+
+    def arrive(self):
+        self.left -= 1
+        if self.left == 0:
+            self.left, self.done = self.count, self.done + 1
+
+    def passed(self, parity):
+        return (self.done - 1) % 2 == parity
+
+
+def ring_roles(ring, tiles, masked, counts, cleaner_arrives):
+    """Loader, MMA and cleaning warp of one CTA as generators that yield while they wait; the i-th tile is a K tile for even
+    i and a V tile for odd i.  A tile that is refilled before the cleaning warp has seen it is an error."""
+    full, empty, clean = ([Barrier(n) for _ in range(ring)] for n in counts)
+    holds, seen = [None] * ring, set()
+
+    def loader():
+        for i in range(tiles):
+            s = i % ring
+            while not empty[s].passed((i // ring) % 2 ^ 1):
+                yield
+            assert i < ring or i - ring in seen, "refilled unseen"
+            holds[s] = i
+            full[s].arrive()
+            yield
+
+    def mma():
+        cleaned = [0] * ring
+        for i in range(tiles):
+            s = i % ring
+            while not full[s].passed((i // ring) % 2):
+                yield
+            if i % 2 and masked[i // 2]:
+                while not clean[s].passed(cleaned[s]):
+                    yield
+                cleaned[s] ^= 1
+            assert holds[s] == i
+            empty[s].arrive()
+            yield
+
+    def cleaner():
+        for i in range(tiles):
+            s = i % ring
+            while not full[s].passed((i // ring) % 2):
+                yield
+            assert holds[s] == i, "another tile"
+            seen.add(i)
+            if i % 2 and masked[i // 2]:
+                clean[s].arrive()
+            if cleaner_arrives:
+                empty[s].arrive()
+            yield
+
+    return {"loader": loader(), "mma": mma(), "cleaner": cleaner()}
+
+
+@pytest.mark.parametrize("slow", ["none", "loader", "mma", "cleaner"])
+@pytest.mark.parametrize("ring", [4, 5, 6, 7, 10])
+def test_no_tile_is_refilled_before_every_role_has_seen_it(ring, slow):
+    """The barriers with the kernel's own arrival counts, under schedules that hold one role back as long as they can."""
+    text = body("k_xattn.cu", "xattn_kernel")
+    counts = [int(re.search(r"mbar_init\(&%s\[i\], (\d+)\)" % b, text).group(1)) for b in ("kv_full", "kv_empty", "v_clean")]
+    at = text.index("{", text.index("if (svc == 2)"))
+    arrives = "&kv_empty[" in text[at:closing(text, at)]
+    rng = random.Random(ring)
+    for share in (0.0, 0.3, 1.0):
+        masked = [rng.random() < share for _ in range(40)]
+        roles = ring_roles(ring, 2 * len(masked), masked, counts, arrives)
+        idle = 0
+        while roles:
+            assert idle < 2000, "roles wait for one another"
+            fast = [r for r in roles if r != slow] if idle < 30 else list(roles)  # the slow one only when nothing else moves
+            name = rng.choice(fast or list(roles))
+            before = roles[name].gi_frame.f_locals.get("i")
+            try:
+                next(roles[name])
+                idle = 0 if roles[name].gi_frame.f_locals.get("i") != before else idle + 1
+            except StopIteration:
+                del roles[name]
+                idle = 0
