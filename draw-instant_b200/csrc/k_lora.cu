@@ -843,7 +843,8 @@ __global__ void __launch_bounds__(kLThreads, 1) lora_tile_kernel(const __grid_co
         }
         if (p.R) {
           const int sl = k % kSlabs;
-          ok = wait_on<false>(&rb[sl], (r_ph >> sl) & 1, abort_flag, p.err, DEVERR_WAIT_EPI) && ok;
+          ok = __all_sync(0xffffffffu, wait_on<false>(&rb[sl], (r_ph >> sl) & 1, abort_flag, p.err, DEVERR_WAIT_EPI));
+          if (!ok) break;  // the slab is not there: the copy is waited for once more below
           r_ph ^= 1u << sl;
           const uint4* rp = reinterpret_cast<const uint4*>(slabs + sl * kSlab + lane * 64);  // 64-byte rows, 64-byte swizzle
 #pragma unroll
@@ -876,6 +877,7 @@ __global__ void __launch_bounds__(kLThreads, 1) lora_tile_kernel(const __grid_co
             }
         }
       }
+      if (!ok) break;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
