@@ -14,7 +14,8 @@
 // adapter's B, with the T rows of other adapters zeroed in shared memory.  A tile may so mix adapters at the price of a
 // block each.  (tcgen05.mma's own mask of output lanes would spare the zeroing, but a masked MMA took some 1000 cycles, whatever
 // its width, against 80 to 128 for a plain one.)  Zero times an infinity or NaN in another adapter's B is NaN: outputs
-// that are not finite in a tile of several adapters are computed again from their own row's terms alone.
+// that are not finite in a tile of several adapters are computed again from their own row's terms alone (1001 x 1024 x 4096,
+// rank 64, with every row NaN: 176 us instead of 29).
 // One persistent CTA per SM, or CTA pair (cta_group::2: 256 rows, each CTA loads half of B):
 //   warp 0       TMA loads through one ring of stages
 //   warp 1       MMA issue (the pair's first CTA)
@@ -440,33 +441,67 @@ __global__ void __launch_bounds__(kTThreads, 1) lora_t_kernel(const __grid_const
 // ---- tiles: Y ----
 
 // Out of the way of the epilogue's instructions: the rows of `bad` of a 32 x 32 chunk again, X[m] . W[n] + T[m] . B[a][n] from
-// each row's own terms (lane l computes column n0 + l); lane `row` holds row m0 + row as pairs of columns.
+// each row's own terms; lane `row` holds row m0 + row as pairs of columns.  One request's activations may be NaN
+// in every one of its rows, so 16 rows and columns are taken at a time with mma.sync, where a row's infinities and NaNs
+// stay in it; an adapter's product goes to the rows that name it.
 template <bool BF16>
 __device__ __noinline__ void own_rows(const LoraParams& p, unsigned bad, int m0, int n0, int lane, uint64_t* v) {
-  const int n = min(n0 + lane, p.N - 1);
-  while (bad) {
-    const int row = __ffs(bad) - 1, m = m0 + row, a = __ldg(p.rows + m);
-    bad &= bad - 1;
-    const uint16_t* x = static_cast<const uint16_t*>(p.X) + m * p.ldx;
-    const uint16_t* w = static_cast<const uint16_t*>(p.W) + (long long)n * p.K;
-    float s = 0.f;
-    for (int k = 0; k < p.K; k += 2) {
-      const float2 f = unpack2<BF16>(*reinterpret_cast<const uint32_t*>(x + k));
-      const float2 g = unpack2<BF16>(*reinterpret_cast<const uint32_t*>(w + k));
-      s = fmaf(f.x, g.x, fmaf(f.y, g.y, s));
-    }
-    if (a >= 0 && a < p.L) {
-      const int half = p.r <= 32 ? 32 : 64;
-      const uint16_t* t = p.T16 + (long long)m * p.t_ld;
-      const uint16_t* b = static_cast<const uint16_t*>(p.B) + ((long long)a * p.N + n) * p.r;
-      for (int j = 0; j < p.r; ++j) {
-        const int at = j / half * (2 * half) + j % half;
-        s = fmaf(unpack2<BF16>(t[at]).x + unpack2<BF16>(t[at + half]).x, unpack2<BF16>(b[j]).x, s);
+  // A lane's 16-byte loads of 8 consecutive k stand for two 16-wide MMA steps: both operands use the same order of k.
+  const int at = (lane & 3) * 8;
+  auto add = [](float (&d)[2][4], const uint4& a0, const uint4& a1, const uint4& b0, const uint4& b1) {
+    const uint32_t f0[4] = {a0.x, a1.x, a0.y, a1.y}, f1[4] = {a0.z, a1.z, a0.w, a1.w};
+    mma_16x8x16<BF16>(d[0], f0, b0.x, b0.y);
+    mma_16x8x16<BF16>(d[1], f0, b1.x, b1.y);
+    mma_16x8x16<BF16>(d[0], f1, b0.z, b0.w);
+    mma_16x8x16<BF16>(d[1], f1, b1.z, b1.w);
+  };
+  auto load = [](const uint16_t* q) { return *reinterpret_cast<const uint4*>(q); };
+#pragma unroll 1
+  for (int q = 0; q < 4; ++q) {
+    const int mq = m0 + q / 2 * 16, nq = n0 + q % 2 * 16;
+    unsigned left = (bad >> q / 2 * 16) & 0xffffu;
+    if (!left || nq >= p.N) continue;
+    const int r0 = min(mq + lane / 4, p.M - 1), r1 = min(mq + 8 + lane / 4, p.M - 1);  // rows past the last are not stored
+    const long long n = nq + lane / 4;                                                // and 8 on: N is a multiple of 16
+    float acc[2][4] = {};
+    const uint16_t* x0 = static_cast<const uint16_t*>(p.X) + r0 * p.ldx + at;
+    const uint16_t* x1 = static_cast<const uint16_t*>(p.X) + r1 * p.ldx + at;
+    const uint16_t* w0 = static_cast<const uint16_t*>(p.W) + n * p.K + at;
+    const uint16_t* w1 = w0 + 8ll * p.K;
+#pragma unroll 2
+    for (int k = 0; k < p.K; k += 32) add(acc, load(x0 + k), load(x1 + k), load(w0 + k), load(w1 + k));
+    const int half = p.r <= 32 ? 32 : 64, a0 = __ldg(p.rows + r0), a1 = __ldg(p.rows + r1);
+    const int mine = __ldg(p.rows + min(mq + (lane & 15), p.M - 1));
+    while (left) {  // one adapter of these rows at a time
+      const int a = __shfl_sync(0xffffffffu, mine, __ffs(left) - 1);
+      left &= ~__ballot_sync(0xffffffffu, mine == a);
+      if (a < 0 || a >= p.L) continue;
+      float own[2][4] = {};
+      const uint16_t* b0 = static_cast<const uint16_t*>(p.B) + ((long long)a * p.N + n) * p.r;
+#pragma unroll 1
+      for (int j = at; j < (p.r + 31) / 32 * 32; j += 32) {
+        const uint4 none = make_uint4(0, 0, 0, 0);
+        const bool in = j < p.r;
+        const int col = j / half * (2 * half) + j % half;  // the hi parts of ranks j.., the lo parts `half` on
+        const uint16_t *t0 = p.T16 + (long long)r0 * p.t_ld + col, *t1 = p.T16 + (long long)r1 * p.t_ld + col;
+        const uint4 bj = in ? load(b0 + j) : none, bk = in ? load(b0 + 8 * p.r + j) : none;
+        add(own, in ? load(t0) : none, in ? load(t1) : none, bj, bk);
+        add(own, in ? load(t0 + half) : none, in ? load(t1 + half) : none, bj, bk);
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        if (a0 == a) acc[c][0] += own[c][0], acc[c][1] += own[c][1];
+        if (a1 == a) acc[c][2] += own[c][2], acc[c][3] += own[c][3];
       }
     }
-    for (int e = 0; e < 16; ++e) {
-      const float t0 = __shfl_sync(0xffffffffu, s, 2 * e), t1 = __shfl_sync(0xffffffffu, s, 2 * e + 1);
-      if (lane == row) v[e] = f2_pack(t0, t1);
+    // d[0..1]: row lane / 4, columns 2 (lane & 3) + {0, 1} of 8; d[2..3]: row + 8
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int from = (lane & 7) * 4 + (e & 3);
+      float t[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t[i] = __shfl_sync(0xffffffffu, acc[e / 4][i], from);
+      if ((bad >> lane) & 1 && lane / 16 == q / 2) v[q % 2 * 8 + e] = lane & 8 ? f2_pack(t[2], t[3]) : f2_pack(t[0], t[1]);
     }
   }
 }

@@ -1,0 +1,68 @@
+"""linear_lora, tiles whose rows name several adapters, with rows and adapters that are not finite: every row from its own
+terms alone, and in a bounded time.  Formulas and tolerances are those of test_gpu_layers.py."""
+from __future__ import annotations
+
+import importlib
+
+import pytest
+import torch
+
+from test_gpu_layers import DT, check, lora_case, lora_ref
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def layers(dib):
+    return importlib.import_module("draw_instant_b200.layers")
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("M,per,K,N,r,L", [(129, 1, 64, 16, 8, 3), (300, 7, 320, 336, 24, 5), (257, 40, 192, 96, 72, 4), (700, 77, 640, 560, 128, 6),
+                                           (1001, 33, 128, 2064, 40, 40)])
+def test_rows_beside_those_that_are_not_finite(ctx, layers, M, per, K, N, r, L, dtype):
+    """One request of NaN, an infinity in another's row and two adapters that hold them: only the rows that they reach show
+    it, and the others, computed again, are right with bias, activation and residual."""
+    rows = [(m // per * 5) % (L + 1) - 1 for m in range(M)]
+    s = lora_case(M + r, M, K, N, r, L, DT[dtype], res=True, rows=rows)
+    names = s["row_adapter"]
+    ref, tol = lora_ref(s, "gelu")
+    gone = torch.zeros(M, dtype=torch.bool, device="cuda")
+    s["x"][per:2 * per], gone[per:2 * per] = float("nan"), True
+    s["x"][M - 1, K - 1], gone[M - 1] = float("inf"), True
+    s["b"][1], s["a"][2] = float("inf"), float("nan")
+    gone |= (names == 1) | (names == 2)
+    assert gone.any() and not gone.all()
+    got = layers.linear_lora(ctx, **s, act="gelu")
+    check(got[~gone], ref[~gone], tol[~gone])
+    assert torch.isnan(got[per:2 * per]).all() and torch.isnan(got[names == 2]).all()
+    assert not torch.isfinite(got[names == 1]).any()
+    assert ctx.fault() == 0
+
+
+@pytest.mark.parametrize("M,per,K,N,r,L", [(1001, 77, 1024, 4096, 64, 6), (512, 77, 4096, 4096, 128, 8)])
+def test_rows_that_are_not_finite_do_not_hold_up_the_batch(ctx, layers, M, per, K, N, r, L):
+    """With every row affected, each warp takes its three chunks again in four parts of 16 rows and columns: K / 32 steps of
+    some 600 cycles and a step or two for every adapter, 0.04 to 0.16 ms a chunk for K of 1024 to 4096.  That is four to ten
+    times the batch's 30 to 60 us, and never thirty times."""
+    s = lora_case(1, M, K, N, r, L, torch.bfloat16, rows=[m // per % L for m in range(M)])
+    out = torch.empty(M, N, dtype=torch.bfloat16, device="cuda")
+
+    def time():
+        best = 1e9
+        for _ in range(5):
+            a, b = torch.cuda.Event(True), torch.cuda.Event(True)
+            a.record(ctx.stream)
+            layers.linear_lora(ctx, **s, out=out)
+            b.record(ctx.stream)
+            b.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+
+    torch.cuda.synchronize()
+    clean = time()
+    s["x"].fill_(float("nan"))
+    torch.cuda.synchronize()
+    bad = time()
+    assert torch.isnan(out).all()
+    assert bad < 30 * max(clean, 0.03), f"{bad:.3f} ms, {clean:.3f} without"
