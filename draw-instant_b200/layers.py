@@ -238,8 +238,8 @@ def cross_attention(ctx: Context, q, k, v, kv_len=None, q_len=None, key_mask=Non
     and head-major layouts, slices of fused projections and keys and values expanded over the batch all go in place.
     Key j of request b is valid when j < kv_len[b] and key_mask[b, j] != 0 (kv_len [B] int32, key_mask [B, Skv] uint8 or
     bool, both on the device, None: all); what masked keys and values hold, infinities and NaN included, has no effect.
-    A request without a valid key gives zeros.  Query rows from q_len[b] on (int32) are not computed and
-    their rows of out stay as they were.  scale: positive, 1 / sqrt(D) by default."""
+    A request without a valid key gives zeros.  Query rows from q_len[b] on (int32) are not computed:
+    their rows of out stay as they were, and are zero in a new tensor.  scale: positive, 1 / sqrt(D) by default."""
     if scale is not None and not 0 < scale < float("inf"):
         raise DIError("cross_attention: scale must be positive and finite")
     key = (ctx.device, _sig(q), _sig(k), _sig(v), _sig(kv_len), _sig(q_len), _sig(key_mask), _sig(out))
@@ -251,6 +251,9 @@ def cross_attention(ctx: Context, q, k, v, kv_len=None, q_len=None, key_mask=Non
         scale = default
     if out is None:
         out = _new(ctx, q.shape, q.dtype)
+        if q_len is not None:  # rows that are not computed hold nothing of another tensor's
+            with torch.cuda.stream(ctx.stream):
+                out.zero_()
     ws = _new(ctx, n, torch.uint8) if n else None
     rc = lib().di_cross_attention(ctx.h, code, cfg, scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                                   None if q_len is None else q_len.data_ptr(), None if kv_len is None else kv_len.data_ptr(),
