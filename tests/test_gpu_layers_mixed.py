@@ -40,6 +40,19 @@ def test_rows_beside_those_that_are_not_finite(ctx, layers, M, per, K, N, r, L, 
     assert ctx.fault() == 0
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("M,K,N,r,L", [(256, 320, 336, 16, 256), (300, 128, 64, 128, 300), (513, 64, 32, 8, 400), (192, 640, 2048, 64, 192)])
+def test_every_row_with_an_adapter_of_its_own(ctx, layers, M, K, N, r, L, dtype):
+    """More adapters in a tile than its lists hold entries for, three of 32 adapters or of 256 / rank: the lists are used again
+    and again within one tile."""
+    s = lora_case(M, M, K, N, r, L, DT[dtype], res=M % 2 == 0, rows=[(m * 7 + 3) % L for m in range(M)])
+    first = layers.linear_lora(ctx, **s)
+    check(first, *lora_ref(s))
+    for _ in range(3):
+        assert torch.equal(layers.linear_lora(ctx, **s), first)
+    assert ctx.fault() == 0
+
+
 @pytest.mark.parametrize("M,per,K,N,r,L", [(1001, 77, 1024, 4096, 64, 6), (512, 77, 4096, 4096, 128, 8)])
 def test_rows_that_are_not_finite_do_not_hold_up_the_batch(ctx, layers, M, per, K, N, r, L):
     """With every row affected, each warp takes its three chunks again in four parts of 16 rows and columns: K / 32 steps of
