@@ -64,6 +64,18 @@ struct Ctx {
 
 Ctx* ctx_of(di_ctx_t h);
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// Whether two sets of `rows` rows (of wa and wb 16-bit values, la and lb from one to the next) share memory.  Exact for one
+// row and for equal strides, as of two slices of one buffer; with different strides, whether their ranges meet.
+inline bool rows_meet(const void* a, long long la, long long wa, const void* b, long long lb, long long wb, long long rows) {
+  const long long d = (reinterpret_cast<intptr_t>(b) - reinterpret_cast<intptr_t>(a)) / 2;
+  if (d >= (rows - 1) * la + wa || -d >= (rows - 1) * lb + wb) return false;
+  if (la != lb || rows == 1) return true;
+  // row j of b begins d + (j - i) la past row i of a: the two differences that bring it nearest
+  const long long k = -d / la;
+  for (long long n = k - 1; n <= k + 1; ++n)
+    if (n > -rows && n < rows && d + n * la < wa && d + n * la > -wb) return true;
+  return false;
+}
 // Makes a context's device current for the scope of one call (its stream may be the default stream, which
 // belongs to whichever device is current) and puts the caller's device back.
 struct DeviceGuard {

@@ -1320,6 +1320,9 @@ extern "C" int di_linear_lora(di_ctx_t h, int dtype, const long long cfg[9], con
   if (!aligned16(X) || !aligned16(W) || !aligned16(A) || !aligned16(B) || !aligned16(R) || !aligned16(Y) || ldx % 8 ||
       ldy % 8 || (R && ldr % 8))
     return set_error(c, DI_EINVAL, "linear_lora: pointers must be 16-byte aligned, row strides multiples of 8 elements");
+  // blocks write Y while others still read X, or a residual that is not the same rows of Y
+  if (rows_meet(X, ldx, K, Y, ldy, N, M) || (R && (R != Y || (M > 1 && ldr != ldy)) && rows_meet(R, ldr, N, Y, ldy, N, M)))
+    return set_error(c, DI_EINVAL, "linear_lora: the output shares memory with x, or with a residual other than itself");
   if ((M + 127LL) / 128 * ((N + 31) / 32) > 0x7fffffffll)
     return set_error(c, DI_EUNSUPPORTED, "linear_lora: too many rows and columns");
   const size_t need = di_linear_lora_workspace(h, cfg);

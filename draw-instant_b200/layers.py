@@ -99,7 +99,7 @@ def linear_lora(ctx: Context, x, w, a, b, scale, row_adapter, bias=None, residua
     x [M, K], w [N, K], a [L, r, K], b [L, N, r] (fp16 or bf16), scale [L] fp32, row_adapter [M] int32 on the
     device (negative: no adapter), bias [N] fp32, residual and out [M, N].  K a multiple of 64, N of 16, r of 8 up
     to 128: adapters of other ranks are padded with zeros.  x, residual and out may have a row stride; out may be
-    the residual.  Rows may take the adapters in any order; from some hundred rows on, equal neighbours are fastest.
+    the residual; it shares no other memory with x, the weights or a residual.  Rows may take the adapters in any order; from some hundred rows on, equal neighbours are fastest.
     act: none, silu or gelu, before the residual.  An index past the last adapter sets flag 16 in the context's fault
     word and counts as none.  In fp16, scale * (x a^T) has to stay inside the type's range."""
     key = (ctx.device, act, _sig(x), _sig(w), _sig(a), _sig(b), _sig(scale), _sig(row_adapter), _sig(bias), _sig(residual), _sig(out))

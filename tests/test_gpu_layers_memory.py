@@ -1,0 +1,50 @@
+"""Outputs that share memory with inputs: what a call may do in place, and what it refuses (the checks are the host's: nothing
+is launched)."""
+from __future__ import annotations
+
+import importlib
+
+import pytest
+import torch
+
+from test_gpu_layers import check, lora_case, lora_ref
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def layers(dib):
+    return importlib.import_module("draw_instant_b200.layers")
+
+
+@pytest.mark.parametrize("M", [1, 12, 300])
+def test_lora_refuses_an_output_over_its_input(ctx, dib, layers, M):
+    s = lora_case(M, M, 320, 320, 16, 3, torch.float16)
+    wide = torch.zeros(M + 2, 960, dtype=torch.float16, device="cuda")
+    x = wide[:M, :320]
+    x.copy_(s["x"])
+    s["x"] = x
+    ref = lora_ref(s)
+    bad = [x, wide[:M, 312:632], wide.view(-1)[8:8 + M * 320].view(M, 320)]
+    bad += [wide[1:M + 1, :320], wide.view(-1)[960 - 312:960 - 312 + 960 * M].view(M, 960)[:, :320]] if M > 1 else []
+    for out in bad:
+        with pytest.raises(dib.DIError, match="shares memory"):
+            layers.linear_lora(ctx, **s, out=out)
+    for out in (wide[:M, 320:640], wide[:M, 640:], wide[1:M + 1, 320:640]):  # beside it, or behind the row before
+        check(layers.linear_lora(ctx, **s, out=out), *ref)
+    assert ctx.fault() == 0
+
+
+@pytest.mark.parametrize("M", [1, 12, 300])
+def test_lora_refuses_a_residual_that_is_partly_the_output(ctx, dib, layers, M):
+    s = lora_case(M + 1, M, 320, 320, 16, 3, torch.bfloat16, res=True)
+    ref = lora_ref(s)
+    hold = torch.zeros(M + 1, 640, dtype=torch.bfloat16, device="cuda")
+    y = hold[:M, :320]
+    for other in ([hold[:M, 8:328]] + ([hold[1:, :320]] if M > 1 else [])):
+        with pytest.raises(dib.DIError, match="shares memory"):
+            layers.linear_lora(ctx, **{**s, "residual": other}, out=y)
+    for other in (y, hold[:M, 320:]):
+        other.copy_(s["residual"])
+        check(layers.linear_lora(ctx, **{**s, "residual": other}, out=y), *ref)
+    assert ctx.fault() == 0
