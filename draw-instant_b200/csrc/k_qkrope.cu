@@ -281,6 +281,13 @@ extern "C" int di_qk_norm_rope(di_ctx_t h, int dtype, const long long cfg[14], f
   if (!aligned16(Q) || !aligned16(Qo) || !aligned16(K) || !aligned16(Ko) || ldq % 8 || ldqo % 8 ||
       (Hk && (ldk % 8 || ldko % 8)))
     return set_error(c, DI_EINVAL, "qk_norm_rope: pointers must be 16-byte aligned, strides multiples of 8 elements");
+  // a head is written where it was read, or elsewhere: never over another that is still to be read
+  auto over = [T, D](const void* x, long long ldx, int hx, const void* y, long long ldy, int hy, bool itself) {
+    return hx && hy && !(itself && x == y && (T == 1 || ldx == ldy)) && rows_meet(x, ldx, hx * D, y, ldy, hy * D, T);
+  };
+  if (over(Q, ldq, Hq, Qo, ldqo, Hq, true) || over(K, ldk, Hk, Ko, ldko, Hk, true) || over(Q, ldq, Hq, Ko, ldko, Hk, false) ||
+      over(K, ldk, Hk, Qo, ldqo, Hq, false) || over(Qo, ldqo, Hq, Ko, ldko, Hk, false))
+    return set_error(c, DI_EINVAL, "qk_norm_rope: an output shares memory with the other one, or with an input that is not its own");
   if (pairing != 0 && pairing != 1) return set_error(c, DI_EINVAL, "qk_norm_rope: pairing must be 0 or 1");
   if (!(eps >= 0.f)) return set_error(c, DI_EINVAL, "qk_norm_rope: eps must not be negative");
   QkParams p;

@@ -157,7 +157,7 @@ def qk_norm_rope(ctx: Context, q, k=None, q_weight=None, k_weight=None, eps: flo
     (q_out, k_out), or q_out alone when there is no k.
 
     q [T, Hq, D] and k [T, Hk, D] with D 64 or 128 (fp16 or bf16; tokens may be strided, as in a fused
-    projection; the outputs may be the inputs).  q_weight, k_weight [D] fp32, None: no norm.  positions [P, n] int32
+    projection; q_out may be q and k_out may be k, and they share no other memory with them or each other).  q_weight, k_weight [D] fp32, None: no norm.  positions [P, n] int32
     on the device, token t takes row t % P, None: no rotation.  axis_dims: n = 1 to 3 even dims that sum to D, in
     the positions' order; pair j of axis a turns by positions[., a] * theta^(-2 j / axis_dims[a]).  pairing:
     "interleaved" (values 2i, 2i + 1) or "halves" (values i, i + D / 2)."""

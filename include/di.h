@@ -233,8 +233,8 @@ DI_API int di_linear_lora(di_ctx_t ctx, int dtype, const long long cfg[9], const
  * with Hk = 0: queries only), outputs with ldqo, ldko, heads contiguous, D 64 or 128; weights [D] fp32, NULL: no
  * norm.  positions [pos_rows, n_axes] int32, NULL: no rotation; axis a (1 to 3 of them) owns the next
  * axis_dims[a] / 2 value pairs, even dims that sum to D, and pair j of axis a turns by position *
- * theta^(-2j / axis_dims[a]) radians.  pairing 0: values (2i, 2i + 1); 1: values (i, i + D/2).  The outputs may
- * be the inputs. */
+ * theta^(-2j / axis_dims[a]) radians.  pairing 0: values (2i, 2i + 1); 1: values (i, i + D/2).  Qo may
+ * be Q and Ko may be K, in place; outputs that meet any other tensor's heads are refused. */
 DI_API int di_qk_norm_rope(di_ctx_t ctx, int dtype, const long long cfg[14], float eps, double theta, const void* Q,
                            const void* K, const float* q_weight, const float* k_weight, const int* positions, void* Qo,
                            void* Ko);

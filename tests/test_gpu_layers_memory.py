@@ -7,7 +7,7 @@ import importlib
 import pytest
 import torch
 
-from test_gpu_layers import check, lora_case, lora_ref
+from test_gpu_layers import check, gen, lora_case, lora_ref, normal, qk_ref
 
 pytestmark = pytest.mark.gpu
 
@@ -47,4 +47,27 @@ def test_lora_refuses_a_residual_that_is_partly_the_output(ctx, dib, layers, M):
     for other in (y, hold[:M, 320:]):
         other.copy_(s["residual"])
         check(layers.linear_lora(ctx, **{**s, "residual": other}, out=y), *ref)
+    assert ctx.fault() == 0
+
+
+@pytest.mark.parametrize("T", [1, 50, 3000])
+@pytest.mark.parametrize("D", [64, 128])
+def test_qk_refuses_outputs_over_other_heads(ctx, dib, layers, T, D):
+    g = gen(T)
+    x = normal(g, T + 1, 9, D)
+    w = torch.ones(D, device="cuda")
+    before = x.clone()
+    q, k = x[:T, :3], x[:T, 3:5]
+    bad = [dict(q_out=x[:T, 1:4]), dict(q_out=x[:T, 2:5]), dict(k_out=x[:T, 2:4]), dict(k_out=x[:T, 4:6]), dict(q_out=q, k_out=x[:T, 1:3]),
+           dict(q_out=x[:T, 5:8], k_out=x[:T, 7:9])]
+    bad += [dict(q_out=x[1:, :3]), dict(k_out=x[1:, 4:6])] if T > 1 else []
+    for outs in bad:
+        with pytest.raises(dib.DIError, match="shares memory"):
+            layers.qk_norm_rope(ctx, q, k, q_weight=w, k_weight=w, **outs)
+    torch.cuda.synchronize()
+    assert torch.equal(x, before)
+    y, z = layers.qk_norm_rope(ctx, q, k, q_weight=w, k_weight=w, q_out=q, k_out=x[:T, 5:7])  # in place, and beside
+    check(y, *qk_ref(before[:T, :3], w, 1e-6, None, (), 1.0, "interleaved"))
+    check(z, *qk_ref(before[:T, 3:5], w, 1e-6, None, (), 1.0, "interleaved"))
+    assert torch.equal(x[:T, 3:5], before[:T, 3:5]) and torch.equal(x[:, 7:], before[:, 7:]) and torch.equal(x[T], before[T])
     assert ctx.fault() == 0
