@@ -1104,12 +1104,14 @@ extern "C" int di_cross_attention(di_ctx_t h, int dtype, const long long cfg[18]
     return set_error(c, DI_EUNSUPPORTED, "cross_attention: too many tokens");
   // strides of axes of length one mean nothing: they are replaced by 8 elements (a valid tensor-map stride)
   long long qs[3], ks[3], vs[3], os[3];
+  bool same = true;  // Q and O in one layout
   for (int i = 0; i < 3; ++i) {
     const int nq = i == 0 ? B : i == 1 ? Sq : H, nk = i == 0 ? B : i == 1 ? Skv : Hkv;
     qs[i] = nq > 1 ? q_strides[i] : 8;
     ks[i] = nk > 1 ? k_strides[i] : 8;
     vs[i] = nk > 1 ? v_strides[i] : 8;
     os[i] = nq > 1 ? o_strides[i] : 16;
+    same = same && (nq == 1 || qs[i] == os[i]);
     if (qs[i] < 0 || ks[i] < 0 || vs[i] < 0 || (qs[i] | ks[i] | vs[i] | os[i]) % 8 || os[i] < 0)
       return set_error(c, DI_EINVAL, "cross_attention: strides must be multiples of 8 elements and not negative");
     if (os[i] == 0) return set_error(c, DI_EINVAL, "cross_attention: the output's rows must not share memory");
@@ -1120,6 +1122,9 @@ extern "C" int di_cross_attention(di_ctx_t h, int dtype, const long long cfg[18]
   const size_t need = di_cross_attention_workspace(h, cfg);
   if (need && (!ws || ws_bytes < need || !aligned16(ws)))
     return set_error(c, DI_EINVAL, "cross_attention: workspace missing, too small or not 16-byte aligned");
+  // an item's queries are read before its rows are written, but its keys and values serve other items too
+  if (O == K || O == V || (O == Q && !same))
+    return set_error(c, DI_EINVAL, "cross_attention: the output shares memory with k, v, or queries in another layout");
   XattnParams p;
   memset(&p, 0, sizeof p);
   const CUtensorMapDataType dt = dtype == DI_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;

@@ -239,7 +239,8 @@ def cross_attention(ctx: Context, q, k, v, kv_len=None, q_len=None, key_mask=Non
     Key j of request b is valid when j < kv_len[b] and key_mask[b, j] != 0 (kv_len [B] int32, key_mask [B, Skv] uint8 or
     bool, both on the device, None: all); what masked keys and values hold, infinities and NaN included, has no effect.
     A request without a valid key gives zeros.  Query rows from q_len[b] on (int32) are not computed:
-    their rows of out stay as they were, and are zero in a new tensor.  scale: positive, 1 / sqrt(D) by default."""
+    their rows of out stay as they were, and are zero in a new tensor.  out may be q itself; it shares no other memory with q, k or v.
+    scale: positive, 1 / sqrt(D) by default."""
     if scale is not None and not 0 < scale < float("inf"):
         raise DIError("cross_attention: scale must be positive and finite")
     key = (ctx.device, _sig(q), _sig(k), _sig(v), _sig(kv_len), _sig(q_len), _sig(key_mask), _sig(out))

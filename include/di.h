@@ -243,7 +243,8 @@ DI_API int di_qk_norm_rope(di_ctx_t ctx, int dtype, const long long cfg[14], flo
  * Masked keys and values may hold anything, infinities and NaN included.  A request without valid keys
  * gives zeros; query rows from q_len[b] on (NULL: Sq) are not written.  cfg = {B, H, Hkv, Sq, Skv, D, Q strides
  * {batch, token, head}, K strides, V strides, O strides}: Q, O [B,Sq,H,D], K, V [B,Skv,Hkv,D], H a multiple of Hkv,
- * D 64 or 128 (a stride of 0 expands an input over its batch or heads); scale > 0. */
+ * D 64 or 128 (a stride of 0 expands an input over its batch or heads); scale > 0.  O may be Q with the same strides
+ * (in place) and shares no other memory with Q, K or V. */
 DI_API size_t di_cross_attention_workspace(di_ctx_t ctx, const long long cfg[18]);
 DI_API int di_cross_attention(di_ctx_t ctx, int dtype, const long long cfg[18], float scale, const void* Q, const void* K,
                               const void* V, void* O, const int* q_len, const int* kv_len, const unsigned char* key_mask,

@@ -7,7 +7,7 @@ import importlib
 import pytest
 import torch
 
-from test_gpu_layers import check, gen, lora_case, lora_ref, normal, qk_ref
+from test_gpu_layers import check, cross_ref, gen, lora_case, lora_ref, normal, qk_ref
 
 pytestmark = pytest.mark.gpu
 
@@ -71,3 +71,31 @@ def test_qk_refuses_outputs_over_other_heads(ctx, dib, layers, T, D):
     check(z, *qk_ref(before[:T, 3:5], w, 1e-6, None, (), 1.0, "interleaved"))
     assert torch.equal(x[:T, 3:5], before[:T, 3:5]) and torch.equal(x[:, 7:], before[:, 7:]) and torch.equal(x[T], before[T])
     assert ctx.fault() == 0
+
+
+@pytest.mark.parametrize("B,Sq,Skv,H,Hkv,D", [(3, 500, 77, 5, 5, 64), (2, 700, 400, 4, 2, 128), (16, 1, 1500, 8, 2, 128), (7, 130, 1600, 3, 3, 64)])
+def test_cross_in_place_of_the_queries(ctx, layers, B, Sq, Skv, H, Hkv, D):
+    """Many queries, ragged ones, and keys shared out over the card: the queries lie in a wider buffer and become the result."""
+    g = gen(Sq)
+    hold = normal(g, B, Sq, H + 2, D)
+    before = hold.clone()
+    q, k, v = hold[:, :, 1:-1], normal(g, B, Skv, Hkv, D), normal(g, B, Skv, Hkv, D)
+    q_len = torch.tensor([max(1, Sq - 3 * i) for i in range(B)], dtype=torch.int32, device="cuda")
+    ref = cross_ref(q.contiguous(), k, v, None, q_len, None, None, q.contiguous())
+    layers.cross_attention(ctx, q, k, v, q_len=q_len, out=q)
+    check(q, *ref)
+    assert torch.equal(hold[:, :, 0], before[:, :, 0]) and torch.equal(hold[:, :, -1], before[:, :, -1])
+    assert ctx.fault() == 0
+
+
+@pytest.mark.parametrize("Sq", [1, 40])
+def test_cross_refuses_an_output_over_keys_and_values(ctx, dib, layers, Sq):
+    g = gen(Sq)
+    q, kv = normal(g, 3, Sq, 4, 64), normal(g, 3, Sq, 2, 4, 64)
+    for out in (kv[:, :, 0], kv[:, :, 1]):
+        with pytest.raises(dib.DIError, match="shares memory"):
+            layers.cross_attention(ctx, q, kv[:, :, 0], kv[:, :, 1], out=out)
+    other = q.view(3, 4, Sq, 64).transpose(1, 2)  # the queries' memory in another order
+    if Sq > 1:
+        with pytest.raises(dib.DIError, match="shares memory"):
+            layers.cross_attention(ctx, q, kv[:, :, 0], kv[:, :, 1], out=other)
