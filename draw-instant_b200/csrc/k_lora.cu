@@ -28,8 +28,8 @@
 // launch streams W into mma.sync fragments (16 weight rows by 8 rows of X) and adds the rows' own B products with plain
 // FMAs: every byte of W, A and B comes from memory once, whoever owns it.
 //
-// Bound and measured (graph replays).  Tiles: 65536 x 320 x 320, rank 32, residual, fp16: 40.9 us, 3.1 TB/s (the shared
-// product alone 33); 16384 x 640 x 1920, rank 16: 48 us, 860 TFLOP/s; 1001 x 1024 x 4096, rank 64, six adapters, gelu:
+// Bound and measured (graph replays).  Tiles: 65536 x 320 x 320, rank 32, residual, fp16: 40.6 us, 3.1 TB/s (the shared
+// product alone 33); 16384 x 640 x 1920, rank 16: 49 us, 845 TFLOP/s; 1001 x 1024 x 4096, rank 64, six adapters, gelu:
 // 24.2 us.  Neither memory nor the tensor pipe is full: a tile's k blocks, T blocks, zeroing and epilogue hand over to one
 // another some ten times, 150 to 300 ns each (without the epilogue the first takes 29.6 us, with a quarter of the MMAs
 // 40.8).  T as a second kernel's work costs 2.5 to 9 us.
@@ -1143,10 +1143,11 @@ __global__ void __launch_bounds__(CLUSTER ? 512 : 256) lora_skinny_kernel(const 
 }
 
 // Few rows in one launch: row tiles of 8 per block, or 0 for two launches.  Each cluster of eight blocks (128 columns)
-// works out T of its rows itself; up to 12 clusters find room at once (16 took twice the time of 10).  It saves a launch,
-// 5 us of a caller's time, and costs the GPU 1 us up to 256 values of T (8 x 1280 x 1280, rank 16: 5.5 us against 4.5;
-// with 1024 values 10 against 7).
-int one_launch(long long M, long long N, long long K, long long r) {
+// works out T of its rows itself; up to 12 clusters find room at once (16 took twice the time of 10).  It saves a launch
+// and the scratch, 5 us of a caller's time (8 x 1280 x 1280, rank 16: 8.4 us a call against 13.5), and costs the GPU up to 2 us
+// at 256 values of T (in a graph, rank 16: 4.5 us against 4.1, rank 32: 6.1 against 4.3; 16 x 640 x 640, rank 16: 3.7 against
+// 3.9; with 512 values 9.3 against 5.2).
+int one_launch(long long M, long long N, long long r) {
   const long long tiles = (M + 7) / 8, columns = (N + 127) / 128;
   for (int mt = 1; mt <= 4; mt *= 2)
     if (columns * ((tiles + mt - 1) / mt) <= 12) return std::min<long long>(M, 8 * mt) * r <= 256 ? mt : 0;
@@ -1156,7 +1157,7 @@ int one_launch(long long M, long long N, long long K, long long r) {
 template <bool BF16>
 int launch_skinny(Ctx* c, const LoraParams& p) {
   const int tiles = (p.M + 7) / 8;
-  if (const int mt = one_launch(p.M, p.N, p.K, p.r)) {
+  if (const int mt = one_launch(p.M, p.N, p.r)) {
     const dim3 grid((p.N + 127) / 128 * 8, (tiles + mt - 1) / mt);
     auto kern = mt == 1 ? lora_skinny_kernel<BF16, 1, true> : mt == 2 ? lora_skinny_kernel<BF16, 2, true> : lora_skinny_kernel<BF16, 4, true>;
     launch_k_cluster(kern, grid, 512, 0, c->stream, 8, p);
@@ -1297,7 +1298,7 @@ bool fits_int(const long long* v, int n) {
 extern "C" size_t di_linear_lora_workspace(di_ctx_t h, const long long cfg[9]) {
   if (!h || !cfg || !fits_int(cfg, 5)) return 0;
   const size_t M = cfg[0], rank = cfg[3];
-  if (M <= (size_t)kSkinnyRows) return one_launch(cfg[0], cfg[1], cfg[2], cfg[3]) ? 0 : M * rank * 4;
+  if (M <= (size_t)kSkinnyRows) return one_launch(cfg[0], cfg[1], cfg[3]) ? 0 : M * rank * 4;
   return M * (rank <= 32 ? 64 : (rank + 63) / 64 * 128) * 2;
 }
 

@@ -12,7 +12,8 @@
 // heads, queries then keys: a lane owns the same 8-value chunk of every head of one token, with the weights times the
 // sines and cosines of its pairs in registers, and all traffic is whole 128-byte lines.  Loads run four steps ahead, and
 // two steps go side by side: their shuffles and roots hide one another (65536 tokens of 5 + 5 heads of 64, fp16: 33.8 us,
-// 5.0 TB/s; one at a time 38.7.  21600 tokens of 16 + 4 heads of 128, bf16: 41.6 us, 5.3 TB/s; 45.8).
+// 5.0 TB/s; one at a time 38.7.  21600 tokens of 16 + 4 heads of 128, bf16: 41.5 us, 5.3 TB/s; 45.8).  Rotated halves
+// exchange all values by shuffles (eight per 16 bytes) and run five blocks per SM instead of six: 40.0 and 45.4 us.
 // The angle is the product of an integer position and a 64-bit frequency in turns, reduced to half a turn in 64 bits
 // before the 32-bit sine (absolute error 2^-20.9): positions of any size keep the accuracy of position zero.
 // Sums and products are 32-bit; the result is rounded once.

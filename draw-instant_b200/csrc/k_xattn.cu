@@ -19,8 +19,11 @@
 // group's products run while the others' exponentials do.  MMAs of the one issuing thread execute in order: S of the next
 // key tile may follow P V into the same columns, and its commit also tells that P V is complete.  The running maximum
 // only moves when a row's true maximum passes it by 2^8, so O is rarely rescaled and P stays below 2^8, in range of both
-// types; O / l is exact under the stale maximum.  P is rounded to the inputs' 16-bit type for the second product (half a
-// step per probability, averaged over the keys); scores, maxima, sums and O are 32-bit.
+// types; O / l is exact under the stale maximum.  Scores, maxima, sums and O are 32-bit.  P is rounded to the inputs' 16-bit
+// type for the second product, half a step per probability: the roundings of a row's keys are independent, but O shrinks
+// with the number of keys as they do, so O carries the error of one more rounding beside its own, up to 1.4 times the
+// error of a result that is rounded once (measured against 64 bits, bf16 2.3e-3 and 1.7e-3, fp16 2.7e-4 and 2.1e-4).  A second
+// 16-bit part of P would remove it for a second P V, half as many MMAs again.
 //
 // Work, by rows: an item is up to NW tiles of 128 rows of one (request, head group), which share its key tiles.
 // Work, by keys (too few rows for the SMs): an item is a range of key tiles of one tile of rows; the key tiles of all
@@ -35,11 +38,11 @@
 // O of a warp whose 32 rows are all to be written goes through shared memory (the group's Q tile, which is spent) and a TMA
 // store; ragged rows are stored from registers.
 //
-// Bound and measured (graph replays).  Long, 2 x 8 heads (4 of keys), 4096 queries, 8191 keys, head dim 128, bf16: 238 us,
-// 1060 TFLOP/s.  A key tile of both groups takes 3600 cycles, of which the MMAs need 2048 and the exponentials as many;
+// Bound and measured (graph replays).  Long, 2 x 8 heads (4 of keys), 4096 queries, 8191 keys, head dim 128, bf16: 241 us,
+// 1050 TFLOP/s (16 heads, 8 of keys, of 64: 428 us).  A key tile of both groups takes 3600 cycles, of which the MMAs need 2048 and the exponentials as many;
 // the rest is each group's chain of score wait, maximum, exponentials and P V, and 256 items on 148 SMs make two rounds
-// of 1.73.  Short, 16 x 5 heads, 4096 queries, 77 keys, head dim 64, fp16: 25.1 us, 3.4 TB/s, the same chain once per item.
-// By keys, 16 x 16 heads (4 of keys), one query, 8192 keys: 39.3 us, 4.2 TB/s, six of them the second kernel's.
+// of 1.73.  Short, 16 x 5 heads, 4096 queries, 77 keys, head dim 64, fp16: 26.0 us, 3.3 TB/s, the same chain once per item.
+// By keys, 16 x 16 heads (4 of keys), one query, 8192 keys: 39.8 us, 4.1 TB/s, six of them the second kernel's.
 #include <algorithm>
 #include <cstring>
 

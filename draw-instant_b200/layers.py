@@ -239,7 +239,9 @@ def cross_attention(ctx: Context, q, k, v, kv_len=None, q_len=None, key_mask=Non
     Key j of request b is valid when j < kv_len[b] and key_mask[b, j] != 0 (kv_len [B] int32, key_mask [B, Skv] uint8 or
     bool, both on the device, None: all); what masked keys and values hold, infinities and NaN included, has no effect.
     A request without a valid key gives zeros.  Query rows from q_len[b] on (int32) are not computed:
-    their rows of out stay as they were, and are zero in a new tensor.  out may be q itself; it shares no other memory with q, k or v.
+    their rows of out stay as they were, and are zero in a new tensor.  The
+    probabilities are rounded to the tensors' type for the product with v, all else is held in 32 bits: for ordinary values
+    the result is off by up to 1.4 times its own rounding.  out may be q itself; it shares no other memory with q, k or v.
     scale: positive, 1 / sqrt(D) by default."""
     if scale is not None and not 0 < scale < float("inf"):
         raise DIError("cross_attention: scale must be positive and finite")

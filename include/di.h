@@ -241,7 +241,8 @@ DI_API int di_qk_norm_rope(di_ctx_t ctx, int dtype, const long long cfg[14], flo
 /* Attention over an encoder's states: O = softmax(scale * Q K^T) V over each request's valid keys: j <
  * kv_len[b] (NULL: Skv; values outside [0, Skv] are clamped) and key_mask[b * Skv + j] != 0 (NULL: all).
  * Masked keys and values may hold anything, infinities and NaN included.  A request without valid keys
- * gives zeros; query rows from q_len[b] on (NULL: Sq) are not written.  cfg = {B, H, Hkv, Sq, Skv, D, Q strides
+ * gives zeros; query rows from q_len[b] on (NULL: Sq) are not written.  Scores, sums and the result are held in 32 bits,
+ * the probabilities in `dtype` for the product with V: O is off by up to 1.4 times the rounding of the result.  cfg = {B, H, Hkv, Sq, Skv, D, Q strides
  * {batch, token, head}, K strides, V strides, O strides}: Q, O [B,Sq,H,D], K, V [B,Skv,Hkv,D], H a multiple of Hkv,
  * D 64 or 128 (a stride of 0 expands an input over its batch or heads); scale > 0.  O may be Q with the same strides
  * (in place) and shares no other memory with Q, K or V. */
