@@ -70,7 +70,7 @@ inline bool rows_meet(const void* a, long long la, long long wa, const void* b, 
   const long long d = (reinterpret_cast<intptr_t>(b) - reinterpret_cast<intptr_t>(a)) / 2;
   if (d >= (rows - 1) * la + wa || -d >= (rows - 1) * lb + wb) return false;
   if (la != lb || rows == 1) return true;
-  // row j of b begins d + (j - i) la past row i of a: the two differences that bring it nearest
+  // row j of b begins d + (j - i) la past row i of a: the differences that bring it nearest
   const long long k = -d / la;
   for (long long n = k - 1; n <= k + 1; ++n)
     if (n > -rows && n < rows && d + n * la < wa && d + n * la > -wb) return true;

@@ -476,7 +476,7 @@ __device__ __noinline__ void own_rows(const LoraParams& p, unsigned bad, int m0,
       const int a = __shfl_sync(0xffffffffu, mine, __ffs(left) - 1);
       left &= ~__ballot_sync(0xffffffffu, mine == a);
       if (a < 0 || a >= p.L) continue;
-      float own[2][4] = {};
+      float own[2][4] = {}, low[2][4] = {};  // of T's hi and lo parts
       const uint16_t* b0 = static_cast<const uint16_t*>(p.B) + ((long long)a * p.N + n) * p.r;
 #pragma unroll 1
       for (int j = at; j < (p.r + 31) / 32 * 32; j += 32) {
@@ -486,13 +486,13 @@ __device__ __noinline__ void own_rows(const LoraParams& p, unsigned bad, int m0,
         const uint16_t *t0 = p.T16 + (long long)r0 * p.t_ld + col, *t1 = p.T16 + (long long)r1 * p.t_ld + col;
         const uint4 bj = in ? load(b0 + j) : none, bk = in ? load(b0 + 8 * p.r + j) : none;
         add(own, in ? load(t0) : none, in ? load(t1) : none, bj, bk);
-        add(own, in ? load(t0 + half) : none, in ? load(t1 + half) : none, bj, bk);
+        add(low, in ? load(t0 + half) : none, in ? load(t1 + half) : none, bj, bk);
       }
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        if (a0 == a) acc[c][0] += own[c][0], acc[c][1] += own[c][1];
-        if (a1 == a) acc[c][2] += own[c][2], acc[c][3] += own[c][3];
-      }
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)  // an infinity of the hi parts stands: a lo part of zero or of the other sign would make it NaN
+          if ((i < 2 ? a0 : a1) == a) acc[c][i] += isinf(own[c][i]) ? own[c][i] : own[c][i] + low[c][i];
     }
     // d[0..1]: row lane / 4, columns 2 (lane & 3) + {0, 1} of 8; d[2..3]: row + 8
 #pragma unroll

@@ -41,6 +41,25 @@ def test_rows_beside_those_that_are_not_finite(ctx, layers, M, per, K, N, r, L, 
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("M,r", [(60, 16), (300, 16), (300, 104)])
+def test_an_infinity_in_an_adapter_stays_one(ctx, layers, M, r, dtype):
+    """One infinite value of B: the column of the rows that name the adapter is infinite, with the sign of the inner value."""
+    s = lora_case(r, M, 320, 48, r, 3, DT[dtype], rows=[m // 7 % 3 for m in range(M)])
+    s["b"][1, 5, 3] = float("inf")
+    mine = s["row_adapter"] == 1
+    t = s["x"].double() @ s["a"][1, 3].double()
+    clear = mine & (t.abs() > 1e-2)
+    assert clear.sum() > 10
+    got = layers.linear_lora(ctx, **s)
+    assert torch.equal(got[clear, 5].double(), t[clear].sign() * float("inf"))
+    s["b"][1, 5, 3] = 0
+    ref, tol = lora_ref(s)
+    other = torch.arange(48, device="cuda") != 5
+    check(got[:, other], ref[:, other], tol[:, other])
+    check(got[~mine], ref[~mine], tol[~mine])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("M,K,N,r,L", [(256, 320, 336, 16, 256), (300, 128, 64, 128, 300), (513, 64, 32, 8, 400), (192, 640, 2048, 64, 192)])
 def test_every_row_with_an_adapter_of_its_own(ctx, layers, M, K, N, r, L, dtype):
     """More adapters in a tile than its lists hold entries for, three of 32 adapters or of 256 / rank: the lists are used again
