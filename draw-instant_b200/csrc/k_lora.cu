@@ -15,7 +15,8 @@
 // block each.  (tcgen05.mma's own mask of output lanes would spare the zeroing, but a masked MMA took some 1000 cycles, whatever
 // its width, against 80 to 128 for a plain one.)  Zero times an infinity or NaN in another adapter's B is NaN: outputs
 // that are not finite in a tile of several adapters are computed again from their own row's terms alone (1001 x 1024 x 4096,
-// rank 64, with every row NaN: 176 us instead of 29).
+// rank 64, with every row NaN: 180 us instead of 29).  In a tile of one adapter they stand: an infinity in its B may come
+// out as NaN there, T's two parts having signs of their own.
 // One persistent CTA per SM, or CTA pair (cta_group::2: 256 rows, each CTA loads half of B):
 //   warp 0       TMA loads through one ring of stages
 //   warp 1       MMA issue (the pair's first CTA)

@@ -222,7 +222,8 @@ DI_API int di_attention_causal(di_ctx_t ctx, int dtype, const void* Q, const voi
  * act}: X [M,K] rows ldx, W [N,K], A [n_adapters,rank,K], B [n_adapters,N,rank], scale [n_adapters] and bias
  * [N] (may be NULL) fp32, R [M,N] rows ldr (may be NULL, may be Y), Y rows ldy, in memory of its own otherwise (rows that meet
  * those of X, or of an R that is not Y, are refused); act as in di_linear_act.  K a multiple of 64, N of 16, rank of 8 up to 128 (pad adapters of other ranks with zeros).  In fp16,
- * scale * (X . A^T) has to stay inside the type's range. */
+ * scale * (X . A^T) has to stay inside the type's range.  Infinities and NaNs of an adapter reach only the rows that
+ * name it (as infinities or NaNs). */
 DI_API size_t di_linear_lora_workspace(di_ctx_t ctx, const long long cfg[9]);
 DI_API int di_linear_lora(di_ctx_t ctx, int dtype, const long long cfg[9], const void* X, const void* W, const void* A,
                           const void* B, const float* scale, const int* row_adapter, const float* bias, const void* R,
